@@ -67,7 +67,8 @@ const char* neus2b_version(void);
 uint64_t neus2b_launch_count(void);
 const char* neus2b_error_string(int code);
 /* sizeof of the structures of this header as the loaded library was compiled, in header order: grid_desc, motion, pcg32, dataset,
- * train_cfg, ray_workspace, adam_cfg, testbed_config, train_stats, render_cfg, render_workspace, render_request, training_state.
+ * train_cfg, ray_workspace, adam_cfg, testbed_config, train_stats, render_cfg, render_workspace, render_request, training_state,
+ * linear_desc, layer_norm_desc, grad_tensor.
  * Writes at most `capacity` entries and returns how many there are; a binding compares them with its own before it passes a pointer. */
 uint32_t neus2b_abi_struct_sizes(uint32_t* sizes, uint32_t capacity);
 
@@ -356,6 +357,98 @@ int neus2b_adam_step_packed(const neus2b_adam_cfg* cfg, uint64_t n, float* d_gra
  * cleared.  d_grad_out (optional, float[12]) receives the gradients; with d_master == NULL only they are computed. */
 int neus2b_delta_optimizer_step(const neus2b_adam_cfg* cfg, float* d_sums, float* d_master, float* d_m, float* d_v, uint16_t* d_delta,
                                 uint16_t* d_delta_ema, float* d_ema_master, float* d_grad_out, neus2b_stream_t stream);
+
+/* ---------------------------------------------------------------- layers of any width (no counterpart in the reference) */
+
+/* The MLP kernels above are built for 64 neurons.  These are a linear layer and a layer norm of any width, forward and backward,
+ * for networks beside them.  Values are fp16 or bf16 (layer norm: fp32 too), sums and statistics fp32.  Matrices are row-major,
+ * one sample per row, rows a caller-given number of ENTRIES apart (*_stride, at least the width; entries of a row are contiguous).
+ * Any width, stride and entry-aligned address is taken; rows that start on 16-byte boundaries are faster.  n == 0 is allowed.
+ * Outputs may not overlap inputs unless a comment says so.  Parameter gradients are fp32 and follow grad_mode
+ * (NEUS2B_GRAD_*, IGNORE: the pointers are not used).  Every sum has a fixed order: the same call gives the same bits. */
+#define NEUS2B_F32 0
+#define NEUS2B_F16 1
+#define NEUS2B_BF16 2
+
+#define NEUS2B_ACT_NONE 0
+#define NEUS2B_ACT_RELU 1 /* max(z, 0); slope 0 at z = 0 */
+#define NEUS2B_ACT_GELU 2 /* z s(2u), u = sqrt(2/pi) (z + 0.044715 z^3), s the logistic function: the tanh form */
+#define NEUS2B_ACT_SILU 3 /* z s(z) */
+
+typedef struct {
+	uint32_t n;          /* samples */
+	uint32_t in_width, out_width;
+	uint32_t dtype;      /* NEUS2B_F16 or NEUS2B_BF16: x, W, bias, residual, y, z and their gradients */
+	uint32_t activation; /* NEUS2B_ACT_* */
+} neus2b_linear_desc;
+
+/* z = x W^T + bias, y = act(z) + residual.  d_x [n][in_width], d_w [out_width][in_width] (rows contiguous), d_bias [out_width] or
+ * NULL, d_residual [n][out_width] or NULL, d_y [n][out_width], d_preact [n][out_width] or NULL: receives z, which the backward
+ * pass of an activated layer reads.  The sum and the epilogue are fp32, y and z are rounded once.  d_residual may be d_y. */
+int neus2b_linear_forward(const neus2b_linear_desc* desc, const void* d_x, uint64_t x_stride, const void* d_w, const void* d_bias,
+                          const void* d_residual, uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_preact,
+                          uint64_t preact_stride, neus2b_stream_t stream);
+
+/* The backward pass.  With dz = dL/dy * act'(z):
+ *   d_dL_dx [n][in_width] = (dz W) * act_below'(z_below) + skip      (NULL: not computed)
+ *   d_wgrad [out_width][in_width] (+)= dz^T x, d_bgrad [out_width] (+)= sum over n of dz     (either may be NULL)
+ * d_preact: z of this layer, read when desc->activation is not NONE; dz is then rounded to the layer's type in the workspace.
+ * below_activation, d_below_preact: what the layer below applied to get x, so that d_dL_dx is already the gradient of that layer's
+ * z and the chain needs no pass of its own over it (NEUS2B_ACT_NONE and NULL: plain dL/dx).  d_skip [n][in_width] or NULL: the
+ * gradient that reaches x around this layer (a residual connection); it may be d_dL_dx.
+ * d_workspace: neus2b_linear_backward_workspace bytes, 16-byte aligned; nothing in it is kept between calls.  Calls that may run
+ * at the same time need workspaces of their own. */
+int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, uint64_t* bytes);
+int neus2b_linear_backward(const neus2b_linear_desc* desc, const void* d_x, uint64_t x_stride, const void* d_w, const void* d_preact,
+                           uint64_t preact_stride, const void* d_dL_dy, uint64_t dy_stride, uint32_t below_activation,
+                           const void* d_below_preact, uint64_t below_stride, const void* d_skip, uint64_t skip_stride, void* d_dL_dx,
+                           uint64_t dx_stride, float* d_wgrad, float* d_bgrad, int grad_mode, void* d_workspace,
+                           uint64_t workspace_bytes, neus2b_stream_t stream);
+
+typedef struct {
+	uint32_t n, width;
+	uint32_t dtype;       /* NEUS2B_F32, _F16, _BF16: x, y and their gradients */
+	uint32_t param_dtype; /* of gamma and beta: NEUS2B_F32 or the same as dtype */
+	float epsilon;        /* > 0 */
+} neus2b_layer_norm_desc;
+
+/* y = gamma (x - mean) rstd + beta over each row, rstd = 1 / sqrt(var + epsilon), var the mean square of x - mean.  d_beta may be
+ * NULL (0); d_mean and d_rstd (fp32 [n], both or neither) receive the statistics for the backward pass.  d_y may be d_x. */
+int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, const void* d_x, uint64_t x_stride, const void* d_gamma, const void* d_beta,
+                              void* d_y, uint64_t y_stride, float* d_mean, float* d_rstd, neus2b_stream_t stream);
+/* d_dL_dx = rstd (a - mean(a) - xhat mean(a xhat)) + skip with a = gamma dL/dy, xhat = (x - mean) rstd; d_dgamma (+)= sum over n of
+ * dL/dy xhat, d_dbeta (+)= sum over n of dL/dy.  d_dL_dx, d_dgamma, d_dbeta, d_skip may each be NULL; d_dL_dx may be d_dL_dy or d_skip.
+ * The workspace is like that of neus2b_linear_backward. */
+int neus2b_layer_norm_backward_workspace(const neus2b_layer_norm_desc* desc, uint64_t* bytes);
+int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, const void* d_x, uint64_t x_stride, const void* d_gamma, const float* d_mean,
+                               const float* d_rstd, const void* d_dL_dy, uint64_t dy_stride, const void* d_skip, uint64_t skip_stride,
+                               void* d_dL_dx, uint64_t dx_stride, float* d_dgamma, float* d_dbeta, int grad_mode, void* d_workspace,
+                               uint64_t workspace_bytes, neus2b_stream_t stream);
+
+/* ---- global norm of a set of gradient tensors, and clipping by it (ahead of neus2b_adam_step) */
+typedef struct {
+	const void* d_in; /* gradients, contiguous, n entries */
+	void* d_out;      /* where the clipped gradients go: d_in for in place, a buffer of the same type, or NULL (norm only) */
+	uint64_t n;
+	uint32_t dtype;   /* NEUS2B_F32, _F16, _BF16 */
+} neus2b_grad_tensor;
+/* Host only: cuts the tensors into pieces for the kernels and writes the table of pieces to h_table (NULL: only its size in bytes and
+ * the number of pieces are returned).  The caller copies the table to device memory once and keeps it as long as the buffers stay
+ * where they are; any number of tensors, empty ones included.  Outputs that overlap each other, or an input other than their own
+ * tensor's in place, are refused (when the table is written). */
+int neus2b_grad_table(const neus2b_grad_tensor* h_tensors, uint32_t n_tensors, void* h_table, uint64_t* table_bytes, uint32_t* n_pieces);
+#define NEUS2B_NORM_SKIP_NONFINITE 1u /* leave NaN and infinite entries out of the norm (neus2b_adam_step does not use them either) */
+/* d_result[0] = N = |scale| * sqrt(sum of g^2), d_result[1] = c = max_norm / N where N is finite and above max_norm, else 1.  `scale` is for
+ * gradients that carry a loss scale (1 / loss_scale).  d_nonfinite (uint32, optional): the number of NaN and infinite entries is
+ * ADDED.  Squares are summed in fp64: no overflow or underflow on the way.  d_workspace: neus2b_grad_norm_workspace bytes, 16-byte
+ * aligned, nothing in it is kept. */
+uint64_t neus2b_grad_norm_workspace(uint32_t n_pieces);
+int neus2b_grad_norm(const void* d_table, uint32_t n_pieces, float scale, float max_norm, uint32_t flags, float* d_result,
+                     uint32_t* d_nonfinite, void* d_workspace, uint64_t workspace_bytes, neus2b_stream_t stream);
+/* neus2b_grad_norm, then out = c * g for every tensor that has a d_out (fp32 product, rounded once).  In place and c == 1: nothing is
+ * rewritten.  The outputs keep the gradients' loss scale. */
+int neus2b_grad_clip(const void* d_table, uint32_t n_pieces, float scale, float max_norm, uint32_t flags, float* d_result,
+                     uint32_t* d_nonfinite, void* d_workspace, uint64_t workspace_bytes, neus2b_stream_t stream);
 
 /* ---------------------------------------------------------------- training loop (Testbed, src/testbed.cu / src/testbed_nerf.cu) */
 

@@ -75,6 +75,23 @@ class AdamCfg(C.Structure):
                 ("n_matrix", C.c_uint32), ("flags", C.c_uint32), ("d_nonfinite", C.c_void_p)]
 
 
+class LinearDesc(C.Structure):
+    _fields_ = [("n", C.c_uint32), ("in_width", C.c_uint32), ("out_width", C.c_uint32), ("dtype", C.c_uint32), ("activation", C.c_uint32)]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [("n", C.c_uint32), ("width", C.c_uint32), ("dtype", C.c_uint32), ("param_dtype", C.c_uint32), ("epsilon", C.c_float)]
+
+
+class GradTensor(C.Structure):
+    _fields_ = [("d_in", C.c_void_p), ("d_out", C.c_void_p), ("n", C.c_uint64), ("dtype", C.c_uint32)]
+
+
+F32, F16, BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "gelu": ACT_GELU, "silu": ACT_SILU}
+NORM_SKIP_NONFINITE = 1
+
 ADAM_UPDATE_UNTOUCHED, ADAM_L2_ALL, ADAM_EMA_NO_DEBIAS = 1, 2, 4
 
 
@@ -126,6 +143,9 @@ EXPORTS = [
     "neus2b_neus_forward_moved", "neus2b_neus_forward_indexed", "neus2b_forward_compute_loss", "neus2b_neus_train_moved", "neus2b_neus_sdf_moved", "neus2b_delta_forward", "neus2b_delta_backward",
     "neus2b_delta_optimizer_step", "neus2b_movement_accumulate", "neus2b_occupancy_update_moved", "neus2b_pcg32_seed", "neus2b_pcg32_advance", "neus2b_abi_struct_sizes",
     "neus2b_generate_samples", "neus2b_generate_samples_static", "neus2b_compute_loss", "neus2b_occupancy_update", "neus2b_occupancy_bounds", "neus2b_adam_step", "neus2b_adam_step_packed",
+    "neus2b_linear_forward", "neus2b_linear_backward_workspace", "neus2b_linear_backward", "neus2b_layer_norm_forward",
+    "neus2b_layer_norm_backward_workspace", "neus2b_layer_norm_backward", "neus2b_grad_table", "neus2b_grad_norm_workspace", "neus2b_grad_norm",
+    "neus2b_grad_clip",
     "neus2b_testbed_default_config", "neus2b_testbed_create", "neus2b_testbed_destroy", "neus2b_testbed_load_training_data",
     "neus2b_testbed_update_cameras", "neus2b_testbed_set_params", "neus2b_testbed_get_params", "neus2b_testbed_n_params",
     "neus2b_testbed_train", "neus2b_testbed_device_ptrs", "neus2b_testbed_train_backward", "neus2b_testbed_train_pregenerate", "neus2b_testbed_train_optimizer_step_async", "neus2b_testbed_train_wait_stats", "neus2b_testbed_train_step",
@@ -154,6 +174,18 @@ def lib():
         _lib.neus2b_per_level_scale_from_top_resolution.argtypes = [C.c_uint32, C.c_uint32, C.c_float, C.c_uint32]
         _lib.neus2b_testbed_config_active_levels.restype = C.c_uint32
         _lib.neus2b_launch_count.restype = C.c_uint64
+        p, u64 = C.c_void_p, C.c_uint64
+        _lib.neus2b_linear_forward.argtypes = [p, p, u64, p, p, p, u64, p, u64, p, u64, p]
+        _lib.neus2b_linear_backward_workspace.argtypes = [p, p]
+        _lib.neus2b_linear_backward.argtypes = [p, p, u64, p, p, u64, p, u64, C.c_uint32, p, u64, p, u64, p, u64, p, p, C.c_int, p, u64, p]
+        _lib.neus2b_layer_norm_forward.argtypes = [p, p, u64, p, p, p, u64, p, p, p]
+        _lib.neus2b_layer_norm_backward_workspace.argtypes = [p, p]
+        _lib.neus2b_layer_norm_backward.argtypes = [p, p, u64, p, p, p, p, u64, p, u64, p, u64, p, p, C.c_int, p, u64, p]
+        _lib.neus2b_grad_table.argtypes = [p, C.c_uint32, p, p, p]
+        _lib.neus2b_grad_norm_workspace.argtypes = [C.c_uint32]
+        _lib.neus2b_grad_norm_workspace.restype = u64
+        for f in (_lib.neus2b_grad_norm, _lib.neus2b_grad_clip):
+            f.argtypes = [p, C.c_uint32, C.c_float, C.c_float, C.c_uint32, p, p, p, u64, p]
         _check_layout(_lib)
     return _lib
 
@@ -161,7 +193,7 @@ def lib():
 def abi_structs():
     """The ctypes mirrors of the header's structures, in the order of neus2b_abi_struct_sizes."""
     return [GridDesc, Motion, Pcg32, Dataset, TrainCfg, RayWorkspace, AdamCfg, TestbedConfig, TrainStats, RenderCfg, RenderWorkspace, RenderRequest,
-            TrainingState]
+            TrainingState, LinearDesc, LayerNormDesc, GradTensor]
 
 
 def _check_layout(library):

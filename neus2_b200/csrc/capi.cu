@@ -35,7 +35,8 @@ extern "C" uint32_t neus2b_abi_struct_sizes(uint32_t* sizes, uint32_t capacity) 
 	                        (uint32_t)sizeof(neus2b_dataset),         (uint32_t)sizeof(neus2b_train_cfg),       (uint32_t)sizeof(neus2b_ray_workspace),
 	                        (uint32_t)sizeof(neus2b_adam_cfg),        (uint32_t)sizeof(neus2b_testbed_config),  (uint32_t)sizeof(neus2b_train_stats),
 	                        (uint32_t)sizeof(neus2b_render_cfg),      (uint32_t)sizeof(neus2b_render_workspace), (uint32_t)sizeof(neus2b_render_request),
-	                        (uint32_t)sizeof(neus2b_training_state)};
+	                        (uint32_t)sizeof(neus2b_training_state),  (uint32_t)sizeof(neus2b_linear_desc),   (uint32_t)sizeof(neus2b_layer_norm_desc),
+	                        (uint32_t)sizeof(neus2b_grad_tensor)};
 	const uint32_t n = (uint32_t)(sizeof(all) / sizeof(all[0]));
 	for (uint32_t i = 0; i < n && i < capacity && sizes; ++i) sizes[i] = all[i];
 	return n;

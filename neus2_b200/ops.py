@@ -268,6 +268,228 @@ def adam_step_packed(cfg, grad_mlp, grad_grid, grad_var, state, params, params_e
                                             L.ptr(grad_var), L.ptr(state), L.ptr(params), L.ptr(params_ema), L.cur_stream()))
 
 
+# ------------------------------------------------------------------------------------------------ layers of any width
+_DTYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+
+
+def _refuse(what):
+    raise L.Neus2bError("neus2b: " + what)
+
+
+def _home(t, name):
+    """The device all tensors of a call have to be on: the current one, whose current stream the call is enqueued on."""
+    if not t.is_cuda:
+        _refuse(f"{name} has to be a CUDA tensor")
+    if t.device.index != torch.cuda.current_device():
+        _refuse(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+def _rows(t, name, n, width, dtype, device):
+    """(address, row stride in entries) of a [n][width] tensor with contiguous rows; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if t.device != device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
+        _refuse(f"{name} has to be {dtype} [{n}][{width}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    row, col = t.stride()
+    if (col != 1 and width > 1) or (row < width and n > 1):
+        _refuse(f"{name}: the entries of a row have to be contiguous and the rows apart, got strides ({row}, {col})")
+    return t.data_ptr(), row if n > 1 else width
+
+
+def _vector(t, name, width, dtype, device):
+    if t is None:
+        return None
+    if t.device != device or t.dtype != dtype or t.shape != (width,) or not t.is_contiguous():
+        _refuse(f"{name} has to be contiguous {dtype} [{width}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _weights(w, dtype, device):
+    if w.dim() != 2 or w.dtype != dtype or w.device != device or not w.is_contiguous():
+        _refuse(f"the weights have to be contiguous {dtype} [out][in] on {device}, got {w.dtype} {list(w.shape)} on {w.device}")
+    return w.shape
+
+
+def _workspace(query, desc, given, device):
+    """(tensor that keeps it alive, address, bytes)"""
+    need = C.c_uint64(0)
+    L.check(query(C.byref(desc), C.byref(need)))
+    if not need.value:
+        return None, None, 0
+    if given is None:
+        given = torch.empty(need.value, dtype=torch.uint8, device=device)
+    elif given.device != device or not given.is_contiguous() or given.numel() * given.element_size() < need.value:
+        _refuse(f"the workspace has to be {need.value} contiguous bytes on {device}")
+    return given, given.data_ptr(), given.numel() * given.element_size()
+
+
+def _gradient(t, name, shape, mode, device):
+    """The fp32 tensor a parameter gradient goes to: the caller's, or a new one where there is nothing to add to."""
+    if t is None:
+        if mode == L.GRAD_ACCUMULATE:
+            return torch.zeros(shape, dtype=torch.float32, device=device)
+        return torch.empty(shape, dtype=torch.float32, device=device)
+    if t.device != device or t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _refuse(f"{name} has to be contiguous float32 {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t
+
+
+def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_preact=False, out=None):
+    """act(x w^T + bias) + residual for fp16 or bf16 tensors: x [n][in], w [out][in], bias [out], residual [n][out].  Rows may be apart
+    (views of wider matrices).  want_preact: returns (y, z) with z = x w^T + bias, which linear_backward reads.  `out` may be
+    `residual`."""
+    dev, t = _home(x, "x"), x.dtype
+    if t != _H and t != torch.bfloat16:
+        _refuse(f"linear layers take float16 and bfloat16, got {t}")
+    n_out, n_in = _weights(w, t, dev)
+    n = x.shape[0]
+    xp, xs = _rows(x, "x", n, n_in, t, dev)
+    rp, rs = _rows(residual, "residual", n, n_out, t, dev)
+    bp = _vector(bias, "bias", n_out, t, dev)
+    if out is None:
+        out = torch.empty((n, n_out), dtype=t, device=dev)
+    yp, ys = _rows(out, "out", n, n_out, t, dev)
+    z = torch.empty((n, n_out), dtype=t, device=dev) if want_preact else None
+    d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
+    L.check(L.lib().neus2b_linear_forward(C.byref(d), xp, xs, w.data_ptr(), bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out,
+                                          L.cur_stream()))
+    return (out, z) if want_preact else out
+
+
+def linear_backward(x, w, dL_dout, activation=L.ACT_NONE, preact=None, below_activation=L.ACT_NONE, below_preact=None, skip=None, wgrad=None,
+                    bgrad=None, mode=L.GRAD_OVERWRITE, want_din=True, want_bias=True, workspace=None):
+    """(dL/dx, wgrad, bgrad) of linear_forward.  activation, preact: this layer's activation and its z.  below_activation,
+    below_preact: dL/dx comes multiplied by the slope of the activation that produced x, which makes it dL/dz of the layer below.
+    skip: added to dL/dx (the gradient of a residual connection around this layer).  The parameter gradients are fp32; mode
+    GRAD_IGNORE computes none, GRAD_ACCUMULATE adds to the tensors given."""
+    dev, t = _home(x, "x"), x.dtype
+    if t != _H and t != torch.bfloat16:
+        _refuse(f"linear layers take float16 and bfloat16, got {t}")
+    n_out, n_in = _weights(w, t, dev)
+    n = x.shape[0]
+    xp, xs = _rows(x, "x", n, n_in, t, dev)
+    dyp, dys = _rows(dL_dout, "dL_dout", n, n_out, t, dev)
+    if activation != L.ACT_NONE and preact is None:
+        _refuse("an activated layer's backward pass needs preact")
+    if want_din and below_activation != L.ACT_NONE and below_preact is None:
+        _refuse("below_activation needs below_preact")
+    zp, zs = _rows(preact, "preact", n, n_out, t, dev)
+    bzp, bzs = _rows(below_preact, "below_preact", n, n_in, t, dev)
+    sp, ss = _rows(skip, "skip", n, n_in, t, dev)
+    din = torch.empty((n, n_in), dtype=t, device=dev) if want_din else None
+    params = mode != L.GRAD_IGNORE
+    wgrad = _gradient(wgrad, "wgrad", (n_out, n_in), mode, dev) if params else None
+    bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, dev) if params and want_bias else None
+    d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
+    lib = L.lib()
+    keep, wsp, wsb = _workspace(lib.neus2b_linear_backward_workspace, d, workspace, dev)
+    L.check(lib.neus2b_linear_backward(C.byref(d), xp, xs, w.data_ptr(), zp, zs, dyp, dys, below_activation, bzp, bzs, sp, ss,
+                                       din.data_ptr() if want_din else None, n_in, wgrad.data_ptr() if params else None,
+                                       bgrad.data_ptr() if bgrad is not None else None, mode, wsp, wsb, L.cur_stream()))
+    return din, wgrad, bgrad
+
+
+def _norm_desc(x, gamma, eps):
+    if x.dtype not in _DTYPES:
+        _refuse(f"layer norm takes float32, float16 and bfloat16, got {x.dtype}")
+    if x.dim() != 2:
+        _refuse(f"x has to be [n][width], got {list(x.shape)}")
+    if gamma.dtype != x.dtype and gamma.dtype != torch.float32:
+        _refuse(f"gamma has to be {x.dtype} or float32, got {gamma.dtype}")
+    return L.LayerNormDesc(x.shape[0], x.shape[1], _DTYPES[x.dtype], _DTYPES[gamma.dtype], eps)
+
+
+def layer_norm_forward(x, gamma, beta=None, eps=1e-5, want_stats=False, out=None):
+    """gamma (x - mean) rstd + beta over the rows of x [n][width] (fp32, fp16, bf16; gamma and beta of the same type or fp32).
+    want_stats: returns (y, mean, rstd), which layer_norm_backward reads.  `out` may be x."""
+    dev = _home(x, "x")
+    d = _norm_desc(x, gamma, eps)
+    n, width = x.shape
+    xp, xs = _rows(x, "x", n, width, x.dtype, dev)
+    gp, bp = _vector(gamma, "gamma", width, gamma.dtype, dev), _vector(beta, "beta", width, gamma.dtype, dev)
+    if out is None:
+        out = torch.empty((n, width), dtype=x.dtype, device=dev)
+    yp, ys = _rows(out, "out", n, width, x.dtype, dev)
+    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if want_stats else None
+    sp = stats.data_ptr() if want_stats else None
+    L.check(L.lib().neus2b_layer_norm_forward(C.byref(d), xp, xs, gp, bp, yp, ys, sp, sp + 4 * n if want_stats else None, L.cur_stream()))
+    return (out, stats[0], stats[1]) if want_stats else out
+
+
+def layer_norm_backward(x, gamma, mean, rstd, dL_dout, skip=None, dgamma=None, dbeta=None, mode=L.GRAD_OVERWRITE, eps=1e-5, want_din=True,
+                        workspace=None):
+    """(dL/dx, dgamma, dbeta) of layer_norm_forward; skip [n][width] is added to dL/dx (a residual connection around the norm)."""
+    dev = _home(x, "x")
+    d = _norm_desc(x, gamma, eps)
+    n, width = x.shape
+    xp, xs = _rows(x, "x", n, width, x.dtype, dev)
+    dyp, dys = _rows(dL_dout, "dL_dout", n, width, x.dtype, dev)
+    sp, ss = _rows(skip, "skip", n, width, x.dtype, dev)
+    gp = _vector(gamma, "gamma", width, gamma.dtype, dev)
+    mp, rp = _vector(mean, "mean", n, torch.float32, dev), _vector(rstd, "rstd", n, torch.float32, dev)
+    din = torch.empty((n, width), dtype=x.dtype, device=dev) if want_din else None
+    params = mode != L.GRAD_IGNORE
+    dgamma = _gradient(dgamma, "dgamma", (width,), mode, dev) if params else None
+    dbeta = _gradient(dbeta, "dbeta", (width,), mode, dev) if params else None
+    lib = L.lib()
+    keep, wsp, wsb = _workspace(lib.neus2b_layer_norm_backward_workspace, d, workspace, dev)
+    L.check(lib.neus2b_layer_norm_backward(C.byref(d), xp, xs, gp, mp, rp, dyp, dys, sp, ss, din.data_ptr() if want_din else None, width,
+                                           dgamma.data_ptr() if params else None, dbeta.data_ptr() if params else None, mode, wsp, wsb,
+                                           L.cur_stream()))
+    return din, dgamma, dbeta
+
+
+class GradientSet:
+    """A set of gradient tensors (contiguous fp32, fp16, bf16 CUDA tensors of any number and sizes) whose global norm is taken and
+    which are clipped by it, ahead of an optimizer step.  out: where the clipped gradients go (same types and sizes), default in
+    place.  The table of pieces is built here once; the tensors are kept.  Calls of one set share its workspace: issue them one after
+    another (or build a set for each stream)."""
+
+    def __init__(self, grads, out=None):
+        grads = list(grads)
+        out = grads if out is None else list(out)
+        if len(out) != len(grads):
+            _refuse(f"{len(grads)} gradients, {len(out)} outputs")
+        if not grads:
+            _refuse("a gradient set needs a tensor")
+        dev = _home(grads[0], "grads[0]")
+        rows = (L.GradTensor * len(grads))()
+        for i, (g, o) in enumerate(zip(grads, out)):
+            for t in (g, o):
+                if t.device != dev or t.dtype not in _DTYPES or t.dtype != g.dtype or t.numel() != g.numel() or not t.is_contiguous():
+                    _refuse(f"tensor {i}: gradients and outputs have to be contiguous float32, float16 or bfloat16 on {dev}, alike in type and size")
+            rows[i] = L.GradTensor(g.data_ptr(), o.data_ptr(), g.numel(), _DTYPES[g.dtype])
+        lib = L.lib()
+        nbytes, pieces = C.c_uint64(0), C.c_uint32(0)
+        L.check(lib.neus2b_grad_table(rows, len(grads), None, C.byref(nbytes), C.byref(pieces)))
+        host = torch.zeros(max(1, nbytes.value // 8), dtype=torch.int64)
+        L.check(lib.neus2b_grad_table(rows, len(grads), host.data_ptr(), C.byref(nbytes), C.byref(pieces)))
+        self.n_pieces = pieces.value
+        self.table = host.to(dev)
+        self.workspace_bytes = int(lib.neus2b_grad_norm_workspace(self.n_pieces))
+        self.workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=dev)
+        self._keep = (grads, out)
+
+    def _call(self, f, max_norm, scale, skip_nonfinite, nonfinite):
+        dev = _home(self.table, "the gradient set")
+        if nonfinite is not None and (nonfinite.device != dev or nonfinite.dtype != torch.int32 or nonfinite.numel() != 1):
+            _refuse(f"nonfinite has to be one int32 on {dev}")
+        result = torch.empty(2, dtype=torch.float32, device=dev)
+        L.check(f(self.table.data_ptr(), self.n_pieces, scale, max_norm, L.NORM_SKIP_NONFINITE if skip_nonfinite else 0, result.data_ptr(),
+                  nonfinite.data_ptr() if nonfinite is not None else None, self.workspace.data_ptr(), self.workspace_bytes, L.cur_stream()))
+        return result
+
+    def norm(self, max_norm=float("inf"), scale=1.0, skip_nonfinite=False, nonfinite=None):
+        """float32 [2]: the norm of `scale` times the gradients, and the factor that would clip it to max_norm."""
+        return self._call(L.lib().neus2b_grad_norm, max_norm, scale, skip_nonfinite, nonfinite)
+
+    def clip(self, max_norm, scale=1.0, skip_nonfinite=False, nonfinite=None):
+        """Writes the gradients times min(1, max_norm / norm) to the outputs; returns float32 [2] {norm, factor}.  A norm that is not
+        finite clips nothing (factor 1); nonfinite (int32 [1]) counts the entries that are not."""
+        return self._call(L.lib().neus2b_grad_clip, max_norm, scale, skip_nonfinite, nonfinite)
+
+
 def marching_cubes(sdf, tri_table=None, thresh=0.0, aabb_min=(0.0, 0.0, 0.0), aabb_max=(1.0, 1.0, 1.0)):
     """sdf: float32 CUDA tensor [rz][ry][rx].  Returns (verts [n][3] float32, indices [m] int32) in canonical order.
     tri_table: int8 [256][16] case table (defaults to the generated one of neus2_b200.mc_table)."""
