@@ -563,6 +563,8 @@ int launch_neus_tc_forward(const NeusArgs& a, uint32_t n_upper, cudaStream_t str
 int launch_neus_tc_train(const NeusArgs& a, uint32_t n_upper, cudaStream_t stream);
 int read_tc_error(uint32_t* h_flags);
 int write_tc_error(uint32_t flags);
+int read_linear_error(uint32_t* h_flags);  // linear_tc.cu
+int write_linear_error(uint32_t flags);
 static int g_mma_path = NEUS2B_MMA_TCGEN05;
 
 }  // namespace n2b
@@ -577,9 +579,16 @@ extern "C" int neus2b_set_mma_path(int path) {
 extern "C" int neus2b_get_mma_path(void) { return g_mma_path; }
 extern "C" int neus2b_device_error_flags(uint32_t* h_flags) {
 	if (!h_flags) return NEUS2B_E_INVALID;
-	return read_tc_error(h_flags);
+	uint32_t fused = 0, linear = 0;
+	if (int rc = read_tc_error(&fused)) return rc;
+	if (int rc = read_linear_error(&linear)) return rc;
+	*h_flags = fused | linear;
+	return NEUS2B_OK;
 }
-extern "C" int neus2b_set_device_error_flags(uint32_t flags) { return write_tc_error(flags); }
+extern "C" int neus2b_set_device_error_flags(uint32_t flags) {
+	if (int rc = write_linear_error(flags)) return rc;
+	return write_tc_error(flags);
+}
 
 static void fill_motion(NeusArgs& a, const neus2b_motion* motion) {
 	if (!motion || !motion->d_delta) return;

@@ -1,4 +1,5 @@
 """Linear layers, layer norm and gradient clipping (any width) against 64-bit restatements."""
+import ctypes as C
 import math
 
 import pytest
@@ -106,6 +107,28 @@ def test_linear_backward_of_an_activated_layer(ops, t):
         R.within("dx", dx, wx, ex + 1.01 * (e @ w.double().abs()))
         R.within("dw", dw, ww, ew + e.T @ x.double().abs())
         R.within("db", db, wb, eb + e.sum(0))
+
+
+@pytest.mark.parametrize("n", [1, 100, 5000, 40000])
+def test_bias_gradient_alone_and_frozen_inputs(ops, n):
+    """Each of the three gradients alone, and none: the same values as together."""
+    from neus2_b200 import _lib as L
+    g = gen(n)
+    t = torch.bfloat16
+    for i, o in ((16, 72), (520, 9), (40, 300)):
+        x, w, dy = rows(g, n, i, t), rows(g, o, i, t, 0.2), rows(g, n, o, t, 0.1)
+        dx, dw, db = ops.linear_backward(x, w, dy)
+        assert torch.equal(ops.linear_backward(x, w, dy, mode=L.GRAD_IGNORE)[0], dx)
+        only = ops.linear_backward(x, w, dy, want_din=False, want_bias=False)
+        assert only[0] is None and only[2] is None and torch.equal(only[1], dw)
+        d, need = L.LinearDesc(n, i, o, L.BF16, 0), C.c_uint64(0)
+        L.check(L.lib().neus2b_linear_backward_workspace(C.byref(d), C.byref(need)))
+        ws, out = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda"), torch.full((o,), 7.0, device="cuda")
+        L.check(L.lib().neus2b_linear_backward(C.byref(d), None, 0, None, None, 0, dy.data_ptr(), o, 0, None, 0, None, 0, None, 0, None, out.data_ptr(),
+                                               L.GRAD_ACCUMULATE, ws.data_ptr(), need.value, L.cur_stream()))
+        want = dy.double().sum(0)
+        R.within("db", out, want + 7.0, (n + 8) * 2.0 ** -23 * (dy.double().abs().sum(0) + 7.0))
+        R.within("db", db, want, (n + 4) * 2.0 ** -23 * dy.double().abs().sum(0))
 
 
 def test_linear_gradients_against_differences(ops):
@@ -285,7 +308,7 @@ def clip_reference(grads, max_norm, scale=1.0, skip=False):
     return norm, max_norm / norm if norm > max_norm and math.isfinite(norm) else 1.0
 
 
-@pytest.mark.parametrize("sizes", [[1], [5, 0, 3], [8192, 8193, 16384], [4, 12288, 1000003], [100 + 37 * i for i in range(700)]], ids=str)
+@pytest.mark.parametrize("sizes", [[1], [5, 0, 3], [8192, 8193, 16384], [4, 12288, 1000003], [100 + 37 * i for i in range(700)]], ids=lambda s: f"{len(s)}_tensors_of_{s[-1]}")
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "mixed"])
 def test_clip(ops, sizes, kind):
     if len(sizes) > 10 and kind != "mixed":
@@ -369,3 +392,9 @@ def test_streams_and_graph(ops):
         x.copy_(rows(g, n, width, t))
         dy.copy_(rows(g, n, width, t, 0.1))
         first = [v.clone() for v in block()]
+
+
+def test_no_wait_ran_out(ops):
+    from neus2_b200 import _lib as L
+    torch.cuda.synchronize()
+    assert L.device_error_flags() == 0
