@@ -565,6 +565,8 @@ int read_tc_error(uint32_t* h_flags);
 int write_tc_error(uint32_t flags);
 int read_linear_error(uint32_t* h_flags);  // linear_tc.cu
 int write_linear_error(uint32_t flags);
+int read_layer_norm_error(uint32_t* h_flags);  // layer_norm.cu
+int write_layer_norm_error(uint32_t flags);
 static int g_mma_path = NEUS2B_MMA_TCGEN05;
 
 }  // namespace n2b
@@ -579,14 +581,16 @@ extern "C" int neus2b_set_mma_path(int path) {
 extern "C" int neus2b_get_mma_path(void) { return g_mma_path; }
 extern "C" int neus2b_device_error_flags(uint32_t* h_flags) {
 	if (!h_flags) return NEUS2B_E_INVALID;
-	uint32_t fused = 0, linear = 0;
+	uint32_t fused = 0, linear = 0, norm = 0;
 	if (int rc = read_tc_error(&fused)) return rc;
 	if (int rc = read_linear_error(&linear)) return rc;
-	*h_flags = fused | linear;
+	if (int rc = read_layer_norm_error(&norm)) return rc;
+	*h_flags = fused | linear | norm;
 	return NEUS2B_OK;
 }
 extern "C" int neus2b_set_device_error_flags(uint32_t flags) {
 	if (int rc = write_linear_error(flags)) return rc;
+	if (int rc = write_layer_norm_error(flags)) return rc;
 	return write_tc_error(flags);
 }
 

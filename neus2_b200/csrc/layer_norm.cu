@@ -2,12 +2,16 @@
 //
 // A group of TPR threads owns a row at a time and keeps it in registers: one read, one write per value.  Groups of up to a warp
 // reduce with shuffles, wider ones through shared memory behind a barrier of their own; blocks are persistent, so gamma and beta
-// (and in the backward pass the sums for their gradients) stay in registers over all rows of a group, and the next row is fetched
-// before the current one is reduced.  The variance is the mean square of the centred row, not a difference of sums.
+// (and in the backward pass the sums for their gradients) stay on the SM over all rows of a group.  The variance is the mean square
+// of the centred row, not a difference of sums.
+#include <type_traits>
+
 #include "dense.cuh"
 
 namespace n2b {
 namespace ln {
+
+static __device__ uint32_t g_error;  // bit 0: a bounded wait ran out
 
 // VEC entries moved by one access: 16 bytes, or one entry where rows do not start on 16-byte boundaries.
 template <typename T, int VEC>
@@ -64,20 +68,53 @@ struct Pack<T, 1> {
 	static __device__ __forceinline__ Raw put(const float (&v)[1]) { return from_f<T>(v[0]); }
 };
 
+// Makes the compiler forget what it knows about a packed value: it unpacks it again where it is used next, instead of keeping the
+// unpacked (or centred) entries of a whole row in registers over a reduction.
+__device__ __forceinline__ void forget(uint4& v) { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }
+__device__ __forceinline__ void forget(float4& v) { asm volatile("" : "+f"(v.x), "+f"(v.y), "+f"(v.z), "+f"(v.w)); }
+__device__ __forceinline__ void forget(float& v) { asm volatile("" : "+f"(v)); }
+template <typename H>
+__device__ __forceinline__ void forget(H& v) { asm volatile("" : "+h"(*reinterpret_cast<uint16_t*>(&v))); }
+
+template <typename Raw>
+__device__ __forceinline__ Raw zero() { return Raw{}; }
+template <>
+__device__ __forceinline__ __half zero<__half>() { return __ushort_as_half(0); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 zero<__nv_bfloat16>() { return __ushort_as_bfloat16(0); }
+
 __device__ __forceinline__ float param_at(const void* p, uint32_t dtype, uint32_t c) {
 	if (dtype == NEUS2B_F32) return ((const float*)p)[c];
 	return dtype == NEUS2B_F16 ? to_f(((const __half*)p)[c]) : to_f(((const __nv_bfloat16*)p)[c]);
 }
 
-// Sums over the TPR threads of a group, in a fixed order, the same value in all of them.  s: shared memory of the group, [2][TPR / 32][2];
-// `turn` alternates so that a barrier per sum is enough.
+// Sums over the TPR threads of a group, in a fixed order, the same values in all of them.  s: shared memory of the group, [2][TPR / 32];
+// `turn` alternates so that one barrier per sum is enough.
 template <int TPR>
-__device__ __forceinline__ void group_sum(float& a, float& b, float2* s, int group, int& turn) {
+__device__ __forceinline__ float group_sum(float a) {
 #pragma unroll
-	for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) {
-		a += __shfl_xor_sync(~0u, a, o);
-		b += __shfl_xor_sync(~0u, b, o);
+	for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+	return a;
+}
+template <int TPR>
+__device__ __forceinline__ float group_sum(float a, float2* s, int group, int& turn) {
+	a = group_sum<TPR>(a);
+	if (TPR > 32) {
+		constexpr int W = TPR / 32;
+		float2* t = s + turn * W;
+		turn ^= 1;
+		if ((threadIdx.x & 31) == 0) t[(threadIdx.x % TPR) >> 5].x = a;
+		asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+		a = 0.f;
+#pragma unroll
+		for (int w = 0; w < W; ++w) a += t[w].x;
 	}
+	return a;
+}
+template <int TPR>
+__device__ __forceinline__ void group_sums(float& a, float& b, float2* s, int group, int& turn) {
+	a = group_sum<TPR>(a);
+	b = group_sum<TPR>(b);
 	if (TPR > 32) {
 		constexpr int W = TPR / 32;
 		float2* t = s + turn * W;
@@ -90,181 +127,339 @@ __device__ __forceinline__ void group_sum(float& a, float& b, float2* s, int gro
 	}
 }
 
+// gamma or beta of the group's columns in shared memory: entry (access k, thread t, i) of a row is the row's column (k TPR + t) VEC + i; four
+// consecutive ones lie together and the threads' fours side by side, so that a warp's reads do not collide.
+template <int VEC, int TPR>
+__device__ __forceinline__ int param_slot(int k, int t, int i) {
+	constexpr int Q = VEC < 4 ? VEC : 4;
+	return ((k * (VEC / Q) + i / Q) * TPR + t) * Q + i % Q;
+}
+template <int VEC, int TPR, int VPT>
+__device__ __forceinline__ void stage_param(float* s, const void* p, uint32_t dtype, uint32_t W, int threads) {
+	for (int c = threadIdx.x; c < VEC * TPR * VPT; c += threads) {
+		const int u = c / VEC;
+		s[param_slot<VEC, TPR>(u / TPR, u % TPR, c % VEC)] = p && (uint32_t)c < W ? param_at(p, dtype, c) : 0.f;
+	}
+}
+template <int VEC, int TPR>
+__device__ __forceinline__ void staged(const float* s, int k, int t, float (&v)[VEC]) {
+	if (VEC >= 4) {
+#pragma unroll
+		for (int q = 0; q < VEC / 4; ++q) {
+			const float4 f = *reinterpret_cast<const float4*>(s + param_slot<VEC, TPR>(k, t, 4 * q));
+			v[4 * q] = f.x, v[4 * q + 1 < VEC ? 4 * q + 1 : 0] = f.y, v[4 * q + 2 < VEC ? 4 * q + 2 : 0] = f.z, v[4 * q + 3 < VEC ? 4 * q + 3 : 0] = f.w;
+		}
+	} else {
+#pragma unroll
+		for (int i = 0; i < VEC; ++i) v[i] = s[param_slot<VEC, TPR>(k, t, i)];
+	}
+}
+
+// ---- rows on their way: every group has a ring of `depth` rows in shared memory that bulk copies fill ahead of it
+__device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+	asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void init_barrier(uint32_t bar) {
+	asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n\tfence.mbarrier_init.release.cluster;" ::"r"(bar) : "memory");
+}
+// both addresses on 16-byte boundaries, bytes a multiple of 16
+__device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+	asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// A row takes microseconds to arrive; the wait gives up after about a second, and the group goes on with what is there.
+__device__ __forceinline__ void wait_row(uint32_t bar, uint32_t parity) {
+	for (uint32_t it = 0; it < (1u << 20); ++it) {
+		uint32_t ok;
+		asm volatile(
+		    "{\n\t.reg .pred p;\n\t"
+		    "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+		    "selp.u32 %0, 1, 0, p;\n\t}"
+		    : "=r"(ok)
+		    : "r"(bar), "r"(parity)
+		    : "memory");
+		if (ok) return;
+	}
+	atomicOr(&g_error, 1u);
+}
 template <int TPR>
-struct Geometry {
-	static constexpr int kThreads = TPR > 256 ? TPR : 256;
-	static constexpr int kGroups = kThreads / TPR;
+__device__ __forceinline__ void group_barrier(int group) {
+	if (TPR > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+	else __syncwarp();
+}
+
+// Up to 8 entries a thread, gamma and beta stay in registers and the next row is fetched ahead; above that they are read from shared
+// memory, the registers hold the packed row, and the rows of the SM's other warps are fetch-ahead enough.
+template <typename T, int VEC, int TPR, int VPT, bool RING>
+struct Forward {
+	static constexpr bool kStaged = VEC * VPT > 8;
+	static constexpr int kWords = VPT * (VEC * (int)sizeof(T) > 4 ? VEC * (int)sizeof(T) / 4 : 1);  // registers of a packed row
+	static constexpr int kThreads = !RING ? 256 : TPR == 64 ? 768 : 1024, kGroups = kThreads / TPR;  // (a group's barrier is one of 15)
+	static constexpr int kBlocks = RING ? 1 : kWords <= 16 ? 4 : kWords <= 32 ? 3 : 2;
 };
 
-template <typename T, int VEC, int TPR, int VPT>
-__global__ void __launch_bounds__(Geometry<TPR>::kThreads) forward_kernel(neus2b_layer_norm_desc d, const T* x, uint64_t x_ld,
-                                                                          const void* __restrict__ gamma, const void* __restrict__ beta, T* y,
-                                                                          uint64_t y_ld, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+template <typename T, int VEC, int TPR, int VPT, bool RING>
+__global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, Forward<T, VEC, TPR, VPT, RING>::kBlocks)
+    forward_kernel(neus2b_layer_norm_desc d, int depth, const T* x, uint64_t x_ld, const void* __restrict__ gamma, const void* __restrict__ beta, T* y, uint64_t y_ld,
+                   float* __restrict__ mean_out, float* __restrict__ rstd_out) {
 	using P = Pack<T, VEC>;
-	constexpr int G = Geometry<TPR>::kGroups;
+	using Raw = typename P::Raw;
+	using F = Forward<T, VEC, TPR, VPT, RING>;
+	constexpr int G = F::kGroups;
+	constexpr bool kAhead = !F::kStaged && !RING;
+	constexpr int kMaxDepth = 4;
+	__shared__ uint64_t bars[RING ? G * kMaxDepth : 1];
 	__shared__ float2 sums[G][2 * (TPR > 32 ? TPR / 32 : 1)];
+	extern __shared__ float4 params4[];  // kStaged: gamma, beta; RING: the rings
+	float* const sg = reinterpret_cast<float*>(params4);
+	float* const sb = sg + VEC * TPR * VPT;
 	const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
 	const uint32_t W = d.width;
-	float ga[VPT * VEC], be[VPT * VEC];
+	const float inv_w = 1.f / (float)W;
+	float ga[F::kStaged ? 1 : VPT * VEC], be[F::kStaged ? 1 : VPT * VEC];
+	if (F::kStaged) {
+		stage_param<VEC, TPR, VPT>(sg, gamma, d.param_dtype, W, F::kThreads);
+		stage_param<VEC, TPR, VPT>(sb, beta, d.param_dtype, W, F::kThreads);
+		__syncthreads();
+	} else {
 #pragma unroll
-	for (int k = 0; k < VPT * VEC; ++k) {
-		const uint32_t c = ((k / VEC) * TPR + t) * VEC + k % VEC;
-		ga[k] = c < W ? param_at(gamma, d.param_dtype, c) : 0.f;
-		be[k] = c < W && beta ? param_at(beta, d.param_dtype, c) : 0.f;
+		for (int k = 0; k < VPT * VEC; ++k) {
+			const uint32_t c = ((k / VEC) * TPR + t) * VEC + k % VEC;
+			ga[F::kStaged ? 0 : k] = c < W ? param_at(gamma, d.param_dtype, c) : 0.f;
+			be[F::kStaged ? 0 : k] = c < W && beta ? param_at(beta, d.param_dtype, c) : 0.f;
+		}
 	}
-	typename P::Raw raw[VPT];
-	auto fetch = [&](uint32_t r) {
+	Raw cur[VPT], ahead[kAhead ? VPT : 1];
+	auto fetch = [&](Raw* raw, uint32_t r) {
 #pragma unroll
 		for (int k = 0; k < VPT; ++k) {
 			const uint32_t c = (k * TPR + t) * VEC;
-			if (r < d.n && c < W) raw[k] = *reinterpret_cast<const typename P::Raw*>(x + r * x_ld + c);
+			raw[k] = r < d.n && c < W ? *reinterpret_cast<const Raw*>(x + r * x_ld + c) : zero<Raw>();
 		}
 	};
-	int turn = 0;
-	uint32_t r = blockIdx.x * G + group;
-	fetch(r);
+	int turn = 0, slot = 0;
+	uint32_t parity = 0, r = blockIdx.x * G + group;
+	const uint32_t step = gridDim.x * G;
+	const uint32_t row_bytes = W * (uint32_t)sizeof(T);
+	unsigned char* const ring = reinterpret_cast<unsigned char*>(params4) + (F::kStaged ? 2 * VEC * TPR * VPT * sizeof(float) : 0) + (size_t)group * depth * row_bytes;
+	if (kAhead) fetch(ahead, r);
+	if (RING && t == 0) {
+		for (int i = 0; i < depth; ++i) init_barrier(sptr(&bars[group * kMaxDepth + i]));
+		for (int i = 0; i < depth; ++i) {
+			const uint64_t row = (uint64_t)r + (uint64_t)i * step;
+			if (row >= d.n) break;
+			const uint32_t bar = sptr(&bars[group * kMaxDepth + i]);
+			expect_bytes(bar, row_bytes);
+			copy_row(sptr(ring + (size_t)i * row_bytes), x + row * x_ld, row_bytes, bar);
+		}
+	}
+	if (RING) __syncthreads();
 	// every group of the block runs the same number of rounds: the shuffles of narrow groups take the whole warp
-	for (uint32_t r0 = blockIdx.x * G; r0 < d.n; r0 += gridDim.x * G, r += gridDim.x * G) {
-		float v[VPT * VEC];
-		float s = 0.f, q = 0.f;
+	for (uint32_t r0 = blockIdx.x * G; r0 < d.n; r0 += step, r += step) {
+		if (kAhead) {
+#pragma unroll
+			for (int k = 0; k < VPT; ++k) cur[k] = ahead[kAhead ? k : 0];
+			fetch(ahead, r + step);
+		} else if (RING) {
+			const uint32_t bar = sptr(&bars[group * kMaxDepth + slot]);
+			unsigned char* const row = ring + (size_t)slot * row_bytes;
+			if (r < d.n) wait_row(bar, parity);
+#pragma unroll
+			for (int k = 0; k < VPT; ++k) {  // (a group that has no row left computes on an old one and stores nothing)
+				const uint32_t c = (k * TPR + t) * VEC;
+				cur[k] = c < W ? *reinterpret_cast<const Raw*>(row + c * sizeof(T)) : zero<Raw>();
+			}
+			group_barrier<TPR>(group);  // the row is in registers: its place is free
+			const uint64_t next = (uint64_t)r + (uint64_t)depth * step;
+			if (t == 0 && next < d.n) {
+				expect_bytes(bar, row_bytes);
+				copy_row(sptr(row), x + next * x_ld, row_bytes, bar);
+			}
+			if (++slot == depth) slot = 0, parity ^= 1u;
+		} else {
+			fetch(cur, r);
+		}
+		float s = 0.f;
 #pragma unroll
 		for (int k = 0; k < VPT; ++k) {
 			float e[VEC];
-			P::get(raw[k], e);
+			P::get(cur[k], e);
 #pragma unroll
-			for (int i = 0; i < VEC; ++i) {
-				v[k * VEC + i] = e[i];
-				if ((k * TPR + t) * VEC + i < W) s += e[i];
-			}
+			for (int i = 0; i < VEC; ++i) s += e[i];
 		}
-		fetch(r + gridDim.x * G);
-		group_sum<TPR>(s, q, sums[group], group, turn);
-		const float mean = s / (float)W;
-		q = s = 0.f;
+		s = group_sum<TPR>(s, sums[group], group, turn);
+		float mean = s * inv_w;
+		mean = fmaf(fmaf(-mean, (float)W, s), inv_w, mean);  // the quotient, corrected by what the product with 1 / W left
+		float q = 0.f;
 #pragma unroll
-		for (int k = 0; k < VPT * VEC; ++k) {
-			v[k] -= mean;
-			if (((k / VEC) * TPR + t) * VEC + k % VEC < W) q = fmaf(v[k], v[k], q);
+		for (int k = 0; k < VPT; ++k) {
+			if (F::kStaged) forget(cur[k]);
+			float e[VEC], part = 0.f;
+			P::get(cur[k], e);
+#pragma unroll
+			for (int i = 0; i < VEC; ++i) part = fmaf(e[i] - mean, e[i] - mean, part);
+			if ((k * TPR + t) * VEC < W) q += part;  // an access lies inside the row or outside of it
 		}
-		group_sum<TPR>(q, s, sums[group], group, turn);
-		const float rstd = 1.f / sqrtf(q / (float)W + d.epsilon);
+		q = group_sum<TPR>(q, sums[group], group, turn);
+		const float rstd = rsqrtf(fmaf(q, inv_w, d.epsilon));
+		if (F::kStaged) asm volatile("" ::: "memory");  // gamma and beta are read again for every row, not kept in registers
 		if (r < d.n) {
 #pragma unroll
 			for (int k = 0; k < VPT; ++k) {
 				const uint32_t c = (k * TPR + t) * VEC;
-				float e[VEC];
+				float e[VEC], g[VEC], b[VEC];
+				if (F::kStaged) forget(cur[k]);
+				P::get(cur[k], e);
+				if (F::kStaged) {
+					staged<VEC, TPR>(sg, k, t, g);
+					staged<VEC, TPR>(sb, k, t, b);
+				}
 #pragma unroll
-				for (int i = 0; i < VEC; ++i) e[i] = fmaf(v[k * VEC + i] * rstd, ga[k * VEC + i], be[k * VEC + i]);
-				if (c < W) *reinterpret_cast<typename P::Raw*>(y + r * y_ld + c) = P::put(e);
+				for (int i = 0; i < VEC; ++i)
+					e[i] = fmaf((e[i] - mean) * rstd, F::kStaged ? g[i] : ga[F::kStaged ? 0 : k * VEC + i], F::kStaged ? b[i] : be[F::kStaged ? 0 : k * VEC + i]);
+				if (c < W) *reinterpret_cast<Raw*>(y + r * y_ld + c) = P::put(e);
 			}
 			if (mean_out && t == 0) mean_out[r] = mean, rstd_out[r] = rstd;
 		}
 	}
 }
 
-// partial: [gridDim.x][2][width], the block's sums for dgamma and dbeta.  A block adds its groups' sums in order.
-template <typename T, int VEC, int TPR, int VPT>
-__global__ void __launch_bounds__(Geometry<TPR>::kThreads) backward_kernel(neus2b_layer_norm_desc d, const T* __restrict__ x, uint64_t x_ld,
-                                                                           const void* __restrict__ gamma, const float* __restrict__ mean,
-                                                                           const float* __restrict__ rstd, const T* dy, uint64_t dy_ld, const T* skip,
-                                                                           uint64_t skip_ld, T* dx, uint64_t dx_ld, float* __restrict__ partial) {
+template <int TPR, int E, bool RING>
+struct Backward {
+	static constexpr int kThreads = RING ? 512 : TPR > 128 ? TPR : 128, kGroups = kThreads / TPR;
+	static constexpr int kBlocks = (!RING && E <= 8 ? 1024 : 512) / kThreads;
+	static constexpr int kGrid = kSMs * kBlocks;
+};
+
+// partial: [gridDim.x][2][width], the block's sums for dgamma and dbeta.  A block adds its groups' sums in order.  The next
+// row's statistics are fetched ahead like the row itself.
+template <typename T, int VEC, int TPR, int VPT, bool RING>
+__global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Backward<TPR, VEC * VPT, RING>::kBlocks)
+    backward_kernel(neus2b_layer_norm_desc d, int depth, const T* __restrict__ x, uint64_t x_ld, const void* __restrict__ gamma, const float* __restrict__ mean,
+                    const float* __restrict__ rstd, const T* dy, uint64_t dy_ld, const T* skip, uint64_t skip_ld, T* dx, uint64_t dx_ld,
+                    float* __restrict__ partial) {
 	using P = Pack<T, VEC>;
 	using Raw = typename P::Raw;
-	constexpr int G = Geometry<TPR>::kGroups, E = VPT * VEC;
+	constexpr int E = VPT * VEC;
+	using B = Backward<TPR, E, RING>;
+	constexpr int kMaxDepth = 4;
+	__shared__ uint64_t bars[RING ? B::kGroups * kMaxDepth : 1];
+	constexpr int G = B::kGroups;
 	__shared__ float2 sums[G][2 * (TPR > 32 ? TPR / 32 : 1)];
-	extern __shared__ float columns[];  // [2][TPR * E] where G > 1
+	extern __shared__ float4 rings4[];  // the rings; afterwards, where G > 1, the threads' sums [2 E][threads]
 	const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
 	const uint32_t W = d.width;
 	const float inv_w = 1.f / (float)W;
-	float ga[E], dg[E], db[E];
+	float ga[E];
 #pragma unroll
 	for (int k = 0; k < E; ++k) {
 		const uint32_t c = ((k / VEC) * TPR + t) * VEC + k % VEC;
 		ga[k] = c < W ? param_at(gamma, d.param_dtype, c) : 0.f;
-		dg[k] = db[k] = 0.f;
 	}
-	Raw rx[VPT], ry[VPT];
-	float mu = 0.f, rs = 0.f;
-	auto fetch = [&](uint32_t r) {
-		if (r >= d.n) return;
-		mu = mean[r], rs = rstd[r];
+	float dg[E], db[E];
 #pragma unroll
-		for (int k = 0; k < VPT; ++k) {
-			const uint32_t c = (k * TPR + t) * VEC;
-			if (c < W) {
-				rx[k] = *reinterpret_cast<const Raw*>(x + r * x_ld + c);
-				ry[k] = *reinterpret_cast<const Raw*>(dy + r * dy_ld + c);
-			}
-		}
+	for (int k = 0; k < E; ++k) dg[k] = db[k] = 0.f;
+	int turn = 0, slot = 0;
+	uint32_t parity = 0, r = blockIdx.x * G + group;
+	const uint32_t step = gridDim.x * G;
+	const bool add = skip && dx;
+	const uint32_t row_bytes = W * (uint32_t)sizeof(T), slot_bytes = row_bytes * (add ? 3 : 2);  // x, dy, skip
+	unsigned char* const ring = reinterpret_cast<unsigned char*>(rings4) + (size_t)group * depth * slot_bytes;
+	auto order = [&](uint64_t row, int i) {
+		const uint32_t bar = sptr(&bars[group * kMaxDepth + i]), dst = sptr(ring + (size_t)i * slot_bytes);
+		expect_bytes(bar, slot_bytes);
+		copy_row(dst, x + row * x_ld, row_bytes, bar);
+		copy_row(dst + row_bytes, dy + row * dy_ld, row_bytes, bar);
+		if (add) copy_row(dst + 2 * row_bytes, skip + row * skip_ld, row_bytes, bar);
 	};
-	int turn = 0;
-	uint32_t r = blockIdx.x * G + group;
-	fetch(r);
-	for (uint32_t r0 = blockIdx.x * G; r0 < d.n; r0 += gridDim.x * G, r += gridDim.x * G) {
+	if (RING && t == 0) {
+		for (int i = 0; i < depth; ++i) init_barrier(sptr(&bars[group * kMaxDepth + i]));
+		for (int i = 0; i < depth; ++i) {
+			const uint64_t row = (uint64_t)r + (uint64_t)i * step;
+			if (row < d.n) order(row, i);
+		}
+	}
+	if (RING) __syncthreads();
+	float mu = 0.f, rs = 0.f;
+	if (r < d.n) mu = mean[r], rs = rstd[r];
+	for (uint32_t r0 = blockIdx.x * G; r0 < d.n; r0 += step, r += step) {
+		Raw rx[VPT], ry[VPT], rk[VPT];
 		const float m = mu, sc = rs;
+		if ((uint64_t)r + step < d.n) mu = mean[r + step], rs = rstd[r + step];  // of the next row, ahead of its turn
+		const unsigned char* const row = ring + (size_t)slot * slot_bytes;
+		if (RING && r < d.n) wait_row(sptr(&bars[group * kMaxDepth + slot]), parity);
+#pragma unroll
+		for (int k = 0; k < VPT; ++k) {  // zeros outside of the row and behind the last one: they add nothing to any sum
+			const uint32_t c = (k * TPR + t) * VEC;
+			const bool in = r < d.n && c < W;
+			auto get = [&](int which, const T* p, uint64_t ld) {
+				return *reinterpret_cast<const Raw*>(RING ? row + which * row_bytes + c * sizeof(T) : (const unsigned char*)(p + r * ld + c));
+			};
+			rx[k] = in ? get(0, x, x_ld) : zero<Raw>();
+			ry[k] = in ? get(1, dy, dy_ld) : zero<Raw>();
+			rk[k] = in && add ? get(2, skip, skip_ld) : zero<Raw>();
+		}
+		if (RING) {
+			group_barrier<TPR>(group);  // the rows are in registers: their place is free
+			const uint64_t next = (uint64_t)r + (uint64_t)depth * step;
+			if (t == 0 && next < d.n) order(next, slot);
+			if (++slot == depth) slot = 0, parity ^= 1u;
+		}
 		float s1 = 0.f, s2 = 0.f;
 		float xh[E], a[E];
-		Raw rk[VPT];
 #pragma unroll
 		for (int k = 0; k < VPT; ++k) {
-			const uint32_t c = (k * TPR + t) * VEC;
 			float ex[VEC], ey[VEC];
 			P::get(rx[k], ex);
 			P::get(ry[k], ey);
-			if (skip && dx && r < d.n && c < W) rk[k] = *reinterpret_cast<const Raw*>(skip + r * skip_ld + c);
 #pragma unroll
 			for (int i = 0; i < VEC; ++i) {
 				const int e = k * VEC + i;
-				const bool in = r < d.n && c + i < W;
-				xh[e] = in ? (ex[i] - m) * sc : 0.f;
-				const float g = in ? ey[i] : 0.f;
-				dg[e] = fmaf(g, xh[e], dg[e]);
-				db[e] += g;
-				a[e] = g * ga[e];
+				xh[e] = (ex[i] - m) * sc, a[e] = ey[i] * ga[e];
+				dg[e] = fmaf(ey[i], xh[e], dg[e]);
+				db[e] += ey[i];
 				s1 += a[e];
 				s2 = fmaf(a[e], xh[e], s2);
 			}
 		}
-		fetch(r + gridDim.x * G);
 		if (dx) {
-			group_sum<TPR>(s1, s2, sums[group], group, turn);
+			group_sums<TPR>(s1, s2, sums[group], group, turn);
 			s1 *= inv_w, s2 *= inv_w;
 			if (r < d.n) {
 #pragma unroll
 				for (int k = 0; k < VPT; ++k) {
 					const uint32_t c = (k * TPR + t) * VEC;
-					float e[VEC], sk[VEC];
-					if (skip) P::get(rk[k], sk);
+					float v[VEC], sk[VEC];
+					P::get(rk[k], sk);
 #pragma unroll
-					for (int i = 0; i < VEC; ++i) {
-						e[i] = sc * (a[k * VEC + i] - s1 - xh[k * VEC + i] * s2);
-						if (skip) e[i] += sk[i];
-					}
-					if (c < W) *reinterpret_cast<Raw*>(dx + r * dx_ld + c) = P::put(e);
+					for (int i = 0; i < VEC; ++i) v[i] = fmaf(sc, a[k * VEC + i] - s1 - xh[k * VEC + i] * s2, sk[i]);
+					if (c < W) *reinterpret_cast<Raw*>(dx + r * dx_ld + c) = P::put(v);
 				}
 			}
 		}
 	}
 	if (!partial) return;
 	float* out = partial + (uint64_t)blockIdx.x * 2 * W;
-	if (G > 1) {
-		for (int g = 0; g < G; ++g) {
-			if (group == g) {
+	if constexpr (G > 1) {  // every thread's sums go to shared memory, and the block's threads share the columns
+		float* const all = reinterpret_cast<float*>(rings4);
+		__syncthreads();
 #pragma unroll
-				for (int k = 0; k < E; ++k) {
-					const int c = ((k / VEC) * TPR + t) * VEC + k % VEC;
-					if (g > 0) dg[k] += columns[c], db[k] += columns[TPR * E + c];
-					if (g < G - 1) columns[c] = dg[k], columns[TPR * E + c] = db[k];
-				}
-			}
-			__syncthreads();
+		for (int k = 0; k < E; ++k) all[k * B::kThreads + threadIdx.x] = dg[k], all[(E + k) * B::kThreads + threadIdx.x] = db[k];
+		__syncthreads();
+		for (int i = threadIdx.x; i < 2 * E * TPR; i += B::kThreads) {
+			const int k = i / TPR, e = k % E;
+			const uint32_t c = ((e / VEC) * TPR + i % TPR) * VEC + e % VEC;
+			float v = 0.f;
+#pragma unroll
+			for (int g = 0; g < G; ++g) v += all[k * B::kThreads + g * TPR + i % TPR];
+			if (c < W) out[(k < E ? 0 : W) + c] = v;
 		}
-		if (group != G - 1) return;
-	}
+	} else {
 #pragma unroll
-	for (int k = 0; k < E; ++k) {
-		const uint32_t c = ((k / VEC) * TPR + t) * VEC + k % VEC;
-		if (c < W) out[c] = dg[k], out[W + c] = db[k];
+			for (int k = 0; k < E; ++k) {
+			const uint32_t c = ((k / VEC) * TPR + t) * VEC + k % VEC;
+			if (c < W) out[c] = dg[k], out[W + c] = db[k];
+		}
 	}
 }
 
@@ -375,60 +570,97 @@ __global__ void __launch_bounds__(1024) wide_params_kernel(uint32_t n, uint32_t 
 }
 
 
-constexpr int kBackwardBlocks = 2 * kSMs;
 constexpr uint32_t kWidest = 8192;  // entries that a backward variant holds at most
-constexpr int kTooWide = -1000;  // no variant holds the row
+constexpr int kTooWide = -1000;     // no variant holds the row
 
 template <typename T, int VEC, int TPR, int VPT>
 struct Variant {
-	using Type = T;
 	static constexpr int kVec = VEC, kTpr = TPR, kVpt = VPT;
 };
 
-// The narrowest group that holds the row: a row of `width` entries is width / VEC accesses.  Forward pass: up to four accesses of 16
-// bytes a thread; backward pass: two, since a thread keeps five values for every entry.
+// The narrowest group that holds the row, `u` accesses of VEC entries, for rows that are read with plain loads: short ones, and those that
+// do not start on 16-byte boundaries (VEC 1).
 template <typename T, int VEC, typename F>
 int with_forward_variant(uint32_t width, F f) {
 	const uint32_t u = (width + VEC - 1) / VEC;
 	if (u <= 8) return f(Variant<T, VEC, 8, 1>());
 	if (u <= 16) return f(Variant<T, VEC, 16, 1>());
 	if (u <= 32) return f(Variant<T, VEC, 32, 1>());
-	if (u <= 64) return f(Variant<T, VEC, 32, 2>());
-	if (u <= 128) return f(Variant<T, VEC, 32, 4>());
-	if (u <= 256) return f(Variant<T, VEC, 128, 2>());
-	if (u <= 512) return f(Variant<T, VEC, 256, 2>());
-	if (u <= 1024) return f(Variant<T, VEC, 256, 4>());
-	if (u <= 2048) return f(Variant<T, VEC, 512, 4>());
-	if (VEC < 8 && u <= 4096) return f(Variant<T, VEC, VEC < 8 ? 1024 : 512, 4>());
-	if (VEC < 4 && u <= 8192) return f(Variant<T, VEC, VEC < 4 ? 1024 : 512, VEC < 4 ? 8 : 4>());
+	if constexpr (VEC == 1) {
+		if (u <= 64) return f(Variant<T, VEC, 32, 2>());
+		if (u <= 128) return f(Variant<T, VEC, 32, 4>());
+		if (u <= 256) return f(Variant<T, VEC, 32, 8>());
+		if (u <= 512) return f(Variant<T, VEC, 32, 16>());
+		if (u <= 1024) return f(Variant<T, VEC, 32, 32>());
+		if (u <= 2048) return f(Variant<T, VEC, 256, 8>());
+		if (u <= 4096) return f(Variant<T, VEC, 256, 16>());
+		if (u <= 8192) return f(Variant<T, VEC, 256, 32>());
+	}
+	if constexpr (VEC == 4) {  // too wide for a ring beside gamma and beta in shared memory
+		if (u > 2048 && u <= 4096) return f(Variant<T, VEC, 256, 16>());
+	}
 	return kTooWide;
 }
 template <typename T, int VEC, typename F>
 int with_backward_variant(uint32_t width, F f) {
 	const uint32_t u = (width + VEC - 1) / VEC;
-	constexpr int X = VEC == 8 ? 1 : VEC == 4 ? 2 : 4;  // accesses that make up 8 entries, 4 at most
 	if (u <= 8) return f(Variant<T, VEC, 8, 1>());
 	if (u <= 16) return f(Variant<T, VEC, 16, 1>());
 	if (u <= 32) return f(Variant<T, VEC, 32, 1>());
-	if (u <= 32 * X) return f(Variant<T, VEC, 32, X>());
-	if (u <= 64 * X) return f(Variant<T, VEC, 64, X>());
-	if (u <= 128 * X) return f(Variant<T, VEC, 128, X>());
-	if (u <= 256 * X) return f(Variant<T, VEC, 256, X>());
-	if (u <= 512 * X) return f(Variant<T, VEC, 256, 2 * X>());
-	if (u <= 1024 * X) return f(Variant<T, VEC, 512, 2 * X>());
+	if constexpr (VEC == 1) {
+		if (u <= 64) return f(Variant<T, VEC, 32, 2>());
+		if (u <= 128) return f(Variant<T, VEC, 32, 4>());
+		if (u <= 512) return f(Variant<T, VEC, 32, 16>());
+		if (u <= 1024) return f(Variant<T, VEC, 64, 16>());
+		if (u <= 2048) return f(Variant<T, VEC, 128, 16>());
+		if (u <= 4096) return f(Variant<T, VEC, 256, 16>());
+	}
 	return kTooWide;
 }
-// backward blocks, and so partial sums, of a call
-template <int TPR>
-static uint32_t backward_blocks(uint32_t n) {
-	const uint32_t need = (n + Geometry<TPR>::kGroups - 1) / Geometry<TPR>::kGroups;
-	return need < (uint32_t)kBackwardBlocks ? need : kBackwardBlocks;
+// Rows of 512 bytes and more are worth a bulk copy each.  The ring variants are those of the widths from there on.
+constexpr size_t kRingRow = 512;
+template <typename T, int VEC, typename F>
+int with_forward_ring(uint32_t width, F f) {
+	const uint32_t u = (width + VEC - 1) / VEC;
+	if (u <= 64) return f(Variant<T, VEC, 32, 2>());
+	if (u <= 128) return f(Variant<T, VEC, 32, 4>());
+	if (u <= 256) return f(Variant<T, VEC, 64, 4>());
+	if (u <= 512) return f(Variant<T, VEC, 128, 4>());
+	if (u <= 1024) return f(Variant<T, VEC, 256, 4>());
+	if (u <= 2048) return f(Variant<T, VEC, 512, 4>());
+	return kTooWide;
+}
+template <typename T, int VEC, typename F>
+int with_backward_ring(uint32_t width, F f) {
+	const uint32_t u = (width + VEC - 1) / VEC;
+	constexpr int M = VEC == 8 ? 2 : 4;  // 16 entries a thread
+	if (u <= 32 * M) return f(Variant<T, VEC, 32, M>());
+	if (u <= 64 * M) return f(Variant<T, VEC, 64, M>());
+	if (u <= 128 * M) return f(Variant<T, VEC, 128, M>());
+	if (u <= 256 * M) return f(Variant<T, VEC, 256, M>());
+	if (u <= 512 * M) return f(Variant<T, VEC, 512, M>());
+	return kTooWide;
+}
+// rows ahead of a group, `round` bytes for one of every group: as many as fit, 4 at most
+static int ring_depth(size_t fixed, size_t round) {
+	const size_t room = 216 * 1024;
+	const size_t d = fixed < room ? (room - fixed) / round : 0;
+	return d < 4 ? (int)d : 4;
 }
 static bool rows16(const void* p, uint64_t ld, size_t bytes) { return !p || (((uintptr_t)p | (ld * bytes)) & 15) == 0; }
 
 }  // namespace ln
 
 using namespace ln;
+
+int read_layer_norm_error(uint32_t* flags) {
+	const cudaError_t e = cudaMemcpyFromSymbol(flags, ln::g_error, sizeof(*flags));
+	return e == cudaSuccess ? NEUS2B_OK : (int)e;
+}
+int write_layer_norm_error(uint32_t flags) {
+	const cudaError_t e = cudaMemcpyToSymbol(ln::g_error, &flags, sizeof(flags));
+	return e == cudaSuccess ? NEUS2B_OK : (int)e;
+}
 
 static int check_desc(const neus2b_layer_norm_desc* d) {
 	if (!d || d->width == 0 || !(d->epsilon > 0.f) || isinf(d->epsilon)) return NEUS2B_E_INVALID;
@@ -452,18 +684,39 @@ extern "C" int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, con
 	return with_float_type(desc->dtype, [&](auto t) {
 		using T = decltype(t);
 		constexpr int V = 16 / sizeof(T);
-		auto go = [&](auto v) {
+		const size_t row = desc->width * b;
+		auto go = [&](auto v, auto ring) {
 			using K = decltype(v);
-			constexpr int G = Geometry<K::kTpr>::kGroups;
-			auto kernel = forward_kernel<T, K::kVec, K::kTpr, K::kVpt>;
-			const uint32_t need = (desc->n + G - 1) / G, most = kSMs * (2048 / Geometry<K::kTpr>::kThreads);
-			kernel<<<need < most ? need : most, Geometry<K::kTpr>::kThreads, 0, stream>>>(*desc, (const T*)d_x, x_stride, d_gamma, d_beta, (T*)d_y, y_stride, d_mean,
-			                                                                          d_rstd);
+			using F = Forward<T, K::kVec, K::kTpr, K::kVpt, decltype(ring)::value>;
+			auto kernel = forward_kernel<T, K::kVec, K::kTpr, K::kVpt, decltype(ring)::value>;
+			size_t smem = F::kStaged ? 2 * K::kTpr * K::kVpt * K::kVec * sizeof(float) : 0;
+			int depth = 0;
+			if (ring) {
+				depth = ring_depth(smem, F::kGroups * row);
+				if (!depth) return kTooWide;
+				smem += (size_t)F::kGroups * row * depth;
+			}
+			if (smem > 32 * 1024) N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+			int resident = 1;
+			if (!ring) {
+				static const int most = [&] {
+					int q = 0;
+					return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&q, kernel, F::kThreads, smem) == cudaSuccess && q > 0 ? q : F::kBlocks;
+				}();
+				resident = most;
+			}
+			const uint32_t need = (desc->n + F::kGroups - 1) / F::kGroups, most = kSMs * resident;
+			kernel<<<need < most ? need : most, F::kThreads, smem, stream>>>(*desc, depth, (const T*)d_x, x_stride, d_gamma, d_beta, (T*)d_y, y_stride, d_mean, d_rstd);
 			N2B_CHECK_LAUNCH();
 			return NEUS2B_OK;
 		};
 		const bool vec = rows16(d_x, x_stride, b) && rows16(d_y, y_stride, b) && desc->width % V == 0;
-		const int rc = vec ? with_forward_variant<T, V>(desc->width, go) : with_forward_variant<T, 1>(desc->width, go);
+		int rc = kTooWide;
+		if (vec && row >= kRingRow) rc = with_forward_ring<T, V>(desc->width, [&](auto v) { return go(v, std::true_type()); });
+		if (rc == kTooWide) {
+			auto plain = [&](auto v) { return go(v, std::false_type()); };
+			rc = vec ? with_forward_variant<T, V>(desc->width, plain) : with_forward_variant<T, 1>(desc->width, plain);
+		}
 		if (rc != kTooWide) return rc;
 		wide_forward_kernel<T><<<desc->n < 8u * kSMs ? desc->n : 8u * kSMs, 256, 0, stream>>>(*desc, (const T*)d_x, x_stride, d_gamma, d_beta, (T*)d_y,
 		                                                                                 y_stride, d_mean, d_rstd);
@@ -475,8 +728,8 @@ extern "C" int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, con
 extern "C" int neus2b_layer_norm_backward_workspace(const neus2b_layer_norm_desc* desc, uint64_t* bytes) {
 	if (int rc = check_desc(desc)) return rc;
 	if (!bytes) return NEUS2B_E_INVALID;
-	// the most blocks that any variant runs: narrow groups share a block, so no variant has more than this
-	const uint64_t blocks = desc->n < (uint32_t)kBackwardBlocks ? desc->n : kBackwardBlocks;
+	// the most blocks that any variant runs
+	const uint64_t blocks = desc->n < 8u * kSMs ? desc->n : 8u * kSMs;
 	*bytes = desc->width <= kWidest ? blocks * 2 * desc->width * sizeof(float) : 0;
 	return NEUS2B_OK;
 }
@@ -510,15 +763,26 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 		const bool params = d_dgamma || d_dbeta;
 		const int accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
 		if (!params && !d_dL_dx) return NEUS2B_OK;
-		auto go = [&](auto v) {
+		const size_t row = width * b;
+		auto go = [&](auto v, auto ring) {
 			using K = decltype(v);
-			constexpr int G = Geometry<K::kTpr>::kGroups;
-			const uint32_t blocks = backward_blocks<K::kTpr>(n);
-			const size_t smem = G > 1 ? 2 * K::kTpr * K::kVpt * K::kVec * sizeof(float) : 0;
-			auto kernel = backward_kernel<T, K::kVec, K::kTpr, K::kVpt>;
-			kernel<<<blocks, Geometry<K::kTpr>::kThreads, smem, stream>>>(*desc, (const T*)d_x, x_stride, d_gamma, d_mean, d_rstd, (const T*)d_dL_dy, dy_stride,
-			                                                            (const T*)d_skip, skip_stride, (T*)d_dL_dx, dx_stride,
-			                                                            params ? (float*)d_workspace : nullptr);
+			using B = Backward<K::kTpr, K::kVpt * K::kVec, decltype(ring)::value>;
+			static_assert(B::kGrid <= 8 * kSMs, "the workspace holds 8 blocks a SM");
+			const uint32_t need = (n + B::kGroups - 1) / B::kGroups, blocks = need < (uint32_t)B::kGrid ? need : B::kGrid;
+			constexpr size_t kSums = B::kGroups > 1 ? 2 * K::kVpt * K::kVec * B::kThreads * sizeof(float) : 0;
+			size_t smem = 0;
+			const size_t slot = row * (d_skip && d_dL_dx ? 3 : 2) * B::kGroups;
+			int depth = 0;
+			if (ring) {
+				depth = ring_depth(smem, slot);
+				if (!depth) return kTooWide;
+				smem += slot * depth;
+			}
+			smem = smem > kSums ? smem : kSums;
+			auto kernel = backward_kernel<T, K::kVec, K::kTpr, K::kVpt, decltype(ring)::value>;
+			if (smem > 32 * 1024) N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+			kernel<<<blocks, B::kThreads, smem, stream>>>(*desc, depth, (const T*)d_x, x_stride, d_gamma, d_mean, d_rstd, (const T*)d_dL_dy, dy_stride,
+			                                              (const T*)d_skip, skip_stride, (T*)d_dL_dx, dx_stride, params ? (float*)d_workspace : nullptr);
 			N2B_CHECK_LAUNCH();
 			if (params) {
 				join_kernel<<<(2 * width + 31) / 32, dim3(32, 32), 0, stream>>>((const float*)d_workspace, blocks, width, d_dgamma, d_dbeta, accumulate);
@@ -527,7 +791,12 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 			return NEUS2B_OK;
 		};
 		const bool vec = rows16(d_x, x_stride, b) && rows16(d_dL_dy, dy_stride, b) && rows16(d_skip, skip_stride, b) && rows16(d_dL_dx, dx_stride, b) && width % V == 0;
-		const int rc = vec ? with_backward_variant<T, V>(width, go) : with_backward_variant<T, 1>(width, go);
+		int rc = kTooWide;
+		if (vec && row >= kRingRow) rc = with_backward_ring<T, V>(width, [&](auto v) { return go(v, std::true_type()); });
+		if (rc == kTooWide) {
+			auto plain = [&](auto v) { return go(v, std::false_type()); };
+			rc = vec ? with_backward_variant<T, V>(width, plain) : with_backward_variant<T, 1>(width, plain);
+		}
 		if (rc != kTooWide) return rc;
 		if (params) {  // ahead of the input gradient, which may overwrite dL/dy
 			wide_params_kernel<T><<<(width + 31) / 32, dim3(32, 32), 0, stream>>>(n, width, (const T*)d_x, x_stride, d_mean, d_rstd, (const T*)d_dL_dy,
