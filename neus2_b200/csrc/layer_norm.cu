@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 		}
 	} else {
 #pragma unroll
-			for (int k = 0; k < E; ++k) {
+		for (int k = 0; k < E; ++k) {
 			const uint32_t c = ((k / VEC) * TPR + t) * VEC + k % VEC;
 			if (c < W) out[c] = dg[k], out[W + c] = db[k];
 		}

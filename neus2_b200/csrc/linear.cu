@@ -21,9 +21,10 @@ static bool bad_matrix(const void* p, uint64_t stride, uint32_t width, size_t al
 static bool bad_optional(const void* p, uint64_t stride, uint32_t width, size_t align) { return p && bad_matrix(p, stride, width, align); }
 
 static bool on16(const void* p, uint64_t ld, size_t bytes) { return !p || (((uintptr_t)p | (ld * bytes)) & 15) == 0; }
-// Whether every row that the epilogue touches starts on a 16-byte boundary.
-static int whole_vectors(const Epilogue& e) {
-	return on16(e.out, e.out_ld, e.out_f32 ? 4 : 2) && on16(e.bias, 0, 2) && on16(e.add, e.add_ld, 2) && on16(e.slope_z, e.slope_ld, 2) &&
+// Whether the epilogue may move 16 bytes at a time: every row that it touches starts on a 16-byte boundary, and rows of 16-bit values
+// are whole numbers of accesses (an fp32 row's end is handled apart).
+static int whole_vectors(const Epilogue& e, uint32_t width) {
+	return (e.out_f32 || width % 8 == 0) && on16(e.out, e.out_ld, e.out_f32 ? 4 : 2) && on16(e.bias, 0, 2) && on16(e.add, e.add_ld, 2) && on16(e.slope_z, e.slope_ld, 2) &&
 	       on16(e.preact, e.preact_ld, 2);
 }
 
@@ -48,7 +49,7 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	Epilogue& e = p.e;
 	e.out = d_y, e.out_ld = y_stride, e.bias = d_bias, e.add = d_residual, e.add_ld = residual_stride;
 	e.preact = d_preact, e.preact_ld = preact_stride, e.act = (int)desc->activation;
-	e.vec = whole_vectors(e);
+	e.vec = whole_vectors(e, out);
 	return run_product(p, stream);
 }
 
@@ -111,7 +112,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		p.M = out, p.N = d_wgrad ? in : sums_only_width(out), p.K = n;
 		p.a_mn = p.b_mn = true;
 		p.e.out = d_wgrad, p.e.out_ld = in, p.e.out_f32 = 1, p.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
-		p.e.vec = whole_vectors(p.e);
+		p.e.vec = whole_vectors(p.e, in);
 		p.column_sums = d_bgrad;
 		p.workspace = (char*)d_workspace + dz_bytes(desc), p.workspace_bytes = workspace_bytes - dz_bytes(desc);
 		if (int rc = run_weight_gradient(p, stream)) return rc;
@@ -123,7 +124,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		p.e = Epilogue{};
 		p.e.out = d_dL_dx, p.e.out_ld = dx_stride, p.e.add = d_skip, p.e.add_ld = skip_stride;
 		if (below_activation != NEUS2B_ACT_NONE) p.e.slope_z = d_below_preact, p.e.slope_ld = below_stride, p.e.act = (int)below_activation;
-		p.e.vec = whole_vectors(p.e);
+		p.e.vec = whole_vectors(p.e, in);
 		if (int rc = run_product(p, stream)) return rc;
 	}
 	return NEUS2B_OK;

@@ -34,35 +34,6 @@ __device__ __forceinline__ float h2f(uint16_t v, bool bf) { return bf ? __uint_a
 __device__ __forceinline__ uint16_t f2h(float v, bool bf) {
 	return bf ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
-__device__ __forceinline__ void unpack8(const uint4& p, bool bf, float (&v)[8]) {
-	const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-	for (int i = 0; i < 4; ++i) {
-		if (bf) {
-			v[2 * i] = __uint_as_float(w[i] << 16);
-			v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-		} else {
-			const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-			v[2 * i] = f.x;
-			v[2 * i + 1] = f.y;
-		}
-	}
-}
-__device__ __forceinline__ uint4 pack8(const float (&v)[8], bool bf) {
-	uint32_t w[4];
-#pragma unroll
-	for (int i = 0; i < 4; ++i) {
-		if (bf) {
-			const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-			w[i] = *reinterpret_cast<const uint32_t*>(&h);
-		} else {
-			const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-			w[i] = *reinterpret_cast<const uint32_t*>(&h);
-		}
-	}
-	return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // one sum, sample r, feature c
 __device__ __forceinline__ void finish_one(const Epilogue& e, bool bf, uint64_t r, uint32_t c, float v) {
 	if (e.out_f32) {
@@ -77,53 +48,15 @@ __device__ __forceinline__ void finish_one(const Epilogue& e, bool bf, uint64_t 
 	((uint16_t*)e.out)[r * e.out_ld + c] = f2h(v, bf);
 }
 
-// eight sums, sample r, features c .. c + 7, all of them inside and on 16-byte boundaries
-__device__ __forceinline__ void finish_eight(const Epilogue& e, bool bf, uint64_t r, uint32_t c, float (&v)[8]) {
-	if (e.out_f32) {
-		float4* o = reinterpret_cast<float4*>((float*)e.out + r * e.out_ld + c);
-		if (e.accumulate) {
-			const float4 a = o[0], b = o[1];
-			v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-		}
-		o[0] = make_float4(v[0], v[1], v[2], v[3]);
-		o[1] = make_float4(v[4], v[5], v[6], v[7]);
-		return;
+// eight fp32 sums of a weight gradient's row, all of them inside and on a 16-byte boundary
+__device__ __forceinline__ void store_eight(const Epilogue& e, uint64_t r, uint32_t c, float (&v)[8]) {
+	float4* o = reinterpret_cast<float4*>((float*)e.out + r * e.out_ld + c);
+	if (e.accumulate) {
+		const float4 a = o[0], b = o[1];
+		v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
 	}
-	float t[8];
-	if (e.bias) {
-		unpack8(__ldg(reinterpret_cast<const uint4*>((const uint16_t*)e.bias + c)), bf, t);
-#pragma unroll
-		for (int i = 0; i < 8; ++i) v[i] += t[i];
-	}
-	if (e.preact) *reinterpret_cast<uint4*>((uint16_t*)e.preact + r * e.preact_ld + c) = pack8(v, bf);
-	if (e.slope_z) {
-		unpack8(__ldg(reinterpret_cast<const uint4*>((const uint16_t*)e.slope_z + r * e.slope_ld + c)), bf, t);
-		if (e.act == NEUS2B_ACT_RELU) {
-#pragma unroll
-			for (int i = 0; i < 8; ++i) v[i] *= act_slope(NEUS2B_ACT_RELU, t[i]);
-		} else if (e.act == NEUS2B_ACT_GELU) {
-#pragma unroll
-			for (int i = 0; i < 8; ++i) v[i] *= act_slope(NEUS2B_ACT_GELU, t[i]);
-		} else if (e.act == NEUS2B_ACT_SILU) {
-#pragma unroll
-			for (int i = 0; i < 8; ++i) v[i] *= act_slope(NEUS2B_ACT_SILU, t[i]);
-		}
-	} else if (e.act == NEUS2B_ACT_RELU) {
-#pragma unroll
-		for (int i = 0; i < 8; ++i) v[i] = act_value(NEUS2B_ACT_RELU, v[i]);
-	} else if (e.act == NEUS2B_ACT_GELU) {
-#pragma unroll
-		for (int i = 0; i < 8; ++i) v[i] = act_value(NEUS2B_ACT_GELU, v[i]);
-	} else if (e.act == NEUS2B_ACT_SILU) {
-#pragma unroll
-		for (int i = 0; i < 8; ++i) v[i] = act_value(NEUS2B_ACT_SILU, v[i]);
-	}
-	if (e.add) {
-		unpack8(*reinterpret_cast<const uint4*>((const uint16_t*)e.add + r * e.add_ld + c), bf, t);  // may be the output itself
-#pragma unroll
-		for (int i = 0; i < 8; ++i) v[i] += t[i];
-	}
-	*reinterpret_cast<uint4*>((uint16_t*)e.out + r * e.out_ld + c) = pack8(v, bf);
+	o[0] = make_float4(v[0], v[1], v[2], v[3]);
+	o[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
 // width of the product that carries the column sums where no weight gradient is wanted (it is not stored)

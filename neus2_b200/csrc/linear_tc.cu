@@ -16,9 +16,8 @@ namespace lin {
 static __device__ uint32_t g_error;  // bit 0: a bounded wait ran out
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpiWarps = 8, kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kGatherWarps = 7;  // warps 9..15
-constexpr int kMaxStages = 8, kSmemBudget = 200 * 1024;
+constexpr int kGatherWarps = 7;
+constexpr int kMaxStages = 8, kSmemMost = 227 * 1024;
 constexpr int kChunk = 8;  // weight gradient: k blocks (512 samples) summed in tensor memory before the sum moves to registers
 
 struct alignas(64) Args {
@@ -64,11 +63,58 @@ __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.ar
 __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
 	asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// x: first column (a multiple of 64), y: first row of a [rows][columns] matrix
+// x: first column (a multiple of 64), y: first row of a [rows][columns] matrix.  PAIR: the barrier may be the other CTA's.
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-	asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
-	             "r"(x), "r"(y), "r"(bar)
-	             : "memory");
+	if (PAIR)
+		asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+		             "r"(x), "r"(y), "r"(bar)
+		             : "memory");
+	else
+		asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+		             "r"(x), "r"(y), "r"(bar)
+		             : "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
+	uint32_t p;
+	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+	return p;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
+	if (PAIR) {
+		asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+	} else {
+		tc::tmem_alloc(dst, cols);
+	}
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
+	if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+	else tc::tmem_dealloc(addr, cols);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t more) {
+	if (PAIR)
+		asm volatile(
+		    "{\n\t.reg .pred p;\n\t"
+		    "setp.ne.b32 p, %4, 0;\n\t"
+		    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+		    :
+		    : "r"(d), "l"(a), "l"(b), "r"(id), "r"(more)
+		    : "memory");
+	else tc::mma_f16(d, a, b, id, more);
+}
+// PAIR: arrives at the barrier of this place in both CTAs.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+	if (PAIR)
+		asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+	else tc::commit(bar);
 }
 // Matrix descriptors of the two 128-byte-swizzled layouts.  K-major: rows of 64 k, 8-row groups 1024 bytes apart.  MN-major: rows of
 // 64 m (or n), one per k, 8-row groups 1024 bytes apart, slabs of 64 m 8192 bytes apart.
@@ -100,111 +146,229 @@ __device__ __forceinline__ void cluster_sync() {
 	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
-	uint32_t p;
 	float v;
-	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-	asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
+	asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(addr, rank)) : "memory");
 	return v;
 }
 
-// Eight 16-bit values that start at any even address, as two aligned 16-byte loads and a shift.
-__device__ __forceinline__ uint4 shifted_load(const char* p) {
-	const uint32_t s = (uint32_t)(uintptr_t)p & 15u;
-	const uint4* q = reinterpret_cast<const uint4*>(p - s);
-	const uint4 lo = __ldg(q);
-	if (s == 0) return lo;
-	const uint4 hi = __ldg(q + 1);
-	uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-	if (s & 8u) {
-#pragma unroll
-		for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-	}
-	if (s & 4u) {
-#pragma unroll
-		for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-	}
-	const uint32_t b = (s & 2u) * 8u;
-	return make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b), __funnelshift_r(w[2], w[3], b), __funnelshift_r(w[3], w[4], b));
-}
-// `count` rows of 64 columns from (row0, col0) of a [rows][cols] matrix of any alignment into a swizzled tile; zeros outside.
-// The two aligned loads of a piece may reach up to 14 bytes around it: they are used only where that stays inside the matrix's
-// extent in memory, which is the caller's.
+// ROWS rows of 64 columns from (row0, col0) of a [rows][cols] matrix of any alignment into a swizzled tile; zeros outside.  Eight values
+// that start at any even address are two aligned 16-byte loads and a shift.  The loads may reach up to 14 bytes around the values: they
+// are used only where that stays inside the matrix's extent in memory, which is the caller's.  All loads of a thread (four pieces at a
+// time) are in flight before the first is used.
+template <int ROWS>
 __device__ __forceinline__ void gather_box(unsigned char* dst, const uint16_t* base, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t row0, uint32_t col0,
-                                           int count, int tid) {
+                                           int tid) {
+	constexpr int kThreads = kGatherWarps * 32, kBatch = 4;
 	const char* begin = reinterpret_cast<const char*>(base);
 	const char* end = begin + ((uint64_t)(rows - 1) * ld + cols) * 2;
-	for (int u = tid; u < count * 8; u += kGatherWarps * 32) {
-		const int r = u >> 3, c8 = u & 7;
-		const uint32_t row = row0 + r, col = col0 + c8 * 8;
-		uint4 v = make_uint4(0, 0, 0, 0);
-		if (row < rows && col < cols) {
-			const uint16_t* p = base + (uint64_t)row * ld + col;
-			const char* q = reinterpret_cast<const char*>(p);
-			const char* lo = q - ((uintptr_t)q & 15u);
-			if (col + 8 <= cols && lo >= begin && lo + 32 <= end) {
-				v = shifted_load(q);
-			} else {
-				uint32_t w[4] = {0, 0, 0, 0};
+	for (int u0 = tid; u0 < ROWS * 8; u0 += kBatch * kThreads) {
+		uint4 lo[kBatch], hi[kBatch];
 #pragma unroll
-				for (int i = 0; i < 8; ++i)
-					if (col + i < cols) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-				v = make_uint4(w[0], w[1], w[2], w[3]);
+		for (int j = 0; j < kBatch; ++j) {
+			const int u = u0 + j * kThreads;
+			const uint32_t row = row0 + (u >> 3), col = col0 + (u & 7) * 8;
+			lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
+			if (u < ROWS * 8 && row < rows && col < cols) {
+				const uint16_t* p = base + (uint64_t)row * ld + col;
+				const char* q = reinterpret_cast<const char*>(p);
+				const char* down = q - ((uintptr_t)q & 15u);
+				if (col + 8 <= cols && down >= begin && down + 32 <= end) {
+					lo[j] = __ldg(reinterpret_cast<const uint4*>(down));
+					hi[j] = __ldg(reinterpret_cast<const uint4*>(down) + 1);
+				} else {  // at the matrix's edges: entry by entry, put where the aligned loads would have put them
+					uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+					const uint32_t first = ((uint32_t)(uintptr_t)q & 15u) >> 1;
+#pragma unroll
+					for (int i = 0; i < 16; ++i)
+						if ((uint32_t)i >= first && (uint32_t)i < first + 8u && col + (i - first) < cols) w[i >> 1] |= (uint32_t)p[i - first] << (16 * (i & 1));
+					lo[j] = make_uint4(w[0], w[1], w[2], w[3]);
+					hi[j] = make_uint4(w[4], w[5], w[6], w[7]);
+				}
 			}
 		}
-		*reinterpret_cast<uint4*>(dst + r * 128 + ((c8 ^ (r & 7)) << 4)) = v;
+#pragma unroll
+		for (int j = 0; j < kBatch; ++j) {
+			const int u = u0 + j * kThreads;
+			if (u >= ROWS * 8) break;
+			const uint32_t row = row0 + (u >> 3), col = col0 + (u & 7) * 8;
+			const uint32_t s = (uint32_t)(uintptr_t)(base + (uint64_t)row * ld + col) & 15u;
+			uint32_t w[8] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w, hi[j].x, hi[j].y, hi[j].z, hi[j].w};
+			if (s & 8u) {
+#pragma unroll
+				for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+			}
+			if (s & 4u) {
+#pragma unroll
+				for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+			}
+			const uint32_t b = (s & 2u) * 8u;
+			const int r = u >> 3, c8 = u & 7;
+			*reinterpret_cast<uint4*>(dst + r * 128 + ((c8 ^ (r & 7)) << 4)) =
+			    make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b), __funnelshift_r(w[2], w[3], b), __funnelshift_r(w[3], w[4], b));
+		}
 	}
 }
 
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER>
+// What a block of one variant is made of.  PAIR: two CTAs of a cluster compute a 256 x BN tile together, each with 128 of its rows in its
+// tensor memory and half of B's tile in its shared memory.  Narrow tiles (BN 64) finish faster than one group of warps can write
+// them: four groups take turns, each with an accumulator of its own; wide ones are shared by two halves of the warps.
+template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
 struct Shape {
+	static constexpr int kBRows = PAIR ? BN / 2 : BN;  // of B's tile in this CTA
 	static constexpr int kABytes = kBM * 128;
-	static constexpr int kBBytes = (BMN && BN < 64 ? 64 : BN) * 128;
+	static constexpr int kBBytes = (BMN && kBRows < 64 ? 64 : kBRows) * 128;
 	static constexpr int kStage = kABytes + kBBytes;
-	static constexpr int kStages = kSmemBudget / kStage < kMaxStages ? kSmemBudget / kStage : kMaxStages;
-	static constexpr int kSmem = kStages * kStage + 2048 + 1024;  // ones tile and barriers; alignment of the base
-	static constexpr int kTmem = WGRAD ? 512 : (2 * BN < 32 ? 32 : 2 * BN);
+	static constexpr bool kTurns = BN == 64 && !SWAP && !WGRAD;
+	static constexpr int kHalves = kTurns ? 1 : 2, kGroups = kTurns ? (GATHER ? 2 : 4) : 1, kBufs = kTurns ? 4 : 2;
+	static constexpr int kEpiWarps = 4 * kHalves * kGroups, kMmaWarp = kEpiWarps, kLoadWarp = kEpiWarps + 1;
 	static constexpr int kThreads = (GATHER ? kLoadWarp + kGatherWarps : kLoadWarp + 1) * 32;
+	static constexpr int kBounce = SWAP || WGRAD ? 0 : kEpiWarps * 2048;  // 32 rows of 32 values for every epilogue warp
+	static constexpr int kFixed = kBounce + 2048 + 1024;                  // ones tile and barriers; alignment of the base
+	static constexpr int kRoom = (kSmemMost - kFixed) / kStage;
+	static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;
+	static constexpr int kSmem = kStages * kStage + kFixed;
+	static constexpr int kCols = kBufs * BN + (WGRAD && !PAIR ? 32 : 0);
+	static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER>
-__global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThreads, 1) product_kernel(const __grid_constant__ Args p) {
-	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>;
+// ---- 32 x 32 values of a matrix between global memory and registers, through a warp's 2 KB of shared memory.  Global memory is read
+// and written in whole row segments (64 bytes), a thread computes on one row.  Where rows do not start on 16-byte boundaries a thread
+// moves one column's values one by one: still one segment of a row per instruction.  The 16-byte units of a row are permuted so that
+// neither side's accesses collide.
+struct Chunk {
+	uint32_t w[16];
+};
+__device__ __forceinline__ uint32_t unit_at(int row, int unit) { return (uint32_t)(row * 64 + ((unit ^ ((row >> 1) & 3)) << 4)); }
+__device__ __forceinline__ void chunk_load(Chunk& k, const void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols, int vec, int lane) {
+	const uint16_t* p = (const uint16_t*)base;
+	if (vec) {
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			const uint32_t r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
+			uint4 v = make_uint4(0, 0, 0, 0);
+			if (r < rows && c < cols) v = *reinterpret_cast<const uint4*>(p + (uint64_t)r * ld + c);
+			k.w[4 * i] = v.x, k.w[4 * i + 1] = v.y, k.w[4 * i + 2] = v.z, k.w[4 * i + 3] = v.w;
+		}
+	} else {
+#pragma unroll
+		for (int i = 0; i < 16; ++i) {
+			const uint32_t r = row0 + 2 * i, c = col0 + lane;
+			const uint32_t lo = r < rows && c < cols ? p[(uint64_t)r * ld + c] : 0u, hi = r + 1 < rows && c < cols ? p[(uint64_t)(r + 1) * ld + c] : 0u;
+			k.w[i] = lo | hi << 16;
+		}
+	}
+}
+// The thread's own row of a chunk that was loaded above.
+__device__ __forceinline__ void chunk_to_row(const Chunk& k, uint32_t (&row)[16], unsigned char* bounce, int vec, int lane) {
+	if (vec) {
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+			*reinterpret_cast<uint4*>(bounce + unit_at(i * 8 + (lane >> 2), lane & 3)) = make_uint4(k.w[4 * i], k.w[4 * i + 1], k.w[4 * i + 2], k.w[4 * i + 3]);
+	} else {
+#pragma unroll
+		for (int i = 0; i < 32; ++i)
+			*reinterpret_cast<uint16_t*>(bounce + unit_at(i, lane >> 3) + (lane & 7) * 2) = (uint16_t)(k.w[i >> 1] >> (16 * (i & 1)));
+	}
+	__syncwarp();
+#pragma unroll
+	for (int u = 0; u < 4; ++u) {
+		const uint4 v = *reinterpret_cast<const uint4*>(bounce + unit_at(lane, u));
+		row[4 * u] = v.x, row[4 * u + 1] = v.y, row[4 * u + 2] = v.z, row[4 * u + 3] = v.w;
+	}
+	__syncwarp();
+}
+__device__ __forceinline__ void row_to_global(const uint32_t (&row)[16], void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols,
+                                              unsigned char* bounce, int vec, int lane) {
+	uint16_t* p = (uint16_t*)base;
+#pragma unroll
+	for (int u = 0; u < 4; ++u)
+		*reinterpret_cast<uint4*>(bounce + unit_at(lane, u)) = make_uint4(row[4 * u], row[4 * u + 1], row[4 * u + 2], row[4 * u + 3]);
+	__syncwarp();
+	if (vec) {
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			const uint32_t r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
+			const uint4 v = *reinterpret_cast<const uint4*>(bounce + unit_at(i * 8 + (lane >> 2), lane & 3));
+			if (r < rows && c < cols) *reinterpret_cast<uint4*>(p + (uint64_t)r * ld + c) = v;
+		}
+	} else {
+#pragma unroll
+		for (int i = 0; i < 32; ++i) {
+			const uint16_t v = *reinterpret_cast<const uint16_t*>(bounce + unit_at(i, lane >> 3) + (lane & 7) * 2);
+			if (row0 + i < rows && col0 + lane < cols) p[(uint64_t)(row0 + i) * ld + col0 + lane] = v;
+		}
+	}
+	__syncwarp();
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf) {
+	return bf ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf) {
+	if (bf) {
+		const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+		return *reinterpret_cast<const uint32_t*>(&h);
+	}
+	const __half2 h = __floats2half2_rn(a, b);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int ACT>
+__device__ __forceinline__ void apply_act(float (&v)[32]) {
+#pragma unroll
+	for (int i = 0; i < 32; ++i) v[i] = act_value(ACT, v[i]);
+}
+template <int ACT>
+__device__ __forceinline__ void apply_slope(float (&v)[32], const uint32_t (&z)[16], bool bf) {
+#pragma unroll
+	for (int i = 0; i < 16; ++i) {
+		const float2 f = unpack2(z[i], bf);
+		v[2 * i] *= act_slope(ACT, f.x);
+		v[2 * i + 1] *= act_slope(ACT, f.y);
+	}
+}
+
+template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
+__global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>::kThreads, 1) product_kernel(const __grid_constant__ Args p) {
+	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
 	extern __shared__ unsigned char smem_raw[];
 	unsigned char* smem = smem_raw + ((1024u - (sptr(smem_raw) & 1023u)) & 1023u);
-	unsigned char* ones = smem + S::kStages * S::kStage;  // 512 bytes: a [16][16] tile of 1.0
+	unsigned char* bounces = smem + S::kStages * S::kStage;
+	unsigned char* ones = bounces + S::kBounce;  // 512 bytes: a [16][16] tile of 1.0
 	uint64_t* bars = reinterpret_cast<uint64_t*>(ones + 1024);
 	uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(ones + 2048 - 16);
-	const uint32_t full = sptr(bars), empty = full + 8 * kMaxStages, tfull = empty + 8 * kMaxStages, tempty = tfull + 16;
+	const uint32_t full = sptr(bars), empty = full + 8 * kMaxStages, tfull = empty + 8 * kMaxStages, tempty = tfull + 8 * 4;
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 	const bool bf = p.bf16 != 0;
+	const uint32_t rank = PAIR || p.cluster > 1 ? cluster_rank() : 0u;
 
 	if (tid == 0) {
 		for (int i = 0; i < S::kStages; ++i) {
 			tc::mbar_init(full + 8 * i, GATHER ? kGatherWarps * 32 : 1);
 			tc::mbar_init(empty + 8 * i, 1);
 		}
-		for (int i = 0; i < 2; ++i) {
+		for (int i = 0; i < S::kBufs; ++i) {
 			tc::mbar_init(tfull + 8 * i, 1);
-			tc::mbar_init(tempty + 8 * i, kEpiWarps);
+			tc::mbar_init(tempty + 8 * i, 4 * S::kHalves * (PAIR ? 2 : 1));
 		}
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 	}
 	if (WGRAD)
 		for (int i = tid; i < 256; i += S::kThreads) reinterpret_cast<uint16_t*>(ones)[i] = bf ? 0x3f80u : 0x3c00u;
 	tc::fence_async_smem();
-	if (warp == 0) tc::tmem_alloc(sptr(tmem_ptr), S::kTmem);
+	if (warp == 0) tmem_alloc<PAIR>(sptr(tmem_ptr), S::kTmem);
 	tc::fence_before_sync();
-	__syncthreads();
+	if (PAIR) cluster_sync();
+	else __syncthreads();
 	tc::fence_after_sync();
 	const uint32_t tmem = *tmem_ptr;
 
+	// A cluster that splits k computes one tile; a pair, or a CTA by itself, takes every `step`-th.
 	const uint32_t tiles = p.tiles_m * p.tiles_n, kblocks = (p.K + kBK - 1) / kBK;
-	const uint32_t rank = p.cluster > 1 ? cluster_rank() : 0u;
-	const uint32_t first = p.cluster > 1 ? (blockIdx.x / p.cluster) + rank * tiles : blockIdx.x;
-	const uint32_t step = p.cluster > 1 ? tiles * p.splits : gridDim.x;  // a cluster computes one tile
+	const uint32_t first = PAIR ? blockIdx.x / 2 : p.cluster > 1 ? (blockIdx.x / p.cluster) + rank * tiles : blockIdx.x;
 	const uint32_t units = tiles * p.splits;
+	const uint32_t step = PAIR ? gridDim.x / 2 : p.cluster > 1 ? units : gridDim.x;
+	const uint32_t row_offset = PAIR ? rank * kBM : 0u;
+	constexpr int kTileM = PAIR ? 2 * kBM : kBM;
 	bool ok = true;
-	uint32_t last_m = 0, last_n = 0;
 
 	// unit -> tile and k range.  Tiles go down 16 rows of tiles before they move to the next column: what runs at one time shares operands.
 	auto locate = [&](uint32_t u, uint32_t& mt, uint32_t& nt, uint32_t& split, uint32_t& kb0, uint32_t& kb1) {
@@ -217,62 +381,66 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 		kb1 = (uint32_t)((uint64_t)(split + 1) * kblocks / p.splits);
 	};
 
-	if (warp >= kLoadWarp) {
+	if (warp >= S::kLoadWarp) {
 		// ---------------------------------------------------------------- operand tiles
 		uint32_t stage = 0, phase = 0;
+		const uint32_t full_lead = PAIR ? peer_address(full, 0) : full;  // a pair's tiles are counted in by the first CTA
 		for (uint32_t u = first; u < units && ok; u += step) {
 			uint32_t mt, nt, split, kb0, kb1;
 			locate(u, mt, nt, split, kb0, kb1);
+			const uint32_t m0 = mt * kTileM + row_offset, n0 = nt * BN + (PAIR ? rank * S::kBRows : 0u);
 			for (uint32_t kb = kb0; kb < kb1; ++kb) {
 				if (GATHER || lane == 0) ok = wait_phase(empty + 8 * stage, phase ^ 1u);
 				if (!ok) break;
 				unsigned char* sa = smem + stage * S::kStage;
 				unsigned char* sb = sa + S::kABytes;
 				if (GATHER) {
-					const int t = tid - kLoadWarp * 32;
+					const int t = tid - S::kLoadWarp * 32;
 					if (AMN) {
-						for (int s = 0; s < 2; ++s) gather_box(sa + s * 8192, p.a, p.a_ld, p.K, p.M, kb * kBK, mt * kBM + s * 64, 64, t);
+						for (int s = 0; s < 2; ++s) gather_box<64>(sa + s * 8192, p.a, p.a_ld, p.K, p.M, kb * kBK, m0 + s * 64, t);
 					} else {
-						gather_box(sa, p.a, p.a_ld, p.M, p.K, mt * kBM, kb * kBK, kBM, t);
+						gather_box<kBM>(sa, p.a, p.a_ld, p.M, p.K, m0, kb * kBK, t);
 					}
 					if (BMN) {
-						for (int s = 0; s < (BN + 63) / 64; ++s) gather_box(sb + s * 8192, p.b, p.b_ld, p.K, p.N, kb * kBK, nt * BN + s * 64, 64, t);
+						for (int s = 0; s < (BN + 63) / 64; ++s) gather_box<64>(sb + s * 8192, p.b, p.b_ld, p.K, p.N, kb * kBK, n0 + s * 64, t);
 					} else {
-						gather_box(sb, p.b, p.b_ld, p.N, p.K, nt * BN, kb * kBK, BN, t);
+						gather_box<BN>(sb, p.b, p.b_ld, p.N, p.K, n0, kb * kBK, t);
 					}
 					tc::fence_async_smem();
 					arrive(full + 8 * stage);
 				} else if (lane == 0) {
-					const uint32_t bar = full + 8 * stage;
+					const uint32_t bar = full_lead + 8 * stage;
 					// slabs that lie outside of the matrix are not loaded: what the tile holds there reaches only sums that are not used
-					const int slabs_a = AMN ? min(2, (int)((p.M - mt * kBM + 63) / 64)) : 1;
-					const int slabs_b = BMN ? min((BN + 63) / 64, (int)((p.N - nt * BN + 63) / 64)) : 1;
-					arrive_expect(bar, (AMN ? slabs_a * 8192 : S::kABytes) + (BMN ? slabs_b * 8192 : S::kBBytes));
+					const int slabs_a = AMN ? (PAIR ? 2 : min(2, (int)((p.M - m0 + 63) / 64))) : 1;
+					const int slabs_b = BMN ? (PAIR ? S::kBRows / 64 : min((BN + 63) / 64, (int)((p.N - n0 + 63) / 64))) : 1;
+					const uint32_t bytes = (AMN ? slabs_a * 8192 : S::kABytes) + (BMN ? slabs_b * 8192 : S::kBBytes);
+					if (!PAIR) arrive_expect(full + 8 * stage, bytes);
+					else if (rank == 0) arrive_expect(full + 8 * stage, 2 * bytes);
 					if (AMN) {
-						for (int s = 0; s < slabs_a; ++s) tma_load(sptr(sa) + s * 8192, &p.ta, mt * kBM + s * 64, kb * kBK, bar);
+						for (int s = 0; s < slabs_a; ++s) tma_load<PAIR>(sptr(sa) + s * 8192, &p.ta, m0 + s * 64, kb * kBK, bar);
 					} else {
-						tma_load(sptr(sa), &p.ta, kb * kBK, mt * kBM, bar);
+						tma_load<PAIR>(sptr(sa), &p.ta, kb * kBK, m0, bar);
 					}
 					if (BMN) {
-						for (int s = 0; s < slabs_b; ++s) tma_load(sptr(sb) + s * 8192, &p.tb, nt * BN + s * 64, kb * kBK, bar);
+						for (int s = 0; s < slabs_b; ++s) tma_load<PAIR>(sptr(sb) + s * 8192, &p.tb, n0 + s * 64, kb * kBK, bar);
 					} else {
-						tma_load(sptr(sb), &p.tb, kb * kBK, nt * BN, bar);
+						tma_load<PAIR>(sptr(sb), &p.tb, kb * kBK, n0, bar);
 					}
 				}
 				if (++stage == S::kStages) stage = 0, phase ^= 1u;
 			}
 			ok = __shfl_sync(~0u, (int)ok, 0) != 0;
 		}
-	} else if (warp == kMmaWarp) {
-		// ---------------------------------------------------------------- MMAs, one thread
-		if (lane == 0) {
+	} else if (warp == S::kMmaWarp) {
+		// ---------------------------------------------------------------- MMAs, one thread (of a pair's first CTA)
+		if (lane == 0 && (!PAIR || rank == 0)) {
 			const uint32_t type = bf ? (1u << 7) | (1u << 10) : 0u;
-			const uint32_t id = tc::idesc_f16(kBM, BN, AMN, BMN) | type, id_ones = tc::idesc_f16(kBM, 16, AMN, 0) | type;
+			const uint32_t id = tc::idesc_f16(kTileM, BN, AMN, BMN) | type, id_ones = tc::idesc_f16(kBM, 16, AMN, 0) | type;
 			uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
 			for (uint32_t u = first; u < units && ok; u += step) {
 				uint32_t mt, nt, split, kb0, kb1;
 				locate(u, mt, nt, split, kb0, kb1);
-				const bool sums = WGRAD && p.want_sums && nt == 0;
+				const bool sums = WGRAD && !PAIR && p.want_sums && nt == 0;
 				for (uint32_t c0 = kb0; c0 < kb1 && ok; c0 += WGRAD ? kChunk : kb1 - kb0) {
 					const uint32_t c1 = WGRAD ? min(c0 + kChunk, kb1) : kb1;
 					ok = wait_phase(tempty + 8 * buf, buf_phase ^ 1u);
@@ -288,35 +456,54 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 							const uint64_t da = AMN ? desc_mn(sa + k * 2048) : desc_k(sa + k * 32);
 							const uint64_t db = BMN ? desc_mn(sb + k * 2048) : desc_k(sb + k * 32);
 							const uint32_t more = kb > c0 || k > 0;
-							tc::mma_f16(tmem + buf * BN, da, db, id, more);
-							if (sums) tc::mma_f16(tmem + 2 * BN + buf * 16, da, tc::smem_desc(sptr(ones), 128, 256), id_ones, more);
+							mma<PAIR>(tmem + buf * BN, da, db, id, more);
+							if (sums) tc::mma_f16(tmem + S::kBufs * BN + buf * 16, da, tc::smem_desc(sptr(ones), 128, 256), id_ones, more);
 						}
-						tc::commit(empty + 8 * stage);
+						commit<PAIR>(empty + 8 * stage);
 						if (++stage == S::kStages) stage = 0, phase ^= 1u;
 					}
 					if (!ok) break;
-					tc::commit(tfull + 8 * buf);
-					if (++buf == 2) buf = 0, buf_phase ^= 1u;
+					commit<PAIR>(tfull + 8 * buf);
+					if (++buf == S::kBufs) buf = 0, buf_phase ^= 1u;
 				}
 			}
 		}
 		__syncwarp();
 	} else {
-		// ---------------------------------------------------------------- epilogue: warp w owns rows 32 (w % 4) .. and columns (w / 4) BN / 2 ..
-		const uint32_t q = warp & 3, half = warp >> 2;
+		// ---------------------------------------------------------------- epilogue: warp w owns rows 32 (w % 4) ..
+		const uint32_t q = warp & 3, half = (warp >> 2) % S::kHalves, group = (warp >> 2) / S::kHalves;
 		const uint32_t lanes = tmem + ((q * 32u) << 16);
-		constexpr int kCols = BN / 2;
-		uint32_t buf = 0, buf_phase = 0;
+		constexpr int kCols = BN / S::kHalves;  // columns half * kCols .. of the tile
+		unsigned char* const bounce = bounces + warp * 2048;
+		uint32_t turn = 0, buf = 0, buf_phase = 0;
+		auto next_buf = [&] {
+			if (++buf == S::kBufs) buf = 0, buf_phase ^= 1u;
+		};
+		auto release = [&] {
+			tc::fence_before_sync();
+			__syncwarp();
+			if (lane == 0) {
+				if (PAIR) arrive_remote(peer_address(tempty + 8 * buf, 0));
+				else arrive(tempty + 8 * buf);
+			}
+		};
 		for (uint32_t u = first; u < units && ok; u += step) {
+			if (S::kGroups > 1) {
+				const bool mine = turn == group;
+				if (++turn == S::kGroups) turn = 0;
+				if (!mine) {
+					next_buf();
+					continue;
+				}
+			}
 			uint32_t mt, nt, split, kb0, kb1;
 			locate(u, mt, nt, split, kb0, kb1);
-			last_m = mt, last_n = nt;
-			const uint32_t m = mt * kBM + q * 32 + lane, n0 = nt * BN + half * kCols;
+			const uint32_t row0 = mt * kTileM + row_offset + q * 32, m = row0 + lane, n0 = nt * BN + half * kCols;
 			if (WGRAD) {
 				float acc[kCols], sum = 0.f;
 #pragma unroll
 				for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-				const bool sums = p.want_sums && nt == 0 && half == 0;
+				const bool sums = !PAIR && p.want_sums && nt == 0 && half == 0;
 				for (uint32_t c0 = kb0; c0 < kb1 && ok; c0 += kChunk) {
 					ok = wait_phase(tfull + 8 * buf, buf_phase);
 					if (!ok) break;
@@ -331,14 +518,12 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 					}
 					if (sums) {
 						uint32_t r[16];
-						tmem_ld16_raw(lanes + 2 * BN + buf * 16, r);
+						tmem_ld16_raw(lanes + S::kBufs * BN + buf * 16, r);
 						tmem_wait16(r);
 						sum += __uint_as_float(r[0]);
 					}
-					tc::fence_before_sync();
-					__syncwarp();
-					if (lane == 0) arrive(tempty + 8 * buf);
-					if (++buf == 2) buf = 0, buf_phase ^= 1u;
+					release();
+					next_buf();
 				}
 				if (!ok) break;
 				if (m < p.M) {
@@ -356,7 +541,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 #pragma unroll
 						for (int i = 0; i < 8; ++i) v[i] = acc[c + i];
 						if (e.vec && n0 + c + 8 <= p.N) {
-							finish_eight(e, bf, m, n0 + c, v);
+							store_eight(e, m, n0 + c, v);
 						} else {
 #pragma unroll
 							for (int i = 0; i < 8; ++i)
@@ -368,7 +553,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 						else p.column_sums[m] = p.e.accumulate ? p.column_sums[m] + sum : sum;
 					}
 				}
-			} else {
+			} else if (SWAP || p.cluster > 1) {
 				ok = wait_phase(tfull + 8 * buf, buf_phase);
 				if (!ok) break;
 				tc::fence_after_sync();
@@ -381,36 +566,93 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 					if (p.cluster > 1) {
 #pragma unroll
 						for (int i = 0; i < 16; ++i) joined[(half * kCols + c + i) * 129 + q * 32 + lane] = __uint_as_float(r[i]);
-					} else if (SWAP) {
+					} else {
 						// m is the feature, the tile's columns are samples
 #pragma unroll
 						for (int i = 0; i < 16; ++i)
 							if (m < p.M && n0 + c + i < p.N) finish_one(p.e, bf, n0 + c + i, m, __uint_as_float(r[i]));
-					} else if (m < p.M) {
-#pragma unroll
-						for (int k = 0; k < 16; k += 8) {
-							float v[8];
-#pragma unroll
-							for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[k + i]);
-							if (p.e.vec && n0 + c + k + 8 <= p.N) {
-								finish_eight(p.e, bf, m, n0 + c + k, v);
-							} else {
-#pragma unroll
-								for (int i = 0; i < 8; ++i)
-									if (n0 + c + k + i < p.N) finish_one(p.e, bf, m, n0 + c + k + i, v[i]);
-							}
-						}
 					}
 				}
-				tc::fence_before_sync();
-				__syncwarp();
-				if (lane == 0) arrive(tempty + 8 * buf);
-				if (++buf == 2) buf = 0, buf_phase ^= 1u;
+				release();
+				next_buf();
+			} else {
+				const Epilogue& e = p.e;
+				Chunk slope, add;  // of the next 32 columns, on their way while the sums are still being computed
+				if (e.slope_z) chunk_load(slope, e.slope_z, e.slope_ld, row0, p.M, n0, p.N, e.vec, lane);
+				if (e.add) chunk_load(add, e.add, e.add_ld, row0, p.M, n0, p.N, e.vec, lane);
+				ok = wait_phase(tfull + 8 * buf, buf_phase);
+				if (!ok) break;
+				tc::fence_after_sync();
+#pragma unroll 1
+				for (int c = 0; c < kCols; c += 32) {
+					uint32_t r0[16], r1[16], other[16];
+					tmem_ld16_raw(lanes + buf * BN + half * kCols + c, r0);
+					tmem_ld16_raw(lanes + buf * BN + half * kCols + c + 16, r1);
+					tmem_wait16(r0);
+					tmem_wait16(r1);
+					float v[32];
+#pragma unroll
+					for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r0[i]), v[16 + i] = __uint_as_float(r1[i]);
+					if (c + 32 >= kCols) release();
+					const uint32_t col = n0 + c;
+					if (e.bias) {
+						const uint16_t* b = (const uint16_t*)e.bias;
+						if (e.vec && col + 32 <= p.N) {
+#pragma unroll
+							for (int i = 0; i < 4; ++i) {
+								const uint4 w = __ldg(reinterpret_cast<const uint4*>(b + col) + i);
+								const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+								for (int j = 0; j < 4; ++j) {
+									const float2 f = unpack2(ws[j], bf);
+									v[8 * i + 2 * j] += f.x;
+									v[8 * i + 2 * j + 1] += f.y;
+								}
+							}
+						} else {
+#pragma unroll
+							for (int i = 0; i < 32; ++i)
+								if (col + i < p.N) v[i] += h2f(b[col + i], bf);
+						}
+					}
+					if (e.preact) {
+#pragma unroll
+						for (int i = 0; i < 16; ++i) other[i] = pack2(v[2 * i], v[2 * i + 1], bf);
+						row_to_global(other, e.preact, e.preact_ld, row0, p.M, col, p.N, bounce, e.vec, lane);
+					}
+					if (e.slope_z) {
+						chunk_to_row(slope, other, bounce, e.vec, lane);
+						if (c + 32 < kCols) chunk_load(slope, e.slope_z, e.slope_ld, row0, p.M, col + 32, p.N, e.vec, lane);
+						if (e.act == NEUS2B_ACT_RELU) apply_slope<NEUS2B_ACT_RELU>(v, other, bf);
+						else if (e.act == NEUS2B_ACT_GELU) apply_slope<NEUS2B_ACT_GELU>(v, other, bf);
+						else apply_slope<NEUS2B_ACT_SILU>(v, other, bf);
+					} else if (e.act == NEUS2B_ACT_RELU) {
+						apply_act<NEUS2B_ACT_RELU>(v);
+					} else if (e.act == NEUS2B_ACT_GELU) {
+						apply_act<NEUS2B_ACT_GELU>(v);
+					} else if (e.act == NEUS2B_ACT_SILU) {
+						apply_act<NEUS2B_ACT_SILU>(v);
+					}
+					if (e.add) {
+						chunk_to_row(add, other, bounce, e.vec, lane);
+						if (c + 32 < kCols) chunk_load(add, e.add, e.add_ld, row0, p.M, col + 32, p.N, e.vec, lane);
+#pragma unroll
+						for (int i = 0; i < 16; ++i) {
+							const float2 f = unpack2(other[i], bf);
+							v[2 * i] += f.x;
+							v[2 * i + 1] += f.y;
+						}
+					}
+#pragma unroll
+					for (int i = 0; i < 16; ++i) other[i] = pack2(v[2 * i], v[2 * i + 1], bf);
+					row_to_global(other, e.out, e.out_ld, row0, p.M, col, p.N, bounce, e.vec, lane);
+				}
+				next_buf();
 			}
 		}
 	}
 	if (!ok) atomicOr(&g_error, 1u);
-	if (!WGRAD && p.cluster > 1) {
+	if (!WGRAD && !PAIR && p.cluster > 1) {
 		// every CTA adds up its share of the tile over the cluster's partial sums, in rank order, and finishes it
 		__syncwarp();
 		cluster_sync();
@@ -430,20 +672,32 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>::kThr
 		cluster_sync();
 	}
 	tc::fence_before_sync();
-	__syncthreads();
-	if (warp == 0) tc::tmem_dealloc(tmem, S::kTmem);
+	__syncwarp();
+	if (PAIR) cluster_sync();  // the other CTA's MMAs and arrivals reach into this one
+	else __syncthreads();
+	tc::fence_after_sync();
+	if (warp == 0) tmem_dealloc<PAIR>(tmem, S::kTmem);
 }
 
-// partial sums of the splits, in order
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, float* __restrict__ out,
-                                                    float* __restrict__ sums, int accumulate) {
-	const uint64_t n = (uint64_t)M * N, total = n + (sums ? M : 0);
-	for (uint64_t i = (out ? 0 : n) + blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
-		const bool is_sum = i >= n;
+// Sums of the splits' parts.  A block takes 32 neighbouring entries; its 8 or 32 rows of threads share the splits and are joined in order.
+template <int ROWS>
+__global__ void __launch_bounds__(32 * ROWS) join_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, float* __restrict__ out,
+                                                         float* __restrict__ sums, int accumulate) {
+	__shared__ float s[ROWS][33];
+	const uint64_t n = (uint64_t)M * N, total = n + (sums ? M : 0), i = (out ? 0 : n) + blockIdx.x * 32ull + threadIdx.x;
+	const bool is_sum = i >= n;
+	float v = 0.f;
+	if (i < total) {
 		const float* q = is_sum ? partial + splits * n + (i - n) : partial + i;
 		const uint64_t pitch = is_sum ? M : n;
-		float v = 0.f;
-		for (uint32_t s = 0; s < splits; ++s) v += q[s * pitch];
+#pragma unroll 4
+		for (uint32_t k = threadIdx.y; k < splits; k += ROWS) v += q[k * pitch];
+	}
+	s[threadIdx.y][threadIdx.x] = v;
+	__syncthreads();
+	if (threadIdx.y == 0 && i < total) {
+#pragma unroll
+		for (int k = 1; k < ROWS; ++k) v += s[k][threadIdx.x];
 		float* o = is_sum ? sums + (i - n) : out + i;
 		*o = accumulate ? *o + v : v;
 	}
@@ -473,13 +727,13 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t ld, uint32_t ro
 // TMA reads rows that start on 16-byte boundaries, less than 2^40 bytes apart
 static bool tma_ok(const void* p, uint64_t ld) { return ((uintptr_t)p & 15u) == 0 && (ld & 7u) == 0 && ld < (1ull << 39); }
 
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER>
+template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
 static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
-	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER>;
-	auto kernel = product_kernel<BN, AMN, BMN, SWAP, WGRAD, GATHER>;
+	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
+	auto kernel = product_kernel<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
 	if (!GATHER) {
 		if (int rc = AMN ? make_map(&a.ta, a.a, a.a_ld, a.K, a.M, 64, a.bf16) : make_map(&a.ta, a.a, a.a_ld, a.M, a.K, kBM, a.bf16)) return rc;
-		if (int rc = BMN ? make_map(&a.tb, a.b, a.b_ld, a.K, a.N, 64, a.bf16) : make_map(&a.tb, a.b, a.b_ld, a.N, a.K, BN, a.bf16)) return rc;
+		if (int rc = BMN ? make_map(&a.tb, a.b, a.b_ld, a.K, a.N, 64, a.bf16) : make_map(&a.tb, a.b, a.b_ld, a.N, a.K, S::kBRows, a.bf16)) return rc;
 	}
 	N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
 	cudaLaunchConfig_t cfg{};
@@ -489,69 +743,81 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 	cfg.stream = stream;
 	cudaLaunchAttribute attr[1];
 	attr[0].id = cudaLaunchAttributeClusterDimension;
-	attr[0].val.clusterDim.x = a.cluster;
+	attr[0].val.clusterDim.x = PAIR ? 2 : a.cluster;
 	attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
 	cfg.attrs = attr;
-	cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+	cfg.numAttrs = PAIR || a.cluster > 1 ? 1 : 0;
 	const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const Args)a);
 	if (e != cudaSuccess) return (int)e;
 	N2B_CHECK_LAUNCH();
 	return NEUS2B_OK;
 }
 
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD>
-static int launch_any(Args& a, uint32_t ctas, cudaStream_t stream) {
-	if (tma_ok(a.a, a.a_ld) && tma_ok(a.b, a.b_ld)) return launch<BN, AMN, BMN, SWAP, WGRAD, false>(a, ctas, stream);
-	return launch<BN, AMN, BMN, SWAP, WGRAD, true>(a, ctas, stream);
-}
-
-// Tile width, and over how many CTAs of a cluster a tile's sum is split, for `tiles_of(BN)` tiles and `kblocks` steps of 64.
-struct Plan {
-	uint32_t bn, cluster;
-};
+// over how many CTAs of a cluster a tile's sum is split: as many as the SMs can take, with at least four steps of 64 for each
 static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks) {
 	uint32_t c = 1;
-	while (c < 8 && tiles * c * 2 <= (uint64_t)kSMs && kblocks >= c * 2 * 4) c *= 2;  // at least four steps stay for every CTA
+	while (c < 8 && tiles * c * 2 <= (uint64_t)kSMs && kblocks >= c * 2 * 4) c *= 2;
 	return c;
 }
+static uint32_t tiles_of(uint32_t n, uint32_t size) { return (n + size - 1) / size; }
 
-template <bool BMN_FORWARD>
+template <bool BMN>
 static int product_of(const Product& p, cudaStream_t stream) {
 	Args a{};
 	a.bf16 = p.bf16;
 	a.K = p.K;
 	a.e = p.e;
 	a.splits = a.cluster = 1;
-	const uint32_t kblocks = (p.K + kBK - 1) / kBK;
-	auto go = [&](auto launcher, uint32_t bn) {
-		a.tiles_m = (a.M + kBM - 1) / kBM;
-		a.tiles_n = (a.N + bn - 1) / bn;
+	const uint32_t kblocks = tiles_of(p.K, kBK);
+	const bool tma = tma_ok(p.a, p.a_ld) && tma_ok(p.b, p.b_ld);
+	// grid of one-CTA tiles; may_split: the kernel can join a cluster's parts
+	auto grid = [&](uint32_t bn, bool may_split) -> uint32_t {
+		a.tiles_m = tiles_of(a.M, kBM);
+		a.tiles_n = tiles_of(a.N, bn);
 		const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
-		if (tiles >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
-		a.cluster = bn <= 128 ? cluster_for(tiles, kblocks) : 1u;
-		a.splits = a.cluster;
-		return launcher(a, (uint32_t)(a.cluster > 1 ? tiles * a.cluster : (tiles < (uint64_t)kSMs ? tiles : (uint64_t)kSMs)), stream);
+		if (tiles >= (1ull << 31)) return 0;
+		a.cluster = a.splits = may_split ? cluster_for(tiles, kblocks) : 1u;
+		return (uint32_t)(a.cluster > 1 ? tiles * a.cluster : tiles < (uint64_t)kSMs ? tiles : (uint64_t)kSMs);
 	};
+#define N2B_GO(BN, AMN, BMN_, SWAP)                                                                  \
+	do {                                                                                             \
+		const uint32_t ctas = grid(BN, BN <= 128);                                                   \
+		if (!ctas) return NEUS2B_E_TOO_LARGE;                                                        \
+		return tma ? launch<BN, AMN, BMN_, SWAP, false, false, false>(a, ctas, stream)               \
+		           : launch<BN, AMN, BMN_, SWAP, false, true, false>(a, ctas, stream);               \
+	} while (0)
 	if (p.M <= 64) {
 		// few samples: the weights are the 128-row operand, the samples its columns
 		a.a = (const uint16_t*)p.b, a.a_ld = p.b_ld, a.M = p.N;
 		a.b = (const uint16_t*)p.a, a.b_ld = p.a_ld, a.N = p.M;
-		if (p.M <= 32) return go(launch_any<32, BMN_FORWARD, false, true, false>, 32);
-		return go(launch_any<64, BMN_FORWARD, false, true, false>, 64);
+		if (p.M <= 32) N2B_GO(32, BMN, false, true);
+		N2B_GO(64, BMN, false, true);
 	}
 	a.a = (const uint16_t*)p.a, a.a_ld = p.a_ld, a.M = p.M;
 	a.b = (const uint16_t*)p.b, a.b_ld = p.b_ld, a.N = p.N;
-	const uint64_t rows = (p.M + kBM - 1) / kBM;
-	if (p.N > 128 && rows * ((p.N + 255) / 256) >= (uint64_t)kSMs) return go(launch_any<256, false, BMN_FORWARD, false, false>, 256);
-	if (p.N > 64 && rows * ((p.N + 127) / 128) >= (uint64_t)kSMs) return go(launch_any<128, false, BMN_FORWARD, false, false>, 128);
-	return go(launch_any<64, false, BMN_FORWARD, false, false>, 64);
+	// The tile with the least time, counted as rounds over the SMs times what a tile costs: its columns, and 64 more for its rows and its
+	// epilogue.  A pair's 256 x 256 tile reads each operand half as often as two CTAs' tiles: it counts 0.85 of two.
+	const uint64_t rows = tiles_of(p.M, kBM);
+	auto cost = [&](uint32_t bn) { return (rows * tiles_of(p.N, bn) + kSMs - 1) / kSMs * (bn + 64) * 20; };
+	const uint64_t pairs = (uint64_t)tiles_of(p.M, 2 * kBM) * tiles_of(p.N, 256), pair_cost = (pairs + kSMs / 2 - 1) / (kSMs / 2) * (256 + 64) * 17;
+	const uint64_t c64 = cost(64), c128 = cost(128), c256 = cost(256);
+	if (tma && pair_cost < c64 && pair_cost < c128 && pair_cost < c256) {
+		a.tiles_m = tiles_of(a.M, 2 * kBM);
+		a.tiles_n = tiles_of(a.N, 256);
+		if (pairs >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
+		return launch<256, false, BMN, false, false, false, true>(a, 2 * (uint32_t)(pairs < kSMs / 2 ? pairs : kSMs / 2), stream);
+	}
+	if (c256 < c128 && c256 < c64) N2B_GO(256, false, BMN, false);
+	if (c128 < c64) N2B_GO(128, false, BMN, false);
+	N2B_GO(64, false, BMN, false);
+#undef N2B_GO
 }
 
+// Weight gradient: tiles of out_width x in_width, k the samples.  Few tiles share the samples out over the SMs and are joined afterwards.
 constexpr uint32_t kWgradBN = 128;
 static uint32_t wgrad_splits(uint32_t M, uint32_t N, uint32_t K) {
-	const uint64_t tiles = (uint64_t)((M + kBM - 1) / kBM) * ((N + kWgradBN - 1) / kWgradBN);
-	const uint32_t kblocks = (K + kBK - 1) / kBK;
-	const uint64_t fill = (uint64_t)kSMs / tiles, most = kblocks / kChunk;
+	const uint64_t tiles = (uint64_t)tiles_of(M, kBM) * tiles_of(N, kWgradBN);
+	const uint64_t fill = (uint64_t)kSMs / tiles, most = tiles_of(K, kBK) / kChunk;
 	const uint64_t s = fill < most ? fill : most;
 	return s > 1 ? (uint32_t)s : 1u;
 }
@@ -596,10 +862,15 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 	if (a.splits > 1 && p.workspace_bytes < partial_bytes(p.M, p.N, p.K)) return NEUS2B_E_INVALID;
 	const uint64_t units = (uint64_t)a.tiles_m * a.tiles_n * a.splits;
 	if (units >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
-	if (int rc = launch_any<kWgradBN, true, true, false, true>(a, (uint32_t)(units < (uint64_t)kSMs ? units : kSMs), stream)) return rc;
+	const uint32_t ctas = (uint32_t)(units < (uint64_t)kSMs ? units : kSMs);
+	if (int rc = tma_ok(a.a, a.a_ld) && tma_ok(a.b, a.b_ld) ? launch<kWgradBN, true, true, false, true, false, false>(a, ctas, stream)
+	                                                        : launch<kWgradBN, true, true, false, true, true, false>(a, ctas, stream))
+		return rc;
 	if (a.splits > 1) {
-		const uint64_t total = (uint64_t)p.M * p.N + p.M;
-		join_kernel<<<(uint32_t)(total < 256ull * 8 * kSMs ? (total + 255) / 256 : 8 * kSMs), 256, 0, stream>>>(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate);
+		const uint64_t entries = (p.e.out ? (uint64_t)p.M * p.N : 0) + (p.column_sums ? p.M : 0);
+		const uint32_t blocks = (uint32_t)((entries + 31) / 32);
+		if (a.splits >= 32) join_kernel<32><<<blocks, dim3(32, 32), 0, stream>>>(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate);
+		else join_kernel<8><<<blocks, dim3(32, 8), 0, stream>>>(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate);
 		N2B_CHECK_LAUNCH();
 	}
 	return NEUS2B_OK;
