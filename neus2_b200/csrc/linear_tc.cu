@@ -451,13 +451,22 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 						if (!ok) break;
 						tc::fence_after_sync();
 						const uint32_t sa = sptr(smem + stage * S::kStage), sb = sa + S::kABytes;
-						const int steps = min(4, (int)((p.K - kb * kBK + 15) / 16));
-						for (int k = 0; k < steps; ++k) {
-							const uint64_t da = AMN ? desc_mn(sa + k * 2048) : desc_k(sa + k * 32);
-							const uint64_t db = BMN ? desc_mn(sb + k * 2048) : desc_k(sb + k * 32);
-							const uint32_t more = kb > c0 || k > 0;
-							mma<PAIR>(tmem + buf * BN, da, db, id, more);
-							if (sums) tc::mma_f16(tmem + S::kBufs * BN + buf * 16, da, tc::smem_desc(sptr(ones), 128, 256), id_ones, more);
+						const uint64_t da = AMN ? desc_mn(sa) : desc_k(sa), db = BMN ? desc_mn(sb) : desc_k(sb);
+						constexpr uint64_t kStepA = (AMN ? 2048 : 32) / 16, kStepB = (BMN ? 2048 : 32) / 16;  // 16 k further
+						const uint32_t d = tmem + buf * BN;
+						if (p.K - kb * kBK >= kBK) {
+							// one thread issues all MMAs of the SM: nothing but the two descriptors' sums between them
+							mma<PAIR>(d, da, db, id, kb > c0);
+#pragma unroll
+							for (int k = 1; k < 4; ++k) mma<PAIR>(d, da + k * kStepA, db + k * kStepB, id, 1u);
+						} else {
+							const int steps = (int)((p.K - kb * kBK + 15) / 16);
+							for (int k = 0; k < steps; ++k) mma<PAIR>(d, da + k * kStepA, db + k * kStepB, id, kb > c0 || k > 0);
+						}
+						if (sums) {
+							const int steps = min(4, (int)((p.K - kb * kBK + 15) / 16));
+							for (int k = 0; k < steps; ++k)
+								tc::mma_f16(tmem + S::kBufs * BN + buf * 16, da + k * kStepA, tc::smem_desc(sptr(ones), 128, 256), id_ones, kb > c0 || k > 0);
 						}
 						commit<PAIR>(empty + 8 * stage);
 						if (++stage == S::kStages) stage = 0, phase ^= 1u;
