@@ -42,17 +42,16 @@ __device__ __forceinline__ float act_value(int act, float z) {
 	if (act == NEUS2B_ACT_SILU) return z * logistic2(kLog2e * z);
 	return z;
 }
-// d act / dz.  gelu: s + z s (1 - s) 2u'; behind |z| = 10 the second term is below 1e-35, and z is held there so that u' stays finite;
-// silu: s + z s (1 - s), z held at 100.  A NaN stays one through s.
+// d act / dz.  gelu: s + z s (1 - s) 2u' with 2u' = 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2); where z^2 is held at 1e30, s (1 - s) is 0.
 __device__ __forceinline__ float act_slope(int act, float z) {
 	if (act == NEUS2B_ACT_RELU) return z > 0.f ? 1.f : 0.f;
 	if (act == NEUS2B_ACT_GELU) {
-		const float s = logistic2(gelu_argument(z)), zc = fminf(fmaxf(z, -10.f), 10.f);
-		return fmaf(zc * fmaf(-s, s, s), fmaf(6.f * kGeluC * kGeluA * zc, zc, 2.f * kGeluC), s);
+		const float s = logistic2(gelu_argument(z)), z2 = fminf(z * z, 1e30f);
+		return fmaf(z * fmaf(-s, s, s), fmaf(6.f * kGeluC * kGeluA, z2, 2.f * kGeluC), s);
 	}
 	if (act == NEUS2B_ACT_SILU) {
-		const float s = logistic2(kLog2e * z), zc = fminf(fmaxf(z, -100.f), 100.f);
-		return fmaf(zc, fmaf(-s, s, s), s);
+		const float s = logistic2(kLog2e * z);
+		return fmaf(z, fmaf(-s, s, s), s);
 	}
 	return 1.f;
 }

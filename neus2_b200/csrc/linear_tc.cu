@@ -18,6 +18,7 @@ static __device__ uint32_t g_error;  // bit 0: a bounded wait ran out
 constexpr int kBM = 128, kBK = 64;
 constexpr int kGatherWarps = 7;
 constexpr int kMaxStages = 8, kSmemMost = 227 * 1024;
+constexpr int kChunkBytes = 32 * 64;  // 32 x 32 values on their way between the epilogue and global memory
 constexpr int kChunk = 8;  // weight gradient: k blocks (512 samples) summed in tensor memory before the sum moves to registers
 
 struct alignas(64) Args {
@@ -210,20 +211,20 @@ __device__ __forceinline__ void gather_box(unsigned char* dst, const uint16_t* b
 }
 
 // What a block of one variant is made of.  PAIR: two CTAs of a cluster compute a 256 x BN tile together, each with 128 of its rows in its
-// tensor memory and half of B's tile in its shared memory.  Narrow tiles (BN 64) finish faster than one group of warps can write
-// them: four groups take turns, each with an accumulator of its own; wide ones are shared by two halves of the warps.
+// tensor memory and half of B's tile in its shared memory.  The epilogue is a long chain of dependent steps, so that it takes 16 warps to
+// keep up with the MMAs: on wide tiles they share the columns, narrow ones (BN 64) go to four groups in turn, each with an accumulator.
 template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
 struct Shape {
 	static constexpr int kBRows = PAIR ? BN / 2 : BN;  // of B's tile in this CTA
 	static constexpr int kABytes = kBM * 128;
 	static constexpr int kBBytes = (BMN && kBRows < 64 ? 64 : kBRows) * 128;
 	static constexpr int kStage = kABytes + kBBytes;
-	static constexpr bool kTurns = BN == 64 && !SWAP && !WGRAD;
-	static constexpr int kHalves = kTurns ? 1 : 2, kGroups = kTurns ? (GATHER ? 2 : 4) : 1, kBufs = kTurns ? 4 : 2;
+	static constexpr bool kTurns = BN == 64 && !SWAP && !WGRAD, kMany = !GATHER && !SWAP && !WGRAD && (PAIR || BN <= 128);
+	static constexpr int kHalves = kTurns ? 1 : kMany ? 4 : 2, kGroups = kTurns ? (kMany ? 4 : 2) : 1, kBufs = kTurns ? 4 : 2;
 	static constexpr int kEpiWarps = 4 * kHalves * kGroups, kMmaWarp = kEpiWarps, kLoadWarp = kEpiWarps + 1;
 	static constexpr int kThreads = (GATHER ? kLoadWarp + kGatherWarps : kLoadWarp + 1) * 32;
-	static constexpr int kBounce = SWAP || WGRAD ? 0 : kEpiWarps * 2048;  // 32 rows of 32 values for every epilogue warp
-	static constexpr int kFixed = kBounce + 2048 + 1024;                  // ones tile and barriers; alignment of the base
+	static constexpr int kBounce = SWAP || WGRAD ? 0 : kEpiWarps * 3 * kChunkBytes;  // a result, a slope and an addend chunk for every epilogue warp
+	static constexpr int kFixed = kBounce + 2048 + 1024;                         // ones tile and barriers; alignment of the base
 	static constexpr int kRoom = (kSmemMost - kFixed) / kStage;
 	static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;
 	static constexpr int kSmem = kStages * kStage + kFixed;
@@ -231,74 +232,61 @@ struct Shape {
 	static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
-// ---- 32 x 32 values of a matrix between global memory and registers, through a warp's 2 KB of shared memory.  Global memory is read
-// and written in whole row segments (64 bytes), a thread computes on one row.  Where rows do not start on 16-byte boundaries a thread
-// moves one column's values one by one: still one segment of a row per instruction.  The 16-byte units of a row are permuted so that
-// neither side's accesses collide.
-struct Chunk {
-	uint32_t w[16];
-};
+// ---- 32 x 32 values of a matrix between global memory and registers, through 2 KB of shared memory of a warp.  Global memory is read
+// (asynchronously) and written in whole row segments (64 bytes), a thread computes on one row.  Where rows do not start on 16-byte
+// boundaries a thread moves one column's values one by one: still one segment of a row per instruction.  The 16-byte units of a row
+// are permuted so that neither side's accesses collide.
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return (uint32_t)(row * 64 + ((unit ^ ((row >> 1) & 3)) << 4)); }
-__device__ __forceinline__ void chunk_load(Chunk& k, const void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols, int vec, int lane) {
+__device__ __forceinline__ void chunk_fetch(uint32_t chunk, const void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols, int vec, int lane) {
 	const uint16_t* p = (const uint16_t*)base;
 	if (vec) {
+		const uint32_t r0 = row0 + (lane >> 2), c = col0 + (lane & 3) * 8;
+		const uint16_t* q = p + (uint64_t)r0 * ld + c;
 #pragma unroll
-		for (int i = 0; i < 4; ++i) {
-			const uint32_t r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
-			uint4 v = make_uint4(0, 0, 0, 0);
-			if (r < rows && c < cols) v = *reinterpret_cast<const uint4*>(p + (uint64_t)r * ld + c);
-			k.w[4 * i] = v.x, k.w[4 * i + 1] = v.y, k.w[4 * i + 2] = v.z, k.w[4 * i + 3] = v.w;
-		}
+		for (int i = 0; i < 4; ++i, q += 8 * ld)
+			if (r0 + 8 * i < rows && c < cols)
+				asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(chunk + unit_at(i * 8 + (lane >> 2), lane & 3)), "l"(q) : "memory");
 	} else {
-#pragma unroll
-		for (int i = 0; i < 16; ++i) {
-			const uint32_t r = row0 + 2 * i, c = col0 + lane;
-			const uint32_t lo = r < rows && c < cols ? p[(uint64_t)r * ld + c] : 0u, hi = r + 1 < rows && c < cols ? p[(uint64_t)(r + 1) * ld + c] : 0u;
-			k.w[i] = lo | hi << 16;
+		const uint16_t* q = p + (uint64_t)row0 * ld + col0 + lane;
+#pragma unroll 8
+		for (int i = 0; i < 32; ++i, q += ld) {
+			const uint16_t v = row0 + i < rows && col0 + lane < cols ? *q : (uint16_t)0;
+			asm volatile("st.shared.u16 [%0], %1;" ::"r"(chunk + unit_at(i, lane >> 3) + (lane & 7) * 2), "h"(v) : "memory");
 		}
 	}
 }
-// The thread's own row of a chunk that was loaded above.
-__device__ __forceinline__ void chunk_to_row(const Chunk& k, uint32_t (&row)[16], unsigned char* bounce, int vec, int lane) {
-	if (vec) {
-#pragma unroll
-		for (int i = 0; i < 4; ++i)
-			*reinterpret_cast<uint4*>(bounce + unit_at(i * 8 + (lane >> 2), lane & 3)) = make_uint4(k.w[4 * i], k.w[4 * i + 1], k.w[4 * i + 2], k.w[4 * i + 3]);
-	} else {
-#pragma unroll
-		for (int i = 0; i < 32; ++i)
-			*reinterpret_cast<uint16_t*>(bounce + unit_at(i, lane >> 3) + (lane & 7) * 2) = (uint16_t)(k.w[i >> 1] >> (16 * (i & 1)));
-	}
-	__syncwarp();
+// The thread's own row of a chunk that has arrived.
+__device__ __forceinline__ void chunk_row(uint32_t (&row)[16], const unsigned char* chunk, int lane) {
 #pragma unroll
 	for (int u = 0; u < 4; ++u) {
-		const uint4 v = *reinterpret_cast<const uint4*>(bounce + unit_at(lane, u));
+		const uint4 v = *reinterpret_cast<const uint4*>(chunk + unit_at(lane, u));
 		row[4 * u] = v.x, row[4 * u + 1] = v.y, row[4 * u + 2] = v.z, row[4 * u + 3] = v.w;
 	}
-	__syncwarp();
 }
-__device__ __forceinline__ void row_to_global(const uint32_t (&row)[16], void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols,
-                                              unsigned char* bounce, int vec, int lane) {
+__device__ __forceinline__ void chunk_store(const uint32_t (&row)[16], void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols,
+                                            unsigned char* chunk, int vec, int lane) {
 	uint16_t* p = (uint16_t*)base;
+	__syncwarp();  // what was here before has been read
 #pragma unroll
 	for (int u = 0; u < 4; ++u)
-		*reinterpret_cast<uint4*>(bounce + unit_at(lane, u)) = make_uint4(row[4 * u], row[4 * u + 1], row[4 * u + 2], row[4 * u + 3]);
+		*reinterpret_cast<uint4*>(chunk + unit_at(lane, u)) = make_uint4(row[4 * u], row[4 * u + 1], row[4 * u + 2], row[4 * u + 3]);
 	__syncwarp();
 	if (vec) {
+		const uint32_t r0 = row0 + (lane >> 2), c = col0 + (lane & 3) * 8;
+		uint16_t* q = p + (uint64_t)r0 * ld + c;
 #pragma unroll
-		for (int i = 0; i < 4; ++i) {
-			const uint32_t r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * 8;
-			const uint4 v = *reinterpret_cast<const uint4*>(bounce + unit_at(i * 8 + (lane >> 2), lane & 3));
-			if (r < rows && c < cols) *reinterpret_cast<uint4*>(p + (uint64_t)r * ld + c) = v;
+		for (int i = 0; i < 4; ++i, q += 8 * ld) {
+			const uint4 v = *reinterpret_cast<const uint4*>(chunk + unit_at(i * 8 + (lane >> 2), lane & 3));
+			if (r0 + 8 * i < rows && c < cols) *reinterpret_cast<uint4*>(q) = v;
 		}
 	} else {
-#pragma unroll
-		for (int i = 0; i < 32; ++i) {
-			const uint16_t v = *reinterpret_cast<const uint16_t*>(bounce + unit_at(i, lane >> 3) + (lane & 7) * 2);
-			if (row0 + i < rows && col0 + lane < cols) p[(uint64_t)(row0 + i) * ld + col0 + lane] = v;
+		uint16_t* q = p + (uint64_t)row0 * ld + col0 + lane;
+#pragma unroll 8
+		for (int i = 0; i < 32; ++i, q += ld) {
+			const uint16_t v = *reinterpret_cast<const uint16_t*>(chunk + unit_at(i, lane >> 3) + (lane & 7) * 2);
+			if (row0 + i < rows && col0 + lane < cols) *q = v;
 		}
 	}
-	__syncwarp();
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w, bool bf) {
 	return bf ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -483,7 +471,9 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 		const uint32_t q = warp & 3, half = (warp >> 2) % S::kHalves, group = (warp >> 2) / S::kHalves;
 		const uint32_t lanes = tmem + ((q * 32u) << 16);
 		constexpr int kCols = BN / S::kHalves;  // columns half * kCols .. of the tile
-		unsigned char* const bounce = bounces + warp * 2048;
+		unsigned char* const result = bounces + warp * 3 * kChunkBytes;
+		unsigned char* const slope = result + kChunkBytes;
+		unsigned char* const addend = slope + kChunkBytes;
 		uint32_t turn = 0, buf = 0, buf_phase = 0;
 		auto next_buf = [&] {
 			if (++buf == S::kBufs) buf = 0, buf_phase ^= 1u;
@@ -518,12 +508,14 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 					if (!ok) break;
 					tc::fence_after_sync();
 #pragma unroll
-					for (int c = 0; c < kCols; c += 16) {
-						uint32_t r[16];
-						tmem_ld16_raw(lanes + buf * BN + half * kCols + c, r);
-						tmem_wait16(r);
+					for (int c = 0; c < kCols; c += 32) {
+						uint32_t r0[16], r1[16];
+						tmem_ld16_raw(lanes + buf * BN + half * kCols + c, r0);
+						tmem_ld16_raw(lanes + buf * BN + half * kCols + c + 16, r1);
+						tmem_wait16(r0);
+						tmem_wait16(r1);
 #pragma unroll
-						for (int i = 0; i < 16; ++i) acc[c + i] += __uint_as_float(r[i]);
+						for (int i = 0; i < 16; ++i) acc[c + i] += __uint_as_float(r0[i]), acc[c + 16 + i] += __uint_as_float(r1[i]);
 					}
 					if (sums) {
 						uint32_t r[16];
@@ -586,14 +578,20 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 				next_buf();
 			} else {
 				const Epilogue& e = p.e;
-				Chunk slope, add;  // of the next 32 columns, on their way while the sums are still being computed
-				if (e.slope_z) chunk_load(slope, e.slope_z, e.slope_ld, row0, p.M, n0, p.N, e.vec, lane);
-				if (e.add) chunk_load(add, e.add, e.add_ld, row0, p.M, n0, p.N, e.vec, lane);
+				// the inputs' next 32 columns are on their way while the sums are still being computed
+				auto fetch = [&](uint32_t col) {
+					if (e.slope_z) chunk_fetch(sptr(slope), e.slope_z, e.slope_ld, row0, p.M, col, p.N, e.vec, lane);
+					if (e.add) chunk_fetch(sptr(addend), e.add, e.add_ld, row0, p.M, col, p.N, e.vec, lane);
+					asm volatile("cp.async.commit_group;" ::: "memory");
+				};
+				const bool inputs = e.slope_z || e.add;
+				if (inputs) fetch(n0);
 				ok = wait_phase(tfull + 8 * buf, buf_phase);
 				if (!ok) break;
 				tc::fence_after_sync();
 #pragma unroll 1
 				for (int c = 0; c < kCols; c += 32) {
+					const uint32_t col = n0 + c;
 					uint32_t r0[16], r1[16], other[16];
 					tmem_ld16_raw(lanes + buf * BN + half * kCols + c, r0);
 					tmem_ld16_raw(lanes + buf * BN + half * kCols + c + 16, r1);
@@ -603,7 +601,6 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 #pragma unroll
 					for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r0[i]), v[16 + i] = __uint_as_float(r1[i]);
 					if (c + 32 >= kCols) release();
-					const uint32_t col = n0 + c;
 					if (e.bias) {
 						const uint16_t* b = (const uint16_t*)e.bias;
 						if (e.vec && col + 32 <= p.N) {
@@ -627,11 +624,14 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 					if (e.preact) {
 #pragma unroll
 						for (int i = 0; i < 16; ++i) other[i] = pack2(v[2 * i], v[2 * i + 1], bf);
-						row_to_global(other, e.preact, e.preact_ld, row0, p.M, col, p.N, bounce, e.vec, lane);
+						chunk_store(other, e.preact, e.preact_ld, row0, p.M, col, p.N, result, e.vec, lane);
+					}
+					if (inputs) {
+						asm volatile("cp.async.wait_all;" ::: "memory");
+						__syncwarp();
 					}
 					if (e.slope_z) {
-						chunk_to_row(slope, other, bounce, e.vec, lane);
-						if (c + 32 < kCols) chunk_load(slope, e.slope_z, e.slope_ld, row0, p.M, col + 32, p.N, e.vec, lane);
+						chunk_row(other, slope, lane);
 						if (e.act == NEUS2B_ACT_RELU) apply_slope<NEUS2B_ACT_RELU>(v, other, bf);
 						else if (e.act == NEUS2B_ACT_GELU) apply_slope<NEUS2B_ACT_GELU>(v, other, bf);
 						else apply_slope<NEUS2B_ACT_SILU>(v, other, bf);
@@ -643,8 +643,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 						apply_act<NEUS2B_ACT_SILU>(v);
 					}
 					if (e.add) {
-						chunk_to_row(add, other, bounce, e.vec, lane);
-						if (c + 32 < kCols) chunk_load(add, e.add, e.add_ld, row0, p.M, col + 32, p.N, e.vec, lane);
+						chunk_row(other, addend, lane);
 #pragma unroll
 						for (int i = 0; i < 16; ++i) {
 							const float2 f = unpack2(other[i], bf);
@@ -652,9 +651,13 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 							v[2 * i + 1] += f.y;
 						}
 					}
+					if (inputs) {
+						__syncwarp();
+						if (c + 32 < kCols) fetch(col + 32);
+					}
 #pragma unroll
 					for (int i = 0; i < 16; ++i) other[i] = pack2(v[2 * i], v[2 * i + 1], bf);
-					row_to_global(other, e.out, e.out_ld, row0, p.M, col, p.N, bounce, e.vec, lane);
+					chunk_store(other, e.out, e.out_ld, row0, p.M, col, p.N, result, e.vec, lane);
 				}
 				next_buf();
 			}
@@ -823,12 +826,72 @@ static int product_of(const Product& p, cudaStream_t stream) {
 }
 
 // Weight gradient: tiles of out_width x in_width, k the samples.  Few tiles share the samples out over the SMs and are joined afterwards.
-constexpr uint32_t kWgradBN = 128;
-static uint32_t wgrad_splits(uint32_t M, uint32_t N, uint32_t K) {
-	const uint64_t tiles = (uint64_t)tiles_of(M, kBM) * tiles_of(N, kWgradBN);
-	const uint64_t fill = (uint64_t)kSMs / tiles, most = tiles_of(K, kBK) / kChunk;
-	const uint64_t s = fill < most ? fill : most;
-	return s > 1 ? (uint32_t)s : 1u;
+// One CTA's 128 x 128 tile takes about 430 cycles for 64 samples (its operands' way through shared memory), a pair's 256 x 256 tile 512
+// (its MMAs); the plan with the fewest cycles is taken.
+struct WgradPlan {
+	bool pair;
+	uint32_t tiles_m, tiles_n, splits;
+};
+static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair) {
+	const uint32_t kblocks = tiles_of(K, kBK);
+	uint64_t best = 0;
+	WgradPlan plan{};
+	for (int pair = 0; pair <= (may_pair ? 1 : 0); ++pair) {
+		const uint32_t size = pair ? 256 : 128, slots = pair ? kSMs / 2 : kSMs;
+		const uint64_t tiles = (uint64_t)tiles_of(M, size) * tiles_of(N, size), fill = slots / tiles, most = kblocks / kChunk;
+		const uint64_t splits = fill < most ? (fill ? fill : 1) : (most ? most : 1);
+		const uint64_t cycles = (tiles * splits + slots - 1) / slots * ((kblocks + splits - 1) / splits) * (pair ? 512 : 430);
+		if (!pair || cycles < best) {
+			best = cycles;
+			plan = WgradPlan{pair != 0, tiles_of(M, size), tiles_of(N, size), (uint32_t)splits};
+		}
+	}
+	return plan;
+}
+// blocks of rows that the column sums of a pair's plan are taken in, at most
+static uint32_t sum_blocks(uint32_t cols) {
+	const uint32_t by = 4 * kSMs / tiles_of(cols, 256);
+	return by ? by : 1;
+}
+static uint64_t plan_bytes(const WgradPlan& w, uint32_t M, uint32_t N) {
+	const uint64_t partial = w.splits > 1 ? (uint64_t)w.splits * ((uint64_t)M * N + M) * 4 : 0, sums = w.pair ? (uint64_t)sum_blocks(M) * M * 4 : 0;
+	return partial > sums ? partial : sums;
+}
+
+// Column sums of a [rows][cols] matrix with rows on 16-byte boundaries: block (x, y) takes 256 columns and every gridDim.y-th group of 8
+// rows, a thread 8 columns; its 8 warps are joined in order.  partial [gridDim.y][cols].
+__global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ a, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t bf16,
+                                                          float* __restrict__ partial) {
+	__shared__ float s[8][32][9];
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	const uint32_t c = blockIdx.x * 256 + lane * 8;
+	const bool bf = bf16 != 0;
+	float v[8] = {};
+	if (c + 8 <= cols) {
+#pragma unroll 4
+		for (uint32_t r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
+			const uint4 q = __ldg(reinterpret_cast<const uint4*>(a + (uint64_t)r * ld + c));
+			const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+			for (int i = 0; i < 4; ++i) {
+				const float2 f = unpack2(w[i], bf);
+				v[2 * i] += f.x, v[2 * i + 1] += f.y;
+			}
+		}
+	} else if (c < cols) {
+		for (uint32_t r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8)
+			for (uint32_t i = 0; c + i < cols; ++i) v[i] += h2f(a[(uint64_t)r * ld + c + i], bf);
+	}
+#pragma unroll
+	for (int i = 0; i < 8; ++i) s[warp][lane][i] = v[i];
+	__syncthreads();
+	const uint32_t col = threadIdx.x;
+	if (blockIdx.x * 256 + col < cols) {
+		float t = 0.f;
+#pragma unroll
+		for (int k = 0; k < 8; ++k) t += s[k][col >> 3][col & 7];
+		partial[(uint64_t)blockIdx.y * cols + blockIdx.x * 256 + col] = t;
+	}
 }
 
 }  // namespace lin
@@ -846,43 +909,58 @@ int write_linear_error(uint32_t flags) {
 
 int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product_of<true>(p, stream) : product_of<false>(p, stream); }
 
-static uint64_t partial_bytes(uint32_t M, uint32_t N, uint32_t K) {
-	const uint64_t s = wgrad_splits(M, N, K);
-	return s > 1 ? s * ((uint64_t)M * N + M) * 4 : 0;
-}
 uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {
-	const uint64_t a = partial_bytes(out_width, in_width, n), b = partial_bytes(out_width, sums_only_width(out_width), n);
-	return a > b ? a : b;
+	// whether the operands can be read by TMA is not known here: the larger of the two plans, and of the sums alone
+	uint64_t most = plan_bytes(wgrad_plan(out_width, in_width, n, true), out_width, in_width);
+	for (uint32_t width : {in_width, sums_only_width(out_width)}) {
+		const uint64_t b = plan_bytes(wgrad_plan(out_width, width, n, false), out_width, width);
+		if (b > most) most = b;
+	}
+	return most;
+}
+
+static int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
+	const uint64_t entries = (out ? (uint64_t)M * N : 0) + (sums ? M : 0);
+	const uint32_t blocks = (uint32_t)((entries + 31) / 32);
+	if (splits >= 32) join_kernel<32><<<blocks, dim3(32, 32), 0, stream>>>(partial, splits, M, N, out, sums, accumulate);
+	else join_kernel<8><<<blocks, dim3(32, 8), 0, stream>>>(partial, splits, M, N, out, sums, accumulate);
+	N2B_CHECK_LAUNCH();
+	return NEUS2B_OK;
 }
 
 int run_weight_gradient(const Product& p, cudaStream_t stream) {
+	const bool tma = tma_ok(p.a, p.a_ld) && tma_ok(p.b, p.b_ld);
+	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, tma && p.e.out);
+	if (p.workspace_bytes < plan_bytes(w, p.M, p.N)) return NEUS2B_E_INVALID;
 	Args a{};
 	a.bf16 = p.bf16;
 	a.M = p.M, a.N = p.N, a.K = p.K;
 	a.a = (const uint16_t*)p.a, a.a_ld = p.a_ld, a.b = (const uint16_t*)p.b, a.b_ld = p.b_ld;
 	a.e = p.e;
-	a.tiles_m = (p.M + kBM - 1) / kBM;
-	a.tiles_n = (p.N + kWgradBN - 1) / kWgradBN;
-	a.splits = wgrad_splits(p.M, p.N, p.K);
+	a.tiles_m = w.tiles_m, a.tiles_n = w.tiles_n, a.splits = w.splits;
 	a.cluster = 1;
-	a.column_sums = p.column_sums;
-	a.want_sums = p.column_sums != nullptr;
 	a.partial = (float*)p.workspace;
-	if (a.splits > 1 && p.workspace_bytes < partial_bytes(p.M, p.N, p.K)) return NEUS2B_E_INVALID;
 	const uint64_t units = (uint64_t)a.tiles_m * a.tiles_n * a.splits;
 	if (units >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
-	const uint32_t ctas = (uint32_t)(units < (uint64_t)kSMs ? units : kSMs);
-	if (int rc = tma_ok(a.a, a.a_ld) && tma_ok(a.b, a.b_ld) ? launch<kWgradBN, true, true, false, true, false, false>(a, ctas, stream)
-	                                                        : launch<kWgradBN, true, true, false, true, true, false>(a, ctas, stream))
-		return rc;
-	if (a.splits > 1) {
-		const uint64_t entries = (p.e.out ? (uint64_t)p.M * p.N : 0) + (p.column_sums ? p.M : 0);
-		const uint32_t blocks = (uint32_t)((entries + 31) / 32);
-		if (a.splits >= 32) join_kernel<32><<<blocks, dim3(32, 32), 0, stream>>>(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate);
-		else join_kernel<8><<<blocks, dim3(32, 8), 0, stream>>>(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate);
-		N2B_CHECK_LAUNCH();
+	if (w.pair) {
+		// a pair's accumulators fill the tensor memory: the column sums are taken by a pass of their own, ahead of the product, which then
+		// finds the matrix in the L2
+		if (p.column_sums) {
+			const uint32_t most = sum_blocks(p.M), need = tiles_of(p.K, 32), by = need < most ? need : most;
+			column_sums_kernel<<<dim3(tiles_of(p.M, 256), by), 256, 0, stream>>>(a.a, a.a_ld, p.K, p.M, a.bf16, (float*)p.workspace);
+			N2B_CHECK_LAUNCH();
+			if (int rc = run_join((const float*)p.workspace, by, p.M, 0, nullptr, p.column_sums, p.e.accumulate, stream)) return rc;
+		}
+		const uint32_t pairs = (uint32_t)(units < (uint64_t)(kSMs / 2) ? units : kSMs / 2);
+		if (int rc = launch<256, true, true, false, true, false, true>(a, 2 * pairs, stream)) return rc;
+		return w.splits > 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, nullptr, p.e.accumulate, stream) : NEUS2B_OK;
 	}
-	return NEUS2B_OK;
+	a.column_sums = p.column_sums;
+	a.want_sums = p.column_sums != nullptr;
+	const uint32_t ctas = (uint32_t)(units < (uint64_t)kSMs ? units : kSMs);
+	if (int rc = tma ? launch<128, true, true, false, true, false, false>(a, ctas, stream) : launch<128, true, true, false, true, true, false>(a, ctas, stream))
+		return rc;
+	return w.splits > 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate, stream) : NEUS2B_OK;
 }
 
 }  // namespace n2b
