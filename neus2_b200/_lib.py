@@ -250,8 +250,9 @@ def ptr(t):
 
 
 def cur_stream():
+    """Address of the current device's current stream (asked of torch's C module: the Python object around it costs microseconds)."""
     import torch
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def grid_desc(n_levels=16, log2_hashmap_size=19, base_resolution=16, per_level_scale=1.447, n_active_levels=None):

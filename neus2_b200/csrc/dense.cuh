@@ -56,6 +56,28 @@ __device__ __forceinline__ float act_slope(int act, float z) {
 	return 1.f;
 }
 
+// Programmatic launches: a kernel launched with `launch_behind` may start while the kernel ahead of it in the stream still runs, from
+// where all blocks of that one have called `let_next_start` (or ended).  It has to call `wait_for_previous` in every block before it
+// touches memory that others write or read; the call returns when everything ahead in the stream is complete and visible.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+	cudaLaunchConfig_t cfg{};
+	cfg.gridDim = grid;
+	cfg.blockDim = block;
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = stream;
+	cudaLaunchAttribute attr[1];
+	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attr[0].val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = attr;
+	cfg.numAttrs = 1;
+	N2B_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, (P)args...));
+	N2B_CHECK_LAUNCH();
+	return NEUS2B_OK;
+}
+
 template <typename F>
 int with_half_type(uint32_t dtype, F f) {
 	if (dtype == NEUS2B_F16) return f(__half());

@@ -169,7 +169,7 @@ __device__ __forceinline__ void by_type(uint32_t dtype, F f) {
 __global__ void __launch_bounds__(kThreads, 6) norm_partial_kernel(const Piece* __restrict__ pieces, uint32_t n_pieces, uint32_t flags,
                                                                     double* __restrict__ partial, uint32_t* __restrict__ nonfinite) {
 	__shared__ double s[kThreads / 32];
-	asm volatile("griddepcontrol.launch_dependents;");  // the clipping kernel may start on what does not depend on the sums
+	let_next_start();  // the clipping kernel may start on what does not depend on the sums
 	Sum sum;
 	sum.skip = flags & NEUS2B_NORM_SKIP_NONFINITE;
 	Piece p{};
@@ -194,6 +194,7 @@ __device__ __forceinline__ float2 norm_and_factor(const double* __restrict__ par
 }
 
 __global__ void __launch_bounds__(kThreads) norm_final_kernel(const double* __restrict__ partial, uint32_t n, float scale, float max_norm, float* __restrict__ result) {
+	wait_for_previous();
 	const float2 r = norm_and_factor(partial, n, scale, max_norm);
 	if (threadIdx.x == 0) result[0] = r.x, result[1] = r.y;
 }
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 5) clip_kernel(const Piece* __restri
 		});
 	};
 	load(p);
-	asm volatile("griddepcontrol.wait;" ::: "memory");
+	wait_for_previous();
 	const float2 f = norm_and_factor(partial, n_partial, scale, max_norm);
 	if (blockIdx.x == 0 && threadIdx.x == 0) result[0] = f.x, result[1] = f.y;
 	const float c = f.y;
@@ -274,21 +275,10 @@ static int run(const void* d_table, uint32_t n_pieces, float scale, float max_no
 		N2B_CHECK_LAUNCH();
 	}
 	if (clip && blocks) {
-		cudaLaunchConfig_t cfg{};
-		cfg.gridDim = dim3(n_pieces < kClipBlocks ? n_pieces : kClipBlocks);
-		cfg.blockDim = dim3(kThreads);
-		cfg.stream = s;
-		cudaLaunchAttribute attr[1];
-		attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-		attr[0].val.programmaticStreamSerializationAllowed = 1;
-		cfg.attrs = attr;
-		cfg.numAttrs = 1;
-		N2B_CHECK_CUDA(cudaLaunchKernelEx(&cfg, clip_kernel, (const Piece*)d_table, n_pieces, (const double*)d_workspace, blocks, scale, max_norm, d_result));
-	} else {
-		norm_final_kernel<<<1, kThreads, 0, s>>>((const double*)d_workspace, blocks, scale, max_norm, d_result);
+		return launch_behind(clip_kernel, n_pieces < kClipBlocks ? n_pieces : kClipBlocks, kThreads, 0, s, (const Piece*)d_table, n_pieces,
+		                     (const double*)d_workspace, blocks, scale, max_norm, d_result);
 	}
-	N2B_CHECK_LAUNCH();
-	return NEUS2B_OK;
+	return launch_behind(norm_final_kernel, 1, kThreads, 0, s, (const double*)d_workspace, blocks, scale, max_norm, d_result);
 }
 
 }  // namespace n2b

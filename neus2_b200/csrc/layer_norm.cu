@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 	const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
 	const uint32_t W = d.width;
 	const float inv_w = 1.f / (float)W;
+	let_next_start();
 	float ga[E];
 #pragma unroll
 	for (int k = 0; k < E; ++k) {
@@ -467,6 +468,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ partial, uint32_t parts, uint32_t width, float* __restrict__ dgamma,
                                                      float* __restrict__ dbeta, int accumulate) {
 	__shared__ float s[32][33];
+	wait_for_previous();
 	const uint32_t c = blockIdx.x * 32 + threadIdx.x;
 	float v = 0.f;
 	if (c < 2 * width)
@@ -785,8 +787,8 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 			                                              (const T*)d_skip, skip_stride, (T*)d_dL_dx, dx_stride, params ? (float*)d_workspace : nullptr);
 			N2B_CHECK_LAUNCH();
 			if (params) {
-				join_kernel<<<(2 * width + 31) / 32, dim3(32, 32), 0, stream>>>((const float*)d_workspace, blocks, width, d_dgamma, d_dbeta, accumulate);
-				N2B_CHECK_LAUNCH();
+				return launch_behind(join_kernel, (2 * width + 31) / 32, dim3(32, 32), 0, stream, (const float*)d_workspace, blocks, width, d_dgamma, d_dbeta,
+				                     accumulate);
 			}
 			return NEUS2B_OK;
 		};

@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 	const bool bf = p.bf16 != 0;
 	const uint32_t rank = PAIR || p.cluster > 1 ? cluster_rank() : 0u;
+	let_next_start();
 
 	if (tid == 0) {
 		for (int i = 0; i < S::kStages; ++i) {
@@ -348,6 +349,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	else __syncthreads();
 	tc::fence_after_sync();
 	const uint32_t tmem = *tmem_ptr;
+	wait_for_previous();  // the set-up above runs beside the end of the kernel ahead
 
 	// A cluster that splits k computes one tile; a pair, or a CTA by itself, takes every `step`-th.
 	const uint32_t tiles = p.tiles_m * p.tiles_n, kblocks = (p.K + kBK - 1) / kBK;
@@ -696,6 +698,7 @@ template <int ROWS>
 __global__ void __launch_bounds__(32 * ROWS) join_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, float* __restrict__ out,
                                                          float* __restrict__ sums, int accumulate) {
 	__shared__ float s[ROWS][33];
+	wait_for_previous();
 	const uint64_t n = (uint64_t)M * N, total = n + (sums ? M : 0), i = (out ? 0 : n) + blockIdx.x * 32ull + threadIdx.x;
 	const bool is_sum = i >= n;
 	float v = 0.f;
@@ -753,12 +756,14 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 	cfg.blockDim = dim3(S::kThreads);
 	cfg.dynamicSmemBytes = S::kSmem;
 	cfg.stream = stream;
-	cudaLaunchAttribute attr[1];
-	attr[0].id = cudaLaunchAttributeClusterDimension;
-	attr[0].val.clusterDim.x = PAIR ? 2 : a.cluster;
-	attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+	cudaLaunchAttribute attr[2];
+	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attr[0].val.programmaticStreamSerializationAllowed = 1;
+	attr[1].id = cudaLaunchAttributeClusterDimension;
+	attr[1].val.clusterDim.x = PAIR ? 2 : a.cluster;
+	attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
 	cfg.attrs = attr;
-	cfg.numAttrs = PAIR || a.cluster > 1 ? 1 : 0;
+	cfg.numAttrs = PAIR || a.cluster > 1 ? 2 : 1;
 	const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const Args)a);
 	if (e != cudaSuccess) return (int)e;
 	N2B_CHECK_LAUNCH();
@@ -922,10 +927,8 @@ uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {
 static int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
 	const uint64_t entries = (out ? (uint64_t)M * N : 0) + (sums ? M : 0);
 	const uint32_t blocks = (uint32_t)((entries + 31) / 32);
-	if (splits >= 32) join_kernel<32><<<blocks, dim3(32, 32), 0, stream>>>(partial, splits, M, N, out, sums, accumulate);
-	else join_kernel<8><<<blocks, dim3(32, 8), 0, stream>>>(partial, splits, M, N, out, sums, accumulate);
-	N2B_CHECK_LAUNCH();
-	return NEUS2B_OK;
+	if (splits >= 32) return launch_behind(join_kernel<32>, blocks, dim3(32, 32), 0, stream, partial, splits, M, N, out, sums, accumulate);
+	return launch_behind(join_kernel<8>, blocks, dim3(32, 8), 0, stream, partial, splits, M, N, out, sums, accumulate);
 }
 
 int run_weight_gradient(const Product& p, cudaStream_t stream) {
