@@ -50,6 +50,7 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	e.out = d_y, e.out_ld = y_stride, e.bias = d_bias, e.add = d_residual, e.add_ld = residual_stride;
 	e.preact = d_preact, e.preact_ld = preact_stride, e.act = (int)desc->activation;
 	e.vec = whole_vectors(e, out);
+	if (narrow_fits(p, false, nullptr)) return run_narrow(p, false, nullptr, stream);
 	return run_product(p, stream);
 }
 
@@ -61,7 +62,13 @@ static uint64_t dz_bytes(const neus2b_linear_desc* d) {
 extern "C" int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, uint64_t* bytes) {
 	if (bad_desc(desc) || !bytes) return NEUS2B_E_INVALID;
 	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
-	*bytes = dz_bytes(desc) + (desc->n ? wgrad_workspace(desc->out_width, desc->in_width, desc->n) : 0);
+	uint64_t parts = 0;
+	if (desc->n) {
+		const uint64_t narrow = narrow_workspace(desc->out_width, desc->in_width, desc->n);
+		parts = wgrad_workspace(desc->out_width, desc->in_width, desc->n);
+		if (narrow > parts) parts = narrow;
+	}
+	*bytes = dz_bytes(desc) + parts;
 	return NEUS2B_OK;
 }
 
@@ -103,29 +110,30 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		dz = d_workspace;
 		dz_ld = out;
 	}
-	Product p{};
-	p.bf16 = desc->dtype == NEUS2B_BF16;
-	p.a = dz, p.a_ld = dz_ld;
+	Product w{}, x{};  // the weight gradient, the input gradient
+	w.bf16 = x.bf16 = desc->dtype == NEUS2B_BF16;
+	w.a = x.a = dz, w.a_ld = x.a_ld = dz_ld;
 	if (d_wgrad || d_bgrad) {
 		// without a weight gradient the column sums ride on a product of dz with its own first columns that is not stored
-		p.b = d_wgrad ? d_x : dz, p.b_ld = d_wgrad ? x_stride : dz_ld;
-		p.M = out, p.N = d_wgrad ? in : sums_only_width(out), p.K = n;
-		p.a_mn = p.b_mn = true;
-		p.e.out = d_wgrad, p.e.out_ld = in, p.e.out_f32 = 1, p.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
-		p.e.vec = whole_vectors(p.e, in);
-		p.column_sums = d_bgrad;
-		p.workspace = (char*)d_workspace + dz_bytes(desc), p.workspace_bytes = workspace_bytes - dz_bytes(desc);
-		if (int rc = run_weight_gradient(p, stream)) return rc;
+		w.b = d_wgrad ? d_x : dz, w.b_ld = d_wgrad ? x_stride : dz_ld;
+		w.M = out, w.N = d_wgrad ? in : sums_only_width(out), w.K = n;
+		w.a_mn = w.b_mn = true;
+		w.e.out = d_wgrad, w.e.out_ld = in, w.e.out_f32 = 1, w.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
+		w.e.vec = whole_vectors(w.e, in);
+		w.column_sums = d_bgrad;
+		w.workspace = (char*)d_workspace + dz_bytes(desc), w.workspace_bytes = workspace_bytes - dz_bytes(desc);
 	}
-	if (d_dL_dx) {
-		p.b = d_w, p.b_ld = in;
-		p.M = n, p.N = in, p.K = out;
-		p.a_mn = false, p.b_mn = true;
-		p.e = Epilogue{};
-		p.e.out = d_dL_dx, p.e.out_ld = dx_stride, p.e.add = d_skip, p.e.add_ld = skip_stride;
-		if (below_activation != NEUS2B_ACT_NONE) p.e.slope_z = d_below_preact, p.e.slope_ld = below_stride, p.e.act = (int)below_activation;
-		p.e.vec = whole_vectors(p.e, in);
-		if (int rc = run_product(p, stream)) return rc;
-	}
+	x.b = d_w, x.b_ld = in;
+	x.M = n, x.N = in, x.K = out;
+	x.a_mn = false, x.b_mn = true;
+	x.e.out = d_dL_dx, x.e.out_ld = dx_stride, x.e.add = d_skip, x.e.add_ld = skip_stride;
+	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE) x.e.slope_z = d_below_preact, x.e.slope_ld = below_stride, x.e.act = (int)below_activation;
+	x.e.vec = whole_vectors(x.e, in);
+	const Product* params = d_wgrad || d_bgrad ? &w : nullptr;
+	if ((params || d_dL_dx) && narrow_fits(x, true, params)) return run_narrow(x, true, params, stream);
+	if (params)
+		if (int rc = run_weight_gradient(w, stream)) return rc;
+	if (d_dL_dx)
+		if (int rc = run_product(x, stream)) return rc;
 	return NEUS2B_OK;
 }

@@ -62,6 +62,15 @@ __device__ __forceinline__ void store_eight(const Epilogue& e, uint64_t r, uint3
 // width of the product that carries the column sums where no weight gradient is wanted (it is not stored)
 inline uint32_t sums_only_width(uint32_t out_width) { return out_width < 64u ? out_width : 64u; }
 uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n);
+// sums of `splits` parts [M][N] (to out, if not null) and, behind all of them, of `splits` parts [M] (to sums, if not null)
+int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream);
+// Results of up to 64 columns (linear_narrow.cu).  forward or input gradient: `rows` the product for dL/dx or y, `weights` null or the
+// weight gradient that shares its first operand.
+bool narrow_fits(const Product& rows, bool backward, const Product* weights);
+uint64_t narrow_workspace(uint32_t out_width, uint32_t in_width, uint32_t n);
+int run_narrow(const Product& rows, bool backward, const Product* weights, cudaStream_t stream);
+int read_narrow_error(uint32_t* flags);
+int write_narrow_error(uint32_t flags);
 int run_product(const Product& p, cudaStream_t stream);         // forward and input gradient; p.M samples, p.N features
 int run_weight_gradient(const Product& p, cudaStream_t stream);  // p.M = out_width, p.N = in_width, p.K = n
 

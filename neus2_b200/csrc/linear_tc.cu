@@ -5,19 +5,14 @@
 // where rows do not start on 16-byte boundaries, by warps that shift them into place (GATHER).  Both layouts of an operand are
 // read as they lie in memory: [m][k] is a K-major tile (128 rows of 64 k), [k][m] an MN-major one (slabs of 64 k x 64 m), so neither
 // backward product transposes anything.
-#include <cuda.h>
-
-#include "linear.cuh"
-#include "tc05.cuh"
+#include "linear_tc.cuh"
 
 namespace n2b {
 namespace lin {
 
 static __device__ uint32_t g_error;  // bit 0: a bounded wait ran out
 
-constexpr int kBM = 128, kBK = 64;
 constexpr int kGatherWarps = 7;
-constexpr int kMaxStages = 8, kSmemMost = 227 * 1024;
 constexpr int kChunkBytes = 32 * 64;  // 32 x 32 values on their way between the epilogue and global memory
 constexpr int kChunk = 8;  // weight gradient: k blocks (512 samples) summed in tensor memory before the sum moves to registers
 
@@ -32,125 +27,6 @@ struct alignas(64) Args {
 	uint32_t want_sums;
 	Epilogue e;
 };
-
-__device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ uint64_t now_ns() {
-	uint64_t t;
-	asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-	return t;
-}
-// False when the phase has not completed after four seconds: nothing that a tile waits for takes a millisecond, and every copy that
-// was issued has landed long before a role gives up and the CTA ends.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
-	uint64_t start = 0;
-	for (uint32_t it = 0;; ++it) {
-		uint32_t ok;
-		asm volatile(
-		    "{\n\t.reg .pred p;\n\t"
-		    "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-		    "selp.u32 %0, 1, 0, p;\n\t}"
-		    : "=r"(ok)
-		    : "r"(bar), "r"(parity)
-		    : "memory");
-		if (ok) return true;
-		if ((it & 63u) == 63u) {
-			const uint64_t t = now_ns();
-			if (!start) start = t;
-			else if (t - start > 4000000000ull) return false;
-		}
-	}
-}
-__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
-	asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// x: first column (a multiple of 64), y: first row of a [rows][columns] matrix.  PAIR: the barrier may be the other CTA's.
-template <bool PAIR>
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-	if (PAIR)
-		asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
-		             "r"(x), "r"(y), "r"(bar)
-		             : "memory");
-	else
-		asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
-		             "r"(x), "r"(y), "r"(bar)
-		             : "memory");
-}
-__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
-	uint32_t p;
-	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-	return p;
-}
-__device__ __forceinline__ void arrive_remote(uint32_t bar) {
-	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
-	if (PAIR) {
-		asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
-		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-	} else {
-		tc::tmem_alloc(dst, cols);
-	}
-}
-template <bool PAIR>
-__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
-	if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
-	else tc::tmem_dealloc(addr, cols);
-}
-template <bool PAIR>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t more) {
-	if (PAIR)
-		asm volatile(
-		    "{\n\t.reg .pred p;\n\t"
-		    "setp.ne.b32 p, %4, 0;\n\t"
-		    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-		    :
-		    : "r"(d), "l"(a), "l"(b), "r"(id), "r"(more)
-		    : "memory");
-	else tc::mma_f16(d, a, b, id, more);
-}
-// PAIR: arrives at the barrier of this place in both CTAs.
-template <bool PAIR>
-__device__ __forceinline__ void commit(uint32_t bar) {
-	if (PAIR)
-		asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-	else tc::commit(bar);
-}
-// Matrix descriptors of the two 128-byte-swizzled layouts.  K-major: rows of 64 k, 8-row groups 1024 bytes apart.  MN-major: rows of
-// 64 m (or n), one per k, 8-row groups 1024 bytes apart, slabs of 64 m 8192 bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-	return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-	return (uint64_t)((addr >> 4) & 0x3FFFu) | (512ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void tmem_ld16_raw(uint32_t taddr, uint32_t (&r)[16]) {
-	asm volatile(
-	    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-	    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-	      "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-	    : "r"(taddr)
-	    : "memory");
-}
-__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
-	asm volatile("tcgen05.wait::ld.sync.aligned;"
-	             : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-	               "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-	uint32_t r;
-	asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-	return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
-	float v;
-	asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(addr, rank)) : "memory");
-	return v;
-}
 
 // ROWS rows of 64 columns from (row0, col0) of a [rows][cols] matrix of any alignment into a swizzled tile; zeros outside.  Eight values
 // that start at any even address are two aligned 16-byte loads and a shift.  The loads may reach up to 14 bytes around the values: they
@@ -288,32 +164,6 @@ __device__ __forceinline__ void chunk_store(const uint32_t (&row)[16], void* bas
 		}
 	}
 }
-__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf) {
-	return bf ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf) {
-	if (bf) {
-		const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-		return *reinterpret_cast<const uint32_t*>(&h);
-	}
-	const __half2 h = __floats2half2_rn(a, b);
-	return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <int ACT>
-__device__ __forceinline__ void apply_act(float (&v)[32]) {
-#pragma unroll
-	for (int i = 0; i < 32; ++i) v[i] = act_value(ACT, v[i]);
-}
-template <int ACT>
-__device__ __forceinline__ void apply_slope(float (&v)[32], const uint32_t (&z)[16], bool bf) {
-#pragma unroll
-	for (int i = 0; i < 16; ++i) {
-		const float2 f = unpack2(z[i], bf);
-		v[2 * i] *= act_slope(ACT, f.x);
-		v[2 * i + 1] *= act_slope(ACT, f.y);
-	}
-}
-
 template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
 __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>::kThreads, 1) product_kernel(const __grid_constant__ Args p) {
 	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
@@ -718,30 +568,6 @@ __global__ void __launch_bounds__(32 * ROWS) join_kernel(const float* __restrict
 	}
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeFn encode_fn() {
-	static EncodeFn fn = [] {
-		void* q = nullptr;
-		cudaDriverEntryPointQueryResult res;
-		if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &q, 12000, cudaEnableDefault, &res) != cudaSuccess) q = nullptr;
-		return (EncodeFn)q;
-	}();
-	return fn;
-}
-// [rows][cols] matrix read in boxes of 64 columns and box_rows rows
-static int make_map(CUtensorMap* map, const void* base, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t box_rows, bool bf16) {
-	const EncodeFn fn = encode_fn();
-	if (!fn) return NEUS2B_E_NO_DEVICE;
-	const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
-	const cuuint32_t box[2] = {64, box_rows}, unit[2] = {1, 1};
-	const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, unit,
-	                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-	return r == CUDA_SUCCESS ? NEUS2B_OK : NEUS2B_E_INVALID;
-}
-// TMA reads rows that start on 16-byte boundaries, less than 2^40 bytes apart
-static bool tma_ok(const void* p, uint64_t ld) { return ((uintptr_t)p & 15u) == 0 && (ld & 7u) == 0 && ld < (1ull << 39); }
-
 template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
 static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
@@ -776,7 +602,6 @@ static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks) {
 	while (c < 8 && tiles * c * 2 <= (uint64_t)kSMs && kblocks >= c * 2 * 4) c *= 2;
 	return c;
 }
-static uint32_t tiles_of(uint32_t n, uint32_t size) { return (n + size - 1) / size; }
 
 template <bool BMN>
 static int product_of(const Product& p, cudaStream_t stream) {
@@ -904,12 +729,16 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __rest
 using namespace lin;
 
 int read_linear_error(uint32_t* flags) {
+	uint32_t narrow = 0;
 	const cudaError_t e = cudaMemcpyFromSymbol(flags, g_error, sizeof(*flags));
-	return e == cudaSuccess ? NEUS2B_OK : (int)e;
+	if (e != cudaSuccess) return (int)e;
+	if (int rc = read_narrow_error(&narrow)) return rc;
+	*flags |= narrow;
+	return NEUS2B_OK;
 }
 int write_linear_error(uint32_t flags) {
 	const cudaError_t e = cudaMemcpyToSymbol(g_error, &flags, sizeof(flags));
-	return e == cudaSuccess ? NEUS2B_OK : (int)e;
+	return e == cudaSuccess ? write_narrow_error(flags) : (int)e;
 }
 
 int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product_of<true>(p, stream) : product_of<false>(p, stream); }
@@ -924,7 +753,7 @@ uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {
 	return most;
 }
 
-static int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
+int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
 	const uint64_t entries = (out ? (uint64_t)M * N : 0) + (sums ? M : 0);
 	const uint32_t blocks = (uint32_t)((entries + 31) / 32);
 	if (splits >= 32) return launch_behind(join_kernel<32>, blocks, dim3(32, 32), 0, stream, partial, splits, M, N, out, sums, accumulate);
