@@ -384,10 +384,15 @@ typedef struct {
 
 /* z = x W^T + bias, y = act(z) + residual.  d_x [n][in_width], d_w [out_width][in_width] (rows contiguous), d_bias [out_width] or
  * NULL, d_residual [n][out_width] or NULL, d_y [n][out_width], d_preact [n][out_width] or NULL: receives z, which the backward
- * pass of an activated layer reads.  The sum and the epilogue are fp32, y and z are rounded once.  d_residual may be d_y. */
+ * pass of an activated layer reads.  The sum and the epilogue are fp32, y and z are rounded once.  d_residual may be d_y (with the
+ * same stride).  d_workspace: neus2b_linear_forward_workspace bytes, 16-byte aligned; NULL and 0 where that is 0.  `unaligned`: whether
+ * rows of x or W may start off 16-byte boundaries (the address, or the stride, or in_width for W, times 2 bytes): with more than a few
+ * samples they are then copied to where they do.  Nothing in a workspace is kept between calls; calls that may run at the same time
+ * need workspaces of their own. */
+int neus2b_linear_forward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes);
 int neus2b_linear_forward(const neus2b_linear_desc* desc, const void* d_x, uint64_t x_stride, const void* d_w, const void* d_bias,
                           const void* d_residual, uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_preact,
-                          uint64_t preact_stride, neus2b_stream_t stream);
+                          uint64_t preact_stride, void* d_workspace, uint64_t workspace_bytes, neus2b_stream_t stream);
 
 /* The backward pass.  With dz = dL/dy * act'(z):
  *   d_dL_dx [n][in_width] = (dz W) * act_below'(z_below) + skip      (NULL: not computed)
@@ -395,10 +400,9 @@ int neus2b_linear_forward(const neus2b_linear_desc* desc, const void* d_x, uint6
  * d_preact: z of this layer, read when desc->activation is not NONE; dz is then rounded to the layer's type in the workspace.
  * below_activation, d_below_preact: what the layer below applied to get x, so that d_dL_dx is already the gradient of that layer's
  * z and the chain needs no pass of its own over it (NEUS2B_ACT_NONE and NULL: plain dL/dx).  d_skip [n][in_width] or NULL: the
- * gradient that reaches x around this layer (a residual connection); it may be d_dL_dx.
- * d_workspace: neus2b_linear_backward_workspace bytes, 16-byte aligned; nothing in it is kept between calls.  Calls that may run
- * at the same time need workspaces of their own. */
-int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, uint64_t* bytes);
+ * gradient that reaches x around this layer (a residual connection); it may be d_dL_dx (with the same stride).
+ * d_workspace: neus2b_linear_backward_workspace bytes, as for the forward pass (`unaligned`: rows of x, W or dL/dy). */
+int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes);
 int neus2b_linear_backward(const neus2b_linear_desc* desc, const void* d_x, uint64_t x_stride, const void* d_w, const void* d_preact,
                            uint64_t preact_stride, const void* d_dL_dy, uint64_t dy_stride, uint32_t below_activation,
                            const void* d_below_preact, uint64_t below_stride, const void* d_skip, uint64_t skip_stride, void* d_dL_dx,

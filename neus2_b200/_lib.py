@@ -143,7 +143,7 @@ EXPORTS = [
     "neus2b_neus_forward_moved", "neus2b_neus_forward_indexed", "neus2b_forward_compute_loss", "neus2b_neus_train_moved", "neus2b_neus_sdf_moved", "neus2b_delta_forward", "neus2b_delta_backward",
     "neus2b_delta_optimizer_step", "neus2b_movement_accumulate", "neus2b_occupancy_update_moved", "neus2b_pcg32_seed", "neus2b_pcg32_advance", "neus2b_abi_struct_sizes",
     "neus2b_generate_samples", "neus2b_generate_samples_static", "neus2b_compute_loss", "neus2b_occupancy_update", "neus2b_occupancy_bounds", "neus2b_adam_step", "neus2b_adam_step_packed",
-    "neus2b_linear_forward", "neus2b_linear_backward_workspace", "neus2b_linear_backward", "neus2b_layer_norm_forward",
+    "neus2b_linear_forward_workspace", "neus2b_linear_forward", "neus2b_linear_backward_workspace", "neus2b_linear_backward", "neus2b_layer_norm_forward",
     "neus2b_layer_norm_backward_workspace", "neus2b_layer_norm_backward", "neus2b_grad_table", "neus2b_grad_norm_workspace", "neus2b_grad_norm",
     "neus2b_grad_clip",
     "neus2b_testbed_default_config", "neus2b_testbed_create", "neus2b_testbed_destroy", "neus2b_testbed_load_training_data",
@@ -175,8 +175,9 @@ def lib():
         _lib.neus2b_testbed_config_active_levels.restype = C.c_uint32
         _lib.neus2b_launch_count.restype = C.c_uint64
         p, u64 = C.c_void_p, C.c_uint64
-        _lib.neus2b_linear_forward.argtypes = [p, p, u64, p, p, p, u64, p, u64, p, u64, p]
-        _lib.neus2b_linear_backward_workspace.argtypes = [p, p]
+        _lib.neus2b_linear_forward_workspace.argtypes = [p, C.c_int, p]
+        _lib.neus2b_linear_forward.argtypes = [p, p, u64, p, p, p, u64, p, u64, p, u64, p, u64, p]
+        _lib.neus2b_linear_backward_workspace.argtypes = [p, C.c_int, p]
         _lib.neus2b_linear_backward.argtypes = [p, p, u64, p, p, u64, p, u64, C.c_uint32, p, u64, p, u64, p, u64, p, p, C.c_int, p, u64, p]
         _lib.neus2b_layer_norm_forward.argtypes = [p, p, u64, p, p, p, u64, p, p, p]
         _lib.neus2b_layer_norm_backward_workspace.argtypes = [p, p]

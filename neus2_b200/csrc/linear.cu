@@ -6,11 +6,11 @@ namespace n2b {
 // dz = dy * act'(z)
 template <typename T>
 __global__ void __launch_bounds__(256) slope_kernel(uint64_t n, uint32_t width, int act, const T* __restrict__ z, uint64_t z_ld,
-                                                     const T* __restrict__ dy, uint64_t dy_ld, T* __restrict__ dz) {
+                                                     const T* __restrict__ dy, uint64_t dy_ld, T* __restrict__ dz, uint64_t dz_ld) {
 	for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n * width; i += gridDim.x * 256ull) {
 		const uint64_t r = i / width;
 		const uint32_t c = (uint32_t)(i - r * width);
-		dz[i] = from_f<T>(to_f(dy[r * dy_ld + c]) * act_slope(act, to_f(z[r * z_ld + c])));
+		dz[r * dz_ld + c] = from_f<T>(to_f(dy[r * dy_ld + c]) * act_slope(act, to_f(z[r * z_ld + c])));
 	}
 }
 
@@ -32,11 +32,28 @@ static int whole_vectors(const Epilogue& e, uint32_t width) {
 
 using namespace n2b;
 
+// A copy of a matrix with rows on 16-byte boundaries
+static uint64_t copy_bytes(uint64_t rows, uint32_t cols) { return (rows * ((cols + 7) / 8) * 16 + 255) / 256 * 256; }
+// Takes the place of a product's operand by its copy, where it needs one; `at` moves on behind it.
+static void realigned(const void*& p, uint64_t& ld, uint32_t rows, uint32_t cols, char*& at, Operand* ops, int& count) {
+	if (operand_aligned(p, ld)) return;
+	ops[count++] = Operand{p, ld, rows, cols, at};
+	p = at, ld = (cols + 7) / 8 * 8;
+	at += copy_bytes(rows, cols);
+}
+
+extern "C" int neus2b_linear_forward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes) {
+	if (bad_desc(desc) || !bytes) return NEUS2B_E_INVALID;
+	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
+	*bytes = unaligned && desc->n > kFewSamples ? copy_bytes(desc->n, desc->in_width) + copy_bytes(desc->out_width, desc->in_width) : 0;
+	return NEUS2B_OK;
+}
+
 extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void* d_x, uint64_t x_stride, const void* d_w, const void* d_bias,
                                      const void* d_residual, uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_preact,
-                                     uint64_t preact_stride, neus2b_stream_t stream) {
-	if (bad_desc(desc)) return NEUS2B_E_INVALID;
-	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
+                                     uint64_t preact_stride, void* d_workspace, uint64_t workspace_bytes, neus2b_stream_t stream) {
+	uint64_t need = 0;
+	if (int rc = neus2b_linear_forward_workspace(desc, 1, &need)) return rc;
 	const uint32_t in = desc->in_width, out = desc->out_width;
 	if (bad_matrix(d_w, in, in, 2) || ((uintptr_t)d_bias & 1)) return NEUS2B_E_INVALID;
 	if (desc->n == 0) return NEUS2B_OK;
@@ -46,6 +63,15 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	Product p{};
 	p.a = d_x, p.a_ld = x_stride, p.b = d_w, p.b_ld = in;
 	p.M = desc->n, p.N = out, p.K = in, p.bf16 = desc->dtype == NEUS2B_BF16;
+	if (desc->n > kFewSamples && !(operand_aligned(p.a, p.a_ld) && operand_aligned(p.b, p.b_ld))) {
+		if (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need) return NEUS2B_E_INVALID;
+		Operand ops[2];
+		int count = 0;
+		char* at = (char*)d_workspace;
+		realigned(p.a, p.a_ld, desc->n, in, at, ops, count);
+		realigned(p.b, p.b_ld, out, in, at, ops, count);
+		if (int rc = run_realign(ops, count, stream)) return rc;
+	}
 	Epilogue& e = p.e;
 	e.out = d_y, e.out_ld = y_stride, e.bias = d_bias, e.add = d_residual, e.add_ld = residual_stride;
 	e.preact = d_preact, e.preact_ld = preact_stride, e.act = (int)desc->activation;
@@ -54,12 +80,13 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	return run_product(p, stream);
 }
 
-// workspace: dz where the layer has an activation, then what the weight gradient needs
-static uint64_t dz_bytes(const neus2b_linear_desc* d) {
-	return d->activation == NEUS2B_ACT_NONE ? 0 : ((uint64_t)d->n * d->out_width * 2 + 255) / 256 * 256;
+// Workspace of the backward pass: dz where the layer has an activation, copies of unaligned operands, what the weight gradient needs.
+static uint64_t dz_bytes(const neus2b_linear_desc* d) { return d->activation == NEUS2B_ACT_NONE ? 0 : copy_bytes(d->n, d->out_width); }
+static uint64_t copies_bytes(const neus2b_linear_desc* d) {
+	return copy_bytes(d->n, d->out_width) + copy_bytes(d->n, d->in_width) + copy_bytes(d->out_width, d->in_width);
 }
 
-extern "C" int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, uint64_t* bytes) {
+extern "C" int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes) {
 	if (bad_desc(desc) || !bytes) return NEUS2B_E_INVALID;
 	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
 	uint64_t parts = 0;
@@ -68,7 +95,7 @@ extern "C" int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, 
 		parts = wgrad_workspace(desc->out_width, desc->in_width, desc->n);
 		if (narrow > parts) parts = narrow;
 	}
-	*bytes = dz_bytes(desc) + parts;
+	*bytes = dz_bytes(desc) + (unaligned ? copies_bytes(desc) : 0) + parts;
 	return NEUS2B_OK;
 }
 
@@ -78,7 +105,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
                                       uint64_t dx_stride, float* d_wgrad, float* d_bgrad, int grad_mode, void* d_workspace,
                                       uint64_t workspace_bytes, neus2b_stream_t stream) {
 	uint64_t need = 0;
-	if (int rc = neus2b_linear_backward_workspace(desc, &need)) return rc;
+	if (int rc = neus2b_linear_backward_workspace(desc, 0, &need)) return rc;
 	if (below_activation > NEUS2B_ACT_SILU || grad_mode < NEUS2B_GRAD_IGNORE || grad_mode > NEUS2B_GRAD_ACCUMULATE) return NEUS2B_E_INVALID;
 	const uint32_t n = desc->n, in = desc->in_width, out = desc->out_width;
 	if (grad_mode == NEUS2B_GRAD_IGNORE) d_wgrad = d_bgrad = nullptr;
@@ -96,41 +123,55 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	if (desc->activation != NEUS2B_ACT_NONE && bad_matrix(d_preact, preact_stride, out, 2)) return NEUS2B_E_INVALID;
 	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE && bad_matrix(d_below_preact, below_stride, in, 2)) return NEUS2B_E_INVALID;
 	if (need && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need)) return NEUS2B_E_INVALID;
-	const void* dz = d_dL_dy;
-	uint64_t dz_ld = dy_stride;
+	const void *dz = d_dL_dy, *xs = d_x, *ws = d_w;
+	uint64_t dz_ld = dy_stride, xs_ld = x_stride, ws_ld = in;
+	char* at = (char*)d_workspace;
 	if (desc->activation != NEUS2B_ACT_NONE) {
+		const uint64_t ld = (out + 7) / 8 * 8;
 		const int rc = with_half_type(desc->dtype, [&](auto t) {
 			using T = decltype(t);
 			slope_kernel<T><<<kSMs * 8, 256, 0, stream>>>(n, out, (int)desc->activation, (const T*)d_preact, preact_stride, (const T*)d_dL_dy, dy_stride,
-			                                           (T*)d_workspace);
+			                                           (T*)d_workspace, ld);
 			N2B_CHECK_LAUNCH();
 			return NEUS2B_OK;
 		});
 		if (rc) return rc;
-		dz = d_workspace;
-		dz_ld = out;
+		dz = d_workspace, dz_ld = ld;
+		at += dz_bytes(desc);
+	}
+	const bool params = d_wgrad || d_bgrad;
+	// the input gradient of a few samples reads rows anywhere, the weight gradient does not
+	const bool copy_dz = !operand_aligned(dz, dz_ld) && (params || (d_dL_dx && n > kFewSamples)), copy_x = d_wgrad && !operand_aligned(xs, xs_ld),
+	           copy_w = d_dL_dx && n > kFewSamples && !operand_aligned(ws, ws_ld);
+	if (copy_dz || copy_x || copy_w) {
+		if (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need + copies_bytes(desc)) return NEUS2B_E_INVALID;
+		Operand ops[3];
+		int count = 0;
+		if (copy_dz) realigned(dz, dz_ld, n, out, at, ops, count);
+		if (copy_x) realigned(xs, xs_ld, n, in, at, ops, count);
+		if (copy_w) realigned(ws, ws_ld, out, in, at, ops, count);
+		if (int rc = run_realign(ops, count, stream)) return rc;
 	}
 	Product w{}, x{};  // the weight gradient, the input gradient
 	w.bf16 = x.bf16 = desc->dtype == NEUS2B_BF16;
 	w.a = x.a = dz, w.a_ld = x.a_ld = dz_ld;
-	if (d_wgrad || d_bgrad) {
+	if (params) {
 		// without a weight gradient the column sums ride on a product of dz with its own first columns that is not stored
-		w.b = d_wgrad ? d_x : dz, w.b_ld = d_wgrad ? x_stride : dz_ld;
+		w.b = d_wgrad ? xs : dz, w.b_ld = d_wgrad ? xs_ld : dz_ld;
 		w.M = out, w.N = d_wgrad ? in : sums_only_width(out), w.K = n;
 		w.a_mn = w.b_mn = true;
 		w.e.out = d_wgrad, w.e.out_ld = in, w.e.out_f32 = 1, w.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
 		w.e.vec = whole_vectors(w.e, in);
 		w.column_sums = d_bgrad;
-		w.workspace = (char*)d_workspace + dz_bytes(desc), w.workspace_bytes = workspace_bytes - dz_bytes(desc);
+		w.workspace = at, w.workspace_bytes = workspace_bytes - (uint64_t)(at - (char*)d_workspace);
 	}
-	x.b = d_w, x.b_ld = in;
+	x.b = ws, x.b_ld = ws_ld;
 	x.M = n, x.N = in, x.K = out;
 	x.a_mn = false, x.b_mn = true;
 	x.e.out = d_dL_dx, x.e.out_ld = dx_stride, x.e.add = d_skip, x.e.add_ld = skip_stride;
 	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE) x.e.slope_z = d_below_preact, x.e.slope_ld = below_stride, x.e.act = (int)below_activation;
 	x.e.vec = whole_vectors(x.e, in);
-	const Product* params = d_wgrad || d_bgrad ? &w : nullptr;
-	if ((params || d_dL_dx) && narrow_fits(x, true, params)) return run_narrow(x, true, params, stream);
+	if ((params || d_dL_dx) && narrow_fits(x, true, params ? &w : nullptr)) return run_narrow(x, true, params ? &w : nullptr, stream);
 	if (params)
 		if (int rc = run_weight_gradient(w, stream)) return rc;
 	if (d_dL_dx)

@@ -71,6 +71,16 @@ uint64_t narrow_workspace(uint32_t out_width, uint32_t in_width, uint32_t n);
 int run_narrow(const Product& rows, bool backward, const Product* weights, cudaStream_t stream);
 int read_narrow_error(uint32_t* flags);
 int write_narrow_error(uint32_t flags);
+// Rows on 16-byte boundaries, as the product kernels read them (with up to kFewSamples samples run_product takes any).
+constexpr uint32_t kFewSamples = 64;
+struct Operand {
+	const void* from;
+	uint64_t ld;
+	uint32_t rows, cols;
+	void* to;  // [rows][cols rounded up to 8]
+};
+bool operand_aligned(const void* p, uint64_t ld);
+int run_realign(const Operand* ops, int count, cudaStream_t stream);  // three at most
 int run_product(const Product& p, cudaStream_t stream);         // forward and input gradient; p.M samples, p.N features
 int run_weight_gradient(const Product& p, cudaStream_t stream);  // p.M = out_width, p.N = in_width, p.K = n
 

@@ -12,7 +12,7 @@ namespace lin {
 
 static __device__ uint32_t g_error;  // bit 0: a bounded wait ran out
 
-constexpr int kGatherWarps = 7;
+constexpr int kGatherWarps = 11;
 constexpr int kChunkBytes = 32 * 64;  // 32 x 32 values on their way between the epilogue and global memory
 constexpr int kChunk = 8;  // weight gradient: k blocks (512 samples) summed in tensor memory before the sum moves to registers
 
@@ -28,61 +28,66 @@ struct alignas(64) Args {
 	Epilogue e;
 };
 
-// ROWS rows of 64 columns from (row0, col0) of a [rows][cols] matrix of any alignment into a swizzled tile; zeros outside.  Eight values
-// that start at any even address are two aligned 16-byte loads and a shift.  The loads may reach up to 14 bytes around the values: they
-// are used only where that stays inside the matrix's extent in memory, which is the caller's.  All loads of a thread (four pieces at a
-// time) are in flight before the first is used.
-template <int ROWS>
-__device__ __forceinline__ void gather_box(unsigned char* dst, const uint16_t* base, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t row0, uint32_t col0,
-                                           int tid) {
-	constexpr int kThreads = kGatherWarps * 32, kBatch = 4;
-	const char* begin = reinterpret_cast<const char*>(base);
-	const char* end = begin + ((uint64_t)(rows - 1) * ld + cols) * 2;
-	for (int u0 = tid; u0 < ROWS * 8; u0 += kBatch * kThreads) {
-		uint4 lo[kBatch], hi[kBatch];
+// One 16-byte unit of an operand tile, eight values that start at any even address of a [rows][cols] matrix: two aligned 16-byte loads and
+// a shift; zeros outside of the matrix.  The loads may reach up to 14 bytes around the values: they are used only where that stays inside
+// the matrix's extent in memory, which is the caller's.
+struct Unit {
+	uint4 lo, hi;
+	uint32_t shift;
+};
+__device__ __forceinline__ void unit_fetch(Unit& v, const uint16_t* base, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t row, uint32_t col) {
+	v.lo = v.hi = make_uint4(0, 0, 0, 0);
+	v.shift = 0;
+	if (row >= rows || col >= cols) return;
+	const char *begin = reinterpret_cast<const char*>(base), *end = begin + ((uint64_t)(rows - 1) * ld + cols) * 2;
+	const uint16_t* p = base + (uint64_t)row * ld + col;
+	const char* q = reinterpret_cast<const char*>(p);
+	v.shift = (uint32_t)(uintptr_t)q & 15u;
+	const char* down = q - v.shift;
+	if (col + 8 <= cols && down >= begin && down + 32 <= end) {
+		v.lo = __ldg(reinterpret_cast<const uint4*>(down));
+		v.hi = __ldg(reinterpret_cast<const uint4*>(down) + 1);
+	} else {  // at the matrix's edges: entry by entry
+		uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-		for (int j = 0; j < kBatch; ++j) {
-			const int u = u0 + j * kThreads;
-			const uint32_t row = row0 + (u >> 3), col = col0 + (u & 7) * 8;
-			lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
-			if (u < ROWS * 8 && row < rows && col < cols) {
-				const uint16_t* p = base + (uint64_t)row * ld + col;
-				const char* q = reinterpret_cast<const char*>(p);
-				const char* down = q - ((uintptr_t)q & 15u);
-				if (col + 8 <= cols && down >= begin && down + 32 <= end) {
-					lo[j] = __ldg(reinterpret_cast<const uint4*>(down));
-					hi[j] = __ldg(reinterpret_cast<const uint4*>(down) + 1);
-				} else {  // at the matrix's edges: entry by entry, put where the aligned loads would have put them
-					uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-					const uint32_t first = ((uint32_t)(uintptr_t)q & 15u) >> 1;
+		for (int i = 0; i < 8; ++i)
+			if (col + i < cols) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+		v.lo = make_uint4(w[0], w[1], w[2], w[3]);
+		v.shift = 0;
+	}
+}
+__device__ __forceinline__ uint4 unit_value(const Unit& v) {
+	uint32_t w[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
+	if (v.shift & 8u) {
 #pragma unroll
-					for (int i = 0; i < 16; ++i)
-						if ((uint32_t)i >= first && (uint32_t)i < first + 8u && col + (i - first) < cols) w[i >> 1] |= (uint32_t)p[i - first] << (16 * (i & 1));
-					lo[j] = make_uint4(w[0], w[1], w[2], w[3]);
-					hi[j] = make_uint4(w[4], w[5], w[6], w[7]);
-				}
-			}
-		}
+		for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+	}
+	if (v.shift & 4u) {
 #pragma unroll
-		for (int j = 0; j < kBatch; ++j) {
-			const int u = u0 + j * kThreads;
-			if (u >= ROWS * 8) break;
-			const uint32_t row = row0 + (u >> 3), col = col0 + (u & 7) * 8;
-			const uint32_t s = (uint32_t)(uintptr_t)(base + (uint64_t)row * ld + col) & 15u;
-			uint32_t w[8] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w, hi[j].x, hi[j].y, hi[j].z, hi[j].w};
-			if (s & 8u) {
-#pragma unroll
-				for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-			}
-			if (s & 4u) {
-#pragma unroll
-				for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-			}
-			const uint32_t b = (s & 2u) * 8u;
-			const int r = u >> 3, c8 = u & 7;
-			*reinterpret_cast<uint4*>(dst + r * 128 + ((c8 ^ (r & 7)) << 4)) =
-			    make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b), __funnelshift_r(w[2], w[3], b), __funnelshift_r(w[3], w[4], b));
-		}
+		for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+	}
+	const uint32_t b = (v.shift & 2u) * 8u;
+	return make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b), __funnelshift_r(w[2], w[3], b), __funnelshift_r(w[3], w[4], b));
+}
+
+// Copies of up to three matrices with rows on 16-byte boundaries, for operands that have none: thread = 16 bytes of a copy.
+struct Realign {
+	const uint16_t* from[3];
+	uint64_t from_ld[3];
+	uint16_t* to[3];
+	uint32_t rows[3], cols[3];
+	uint64_t units[4];  // first unit of each, and behind the last
+};
+__global__ void __launch_bounds__(256) realign_kernel(const Realign r) {
+	let_next_start();
+	wait_for_previous();
+	for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < r.units[3]; i += gridDim.x * 256ull) {
+		const int k = i >= r.units[2] ? 2 : i >= r.units[1] ? 1 : 0;
+		const uint64_t u = i - r.units[k];
+		const uint32_t per = (r.cols[k] + 7) / 8, row = (uint32_t)(u / per), col = (uint32_t)(u - (uint64_t)row * per) * 8;
+		Unit v;
+		unit_fetch(v, r.from[k], r.from_ld[k], r.rows[k], r.cols[k], row, col);
+		*reinterpret_cast<uint4*>(r.to[k] + (uint64_t)row * per * 8 + col) = unit_value(v);
 	}
 }
 
@@ -91,12 +96,13 @@ __device__ __forceinline__ void gather_box(unsigned char* dst, const uint16_t* b
 // keep up with the MMAs: on wide tiles they share the columns, narrow ones (BN 64) go to four groups in turn, each with an accumulator.
 template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
 struct Shape {
+	static_assert(!GATHER || SWAP, "operands of larger products are realigned ahead of them");
 	static constexpr int kBRows = PAIR ? BN / 2 : BN;  // of B's tile in this CTA
 	static constexpr int kABytes = kBM * 128;
 	static constexpr int kBBytes = (BMN && kBRows < 64 ? 64 : kBRows) * 128;
 	static constexpr int kStage = kABytes + kBBytes;
-	static constexpr bool kTurns = BN == 64 && !SWAP && !WGRAD, kMany = !GATHER && !SWAP && !WGRAD && (PAIR || BN <= 128);
-	static constexpr int kHalves = kTurns ? 1 : kMany ? 4 : 2, kGroups = kTurns ? (kMany ? 4 : 2) : 1, kBufs = kTurns ? 4 : 2;
+	static constexpr bool kTurns = BN == 64 && !SWAP && !WGRAD, kMany = !SWAP && !WGRAD && (PAIR || BN <= 128);
+	static constexpr int kHalves = kTurns || GATHER ? 1 : kMany ? 4 : 2, kGroups = kTurns ? 4 : 1, kBufs = kTurns ? 4 : 2;
 	static constexpr int kEpiWarps = 4 * kHalves * kGroups, kMmaWarp = kEpiWarps, kLoadWarp = kEpiWarps + 1;
 	static constexpr int kThreads = (GATHER ? kLoadWarp + kGatherWarps : kLoadWarp + 1) * 32;
 	static constexpr int kBounce = SWAP || WGRAD ? 0 : kEpiWarps * 3 * kChunkBytes;  // a result, a slope and an addend chunk for every epilogue warp
@@ -221,56 +227,76 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 		kb1 = (uint32_t)((uint64_t)(split + 1) * kblocks / p.splits);
 	};
 
-	if (warp >= S::kLoadWarp) {
-		// ---------------------------------------------------------------- operand tiles
+	if (GATHER && warp >= S::kLoadWarp) {
+		// ---------------------------------------------------------------- operand tiles, rows anywhere: the next tile's units are on their way
+		// while this one's are put into place
+		constexpr int kUnits = (kBM + BN) * 8, kEach = (kUnits + kGatherWarps * 32 - 1) / (kGatherWarps * 32);
+		const int t = tid - S::kLoadWarp * 32;
 		uint32_t stage = 0, phase = 0;
-		const uint32_t full_lead = PAIR ? peer_address(full, 0) : full;  // a pair's tiles are counted in by the first CTA
 		for (uint32_t u = first; u < units && ok; u += step) {
 			uint32_t mt, nt, split, kb0, kb1;
 			locate(u, mt, nt, split, kb0, kb1);
-			const uint32_t m0 = mt * kTileM + row_offset, n0 = nt * BN + (PAIR ? rank * S::kBRows : 0u);
+			Unit now[kEach], next[kEach];
+			auto fetch = [&](Unit (&v)[kEach], uint32_t kb) {
+#pragma unroll
+				for (int j = 0; j < kEach; ++j) {
+					const int i = t + j * kGatherWarps * 32, r = i >> 3, c = (i & 7) * 8;
+					if (i >= kUnits) break;
+					if (r >= kBM) unit_fetch(v[j], p.b, p.b_ld, p.N, p.K, nt * BN + (r - kBM), kb * kBK + c);
+					else if (AMN) unit_fetch(v[j], p.a, p.a_ld, p.K, p.M, kb * kBK + (r & 63), mt * kBM + (r & 64) + c);
+					else unit_fetch(v[j], p.a, p.a_ld, p.M, p.K, mt * kBM + r, kb * kBK + c);
+				}
+			};
+			fetch(now, kb0);
 			for (uint32_t kb = kb0; kb < kb1; ++kb) {
-				if (GATHER || lane == 0) ok = wait_phase(empty + 8 * stage, phase ^ 1u);
+				ok = wait_phase(empty + 8 * stage, phase ^ 1u);
 				if (!ok) break;
-				unsigned char* sa = smem + stage * S::kStage;
-				unsigned char* sb = sa + S::kABytes;
-				if (GATHER) {
-					const int t = tid - S::kLoadWarp * 32;
-					if (AMN) {
-						for (int s = 0; s < 2; ++s) gather_box<64>(sa + s * 8192, p.a, p.a_ld, p.K, p.M, kb * kBK, m0 + s * 64, t);
-					} else {
-						gather_box<kBM>(sa, p.a, p.a_ld, p.M, p.K, m0, kb * kBK, t);
-					}
-					if (BMN) {
-						for (int s = 0; s < (BN + 63) / 64; ++s) gather_box<64>(sb + s * 8192, p.b, p.b_ld, p.K, p.N, kb * kBK, n0 + s * 64, t);
-					} else {
-						gather_box<BN>(sb, p.b, p.b_ld, p.N, p.K, n0, kb * kBK, t);
-					}
-					tc::fence_async_smem();
-					arrive(full + 8 * stage);
-				} else if (lane == 0) {
-					const uint32_t bar = full_lead + 8 * stage;
-					// slabs that lie outside of the matrix are not loaded: what the tile holds there reaches only sums that are not used
-					const int slabs_a = AMN ? (PAIR ? 2 : min(2, (int)((p.M - m0 + 63) / 64))) : 1;
-					const int slabs_b = BMN ? (PAIR ? S::kBRows / 64 : min((BN + 63) / 64, (int)((p.N - n0 + 63) / 64))) : 1;
-					const uint32_t bytes = (AMN ? slabs_a * 8192 : S::kABytes) + (BMN ? slabs_b * 8192 : S::kBBytes);
-					if (!PAIR) arrive_expect(full + 8 * stage, bytes);
-					else if (rank == 0) arrive_expect(full + 8 * stage, 2 * bytes);
-					if (AMN) {
-						for (int s = 0; s < slabs_a; ++s) tma_load<PAIR>(sptr(sa) + s * 8192, &p.ta, m0 + s * 64, kb * kBK, bar);
-					} else {
-						tma_load<PAIR>(sptr(sa), &p.ta, kb * kBK, m0, bar);
-					}
-					if (BMN) {
-						for (int s = 0; s < slabs_b; ++s) tma_load<PAIR>(sptr(sb) + s * 8192, &p.tb, n0 + s * 64, kb * kBK, bar);
-					} else {
-						tma_load<PAIR>(sptr(sb), &p.tb, kb * kBK, n0, bar);
-					}
+				if (kb + 1 < kb1) fetch(next, kb + 1);
+				unsigned char* const sa = smem + stage * S::kStage;  // A's 128 rows and B's behind them
+#pragma unroll
+				for (int j = 0; j < kEach; ++j) {
+					const int i = t + j * kGatherWarps * 32, r = i >> 3;
+					if (i < kUnits) *reinterpret_cast<uint4*>(sa + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = unit_value(now[j]);
+					now[j] = next[j];
+				}
+				tc::fence_async_smem();
+				arrive(full + 8 * stage);
+				if (++stage == S::kStages) stage = 0, phase ^= 1u;
+			}
+		}
+		__syncwarp();
+	} else if (warp >= S::kLoadWarp) {
+		// ---------------------------------------------------------------- operand tiles by TMA, one thread
+		uint32_t stage = 0, phase = 0;
+		const uint32_t full_lead = PAIR ? peer_address(full, 0) : full;  // a pair's tiles are counted in by the first CTA
+		for (uint32_t u = first; lane == 0 && u < units && ok; u += step) {
+			uint32_t mt, nt, split, kb0, kb1;
+			locate(u, mt, nt, split, kb0, kb1);
+			const uint32_t m0 = mt * kTileM + row_offset, n0 = nt * BN + (PAIR ? rank * S::kBRows : 0u);
+			// slabs that lie outside of the matrix are not loaded: what the tile holds there reaches only sums that are not used
+			const int slabs_a = AMN ? (PAIR ? 2 : min(2, (int)((p.M - m0 + 63) / 64))) : 1;
+			const int slabs_b = BMN ? (PAIR ? S::kBRows / 64 : min((BN + 63) / 64, (int)((p.N - n0 + 63) / 64))) : 1;
+			const uint32_t bytes = (AMN ? slabs_a * 8192 : S::kABytes) + (BMN ? slabs_b * 8192 : S::kBBytes);
+			for (uint32_t kb = kb0; kb < kb1; ++kb) {
+				ok = wait_phase(empty + 8 * stage, phase ^ 1u);
+				if (!ok) break;
+				const uint32_t sa = sptr(smem + stage * S::kStage), sb = sa + S::kABytes, bar = full_lead + 8 * stage;
+				if (!PAIR) arrive_expect(full + 8 * stage, bytes);
+				else if (rank == 0) arrive_expect(full + 8 * stage, 2 * bytes);
+				if (AMN) {
+					for (int s = 0; s < slabs_a; ++s) tma_load<PAIR>(sa + s * 8192, &p.ta, m0 + s * 64, kb * kBK, bar);
+				} else {
+					tma_load<PAIR>(sa, &p.ta, kb * kBK, m0, bar);
+				}
+				if (BMN) {
+					for (int s = 0; s < slabs_b; ++s) tma_load<PAIR>(sb + s * 8192, &p.tb, n0 + s * 64, kb * kBK, bar);
+				} else {
+					tma_load<PAIR>(sb, &p.tb, kb * kBK, n0, bar);
 				}
 				if (++stage == S::kStages) stage = 0, phase ^= 1u;
 			}
-			ok = __shfl_sync(~0u, (int)ok, 0) != 0;
 		}
+		__syncwarp();
 	} else if (warp == S::kMmaWarp) {
 		// ---------------------------------------------------------------- MMAs, one thread (of a pair's first CTA)
 		if (lane == 0 && (!PAIR || rank == 0)) {
@@ -611,7 +637,6 @@ static int product_of(const Product& p, cudaStream_t stream) {
 	a.e = p.e;
 	a.splits = a.cluster = 1;
 	const uint32_t kblocks = tiles_of(p.K, kBK);
-	const bool tma = tma_ok(p.a, p.a_ld) && tma_ok(p.b, p.b_ld);
 	// grid of one-CTA tiles; may_split: the kernel can join a cluster's parts
 	auto grid = [&](uint32_t bn, bool may_split) -> uint32_t {
 		a.tiles_m = tiles_of(a.M, kBM);
@@ -621,19 +646,21 @@ static int product_of(const Product& p, cudaStream_t stream) {
 		a.cluster = a.splits = may_split ? cluster_for(tiles, kblocks) : 1u;
 		return (uint32_t)(a.cluster > 1 ? tiles * a.cluster : tiles < (uint64_t)kSMs ? tiles : (uint64_t)kSMs);
 	};
-#define N2B_GO(BN, AMN, BMN_, SWAP)                                                                  \
+#define N2B_GO(BN, AMN, BMN_, SWAP, GATHER)                                                          \
 	do {                                                                                             \
 		const uint32_t ctas = grid(BN, BN <= 128);                                                   \
 		if (!ctas) return NEUS2B_E_TOO_LARGE;                                                        \
-		return tma ? launch<BN, AMN, BMN_, SWAP, false, false, false>(a, ctas, stream)               \
-		           : launch<BN, AMN, BMN_, SWAP, false, true, false>(a, ctas, stream);               \
+		return launch<BN, AMN, BMN_, SWAP, false, GATHER, false>(a, ctas, stream);                   \
 	} while (0)
 	if (p.M <= 64) {
 		// few samples: the weights are the 128-row operand, the samples its columns
 		a.a = (const uint16_t*)p.b, a.a_ld = p.b_ld, a.M = p.N;
 		a.b = (const uint16_t*)p.a, a.b_ld = p.a_ld, a.N = p.M;
-		if (p.M <= 32) N2B_GO(32, BMN, false, true);
-		N2B_GO(64, BMN, false, true);
+		const bool tma = tma_ok(p.a, p.a_ld) && tma_ok(p.b, p.b_ld);
+		if (p.M <= 32 && tma) N2B_GO(32, BMN, false, true, false);
+		if (p.M <= 32) N2B_GO(32, BMN, false, true, true);
+		if (tma) N2B_GO(64, BMN, false, true, false);
+		N2B_GO(64, BMN, false, true, true);
 	}
 	a.a = (const uint16_t*)p.a, a.a_ld = p.a_ld, a.M = p.M;
 	a.b = (const uint16_t*)p.b, a.b_ld = p.b_ld, a.N = p.N;
@@ -643,15 +670,15 @@ static int product_of(const Product& p, cudaStream_t stream) {
 	auto cost = [&](uint32_t bn) { return (rows * tiles_of(p.N, bn) + kSMs - 1) / kSMs * (bn + 64) * 20; };
 	const uint64_t pairs = (uint64_t)tiles_of(p.M, 2 * kBM) * tiles_of(p.N, 256), pair_cost = (pairs + kSMs / 2 - 1) / (kSMs / 2) * (256 + 64) * 17;
 	const uint64_t c64 = cost(64), c128 = cost(128), c256 = cost(256);
-	if (tma && pair_cost < c64 && pair_cost < c128 && pair_cost < c256) {
+	if (pair_cost < c64 && pair_cost < c128 && pair_cost < c256) {
 		a.tiles_m = tiles_of(a.M, 2 * kBM);
 		a.tiles_n = tiles_of(a.N, 256);
 		if (pairs >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
 		return launch<256, false, BMN, false, false, false, true>(a, 2 * (uint32_t)(pairs < kSMs / 2 ? pairs : kSMs / 2), stream);
 	}
-	if (c256 < c128 && c256 < c64) N2B_GO(256, false, BMN, false);
-	if (c128 < c64) N2B_GO(128, false, BMN, false);
-	N2B_GO(64, false, BMN, false);
+	if (c256 < c128 && c256 < c64) N2B_GO(256, false, BMN, false, false);
+	if (c128 < c64) N2B_GO(128, false, BMN, false, false);
+	N2B_GO(64, false, BMN, false, false);
 #undef N2B_GO
 }
 
@@ -662,7 +689,7 @@ struct WgradPlan {
 	bool pair;
 	uint32_t tiles_m, tiles_n, splits;
 };
-static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair) {
+static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair) {  // (a pair's kernel always stores the product)
 	const uint32_t kblocks = tiles_of(K, kBK);
 	uint64_t best = 0;
 	WgradPlan plan{};
@@ -741,16 +768,26 @@ int write_linear_error(uint32_t flags) {
 	return e == cudaSuccess ? write_narrow_error(flags) : (int)e;
 }
 
+bool operand_aligned(const void* p, uint64_t ld) { return tma_ok(p, ld); }
+int run_realign(const Operand* ops, int count, cudaStream_t stream) {
+	Realign r{};
+	for (int k = 0; k < 3; ++k) {
+		r.units[k + 1] = r.units[k];
+		if (k >= count) continue;
+		r.from[k] = (const uint16_t*)ops[k].from, r.from_ld[k] = ops[k].ld, r.to[k] = (uint16_t*)ops[k].to, r.rows[k] = ops[k].rows, r.cols[k] = ops[k].cols;
+		r.units[k + 1] += (uint64_t)ops[k].rows * ((ops[k].cols + 7) / 8);
+	}
+	const uint64_t blocks = (r.units[3] + 255) / 256;
+	return launch_behind(realign_kernel, (uint32_t)(blocks < 16ull * kSMs ? blocks : 16 * kSMs), 256, 0, stream, r);
+}
+
 int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product_of<true>(p, stream) : product_of<false>(p, stream); }
 
 uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {
-	// whether the operands can be read by TMA is not known here: the larger of the two plans, and of the sums alone
-	uint64_t most = plan_bytes(wgrad_plan(out_width, in_width, n, true), out_width, in_width);
-	for (uint32_t width : {in_width, sums_only_width(out_width)}) {
-		const uint64_t b = plan_bytes(wgrad_plan(out_width, width, n, false), out_width, width);
-		if (b > most) most = b;
-	}
-	return most;
+	// whether the product or the column sums alone are wanted is not known here
+	const uint32_t alone = sums_only_width(out_width);
+	const uint64_t product = plan_bytes(wgrad_plan(out_width, in_width, n, true), out_width, in_width), sums = plan_bytes(wgrad_plan(out_width, alone, n, false), out_width, alone);
+	return product > sums ? product : sums;
 }
 
 int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
@@ -761,8 +798,7 @@ int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, floa
 }
 
 int run_weight_gradient(const Product& p, cudaStream_t stream) {
-	const bool tma = tma_ok(p.a, p.a_ld) && tma_ok(p.b, p.b_ld);
-	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, tma && p.e.out);
+	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, p.e.out != nullptr);
 	if (p.workspace_bytes < plan_bytes(w, p.M, p.N)) return NEUS2B_E_INVALID;
 	Args a{};
 	a.bf16 = p.bf16;
@@ -790,8 +826,7 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 	a.column_sums = p.column_sums;
 	a.want_sums = p.column_sums != nullptr;
 	const uint32_t ctas = (uint32_t)(units < (uint64_t)kSMs ? units : kSMs);
-	if (int rc = tma ? launch<128, true, true, false, true, false, false>(a, ctas, stream) : launch<128, true, true, false, true, true, false>(a, ctas, stream))
-		return rc;
+	if (int rc = launch<128, true, true, false, true, false, false>(a, ctas, stream)) return rc;
 	return w.splits > 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate, stream) : NEUS2B_OK;
 }
 

@@ -311,17 +311,21 @@ def _weights(w, dtype, device):
     return w.shape
 
 
-def _workspace(query, desc, given, device):
+def _workspace(need, given, device):
     """(tensor that keeps it alive, address, bytes)"""
-    need = C.c_uint64(0)
-    L.check(query(C.byref(desc), C.byref(need)))
-    if not need.value:
+    if not need:
         return None, None, 0
     if given is None:
-        given = torch.empty(need.value, dtype=torch.uint8, device=device)
-    elif given.device != device or not given.is_contiguous() or given.numel() * given.element_size() < need.value:
-        _refuse(f"the workspace has to be {need.value} contiguous bytes on {device}")
+        given = torch.empty(need, dtype=torch.uint8, device=device)
+    elif given.device != device or not given.is_contiguous() or given.numel() * given.element_size() < need:
+        _refuse(f"the workspace has to be {need} contiguous bytes on {device}")
     return given, given.data_ptr(), given.numel() * given.element_size()
+
+
+def _bytes(query, desc, *flags):
+    need = C.c_uint64(0)
+    L.check(query(C.byref(desc), *flags, C.byref(need)))
+    return need.value
 
 
 def _gradient(t, name, shape, mode, device):
@@ -335,7 +339,7 @@ def _gradient(t, name, shape, mode, device):
     return t
 
 
-def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_preact=False, out=None):
+def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_preact=False, out=None, workspace=None):
     """act(x w^T + bias) + residual for fp16 or bf16 tensors: x [n][in], w [out][in], bias [out], residual [n][out].  Rows may be apart
     (views of wider matrices).  want_preact: returns (y, z) with z = x w^T + bias, which linear_backward reads.  `out` may be
     `residual`."""
@@ -352,8 +356,12 @@ def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_p
     yp, ys = _rows(out, "out", n, n_out, t, dev)
     z = torch.empty((n, n_out), dtype=t, device=dev) if want_preact else None
     d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
-    L.check(L.lib().neus2b_linear_forward(C.byref(d), xp, xs, w.data_ptr(), bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out,
-                                          L.cur_stream()))
+    lib, wp = L.lib(), w.data_ptr()
+    keep, wsp, wsb = None, None, 0
+    if (xp | wp | xs * 2 | n_in * 2) & 15:
+        keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_forward_workspace, d, 1), workspace, dev)
+    L.check(lib.neus2b_linear_forward(C.byref(d), xp, xs, wp, bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out, wsp, wsb,
+                                      L.cur_stream()))
     return (out, z) if want_preact else out
 
 
@@ -383,7 +391,8 @@ def linear_backward(x, w, dL_dout, activation=L.ACT_NONE, preact=None, below_act
     bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, dev) if params and want_bias else None
     d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
     lib = L.lib()
-    keep, wsp, wsb = _workspace(lib.neus2b_linear_backward_workspace, d, workspace, dev)
+    unaligned = 1 if (xp | w.data_ptr() | dyp | xs * 2 | n_in * 2 | dys * 2) & 15 else 0
+    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_backward_workspace, d, unaligned), workspace, dev)
     L.check(lib.neus2b_linear_backward(C.byref(d), xp, xs, w.data_ptr(), zp, zs, dyp, dys, below_activation, bzp, bzs, sp, ss,
                                        din.data_ptr() if want_din else None, n_in, wgrad.data_ptr() if params else None,
                                        bgrad.data_ptr() if bgrad is not None else None, mode, wsp, wsb, L.cur_stream()))
@@ -433,7 +442,7 @@ def layer_norm_backward(x, gamma, mean, rstd, dL_dout, skip=None, dgamma=None, d
     dgamma = _gradient(dgamma, "dgamma", (width,), mode, dev) if params else None
     dbeta = _gradient(dbeta, "dbeta", (width,), mode, dev) if params else None
     lib = L.lib()
-    keep, wsp, wsb = _workspace(lib.neus2b_layer_norm_backward_workspace, d, workspace, dev)
+    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_layer_norm_backward_workspace, d) if params else 0, workspace, dev)
     L.check(lib.neus2b_layer_norm_backward(C.byref(d), xp, xs, gp, mp, rp, dyp, dys, sp, ss, din.data_ptr() if want_din else None, width,
                                            dgamma.data_ptr() if params else None, dbeta.data_ptr() if params else None, mode, wsp, wsb,
                                            L.cur_stream()))

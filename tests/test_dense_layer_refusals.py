@@ -19,18 +19,25 @@ INVALID, UNSUPPORTED = -1, -2
 
 def test_linear_forward(lib):
     L, f = lib
-    ok = dict(n=4, in_width=32, out_width=16, dtype=L.F16, activation=0, x=FAKE, xs=32, w=FAKE, b=None, r=None, rs=0, y=FAKE, ys=16, z=None, zs=0)
+    ok = dict(n=4, in_width=32, out_width=16, dtype=L.F16, activation=0, x=FAKE, xs=32, w=FAKE, b=None, r=None, rs=0, y=FAKE, ys=16, z=None, zs=0, ws=None, wsb=0)
 
     def call(**kw):
         a = dict(ok, **kw)
         d = L.LinearDesc(a["n"], a["in_width"], a["out_width"], a["dtype"], a["activation"])
-        return f.neus2b_linear_forward(C.byref(d), a["x"], a["xs"], a["w"], a["b"], a["r"], a["rs"], a["y"], a["ys"], a["z"], a["zs"], None)
-    assert f.neus2b_linear_forward(None, FAKE, 32, FAKE, None, None, 0, FAKE, 16, None, 0, None) == INVALID
+        return f.neus2b_linear_forward(C.byref(d), a["x"], a["xs"], a["w"], a["b"], a["r"], a["rs"], a["y"], a["ys"], a["z"], a["zs"], a["ws"], a["wsb"], None)
+    assert f.neus2b_linear_forward(None, FAKE, 32, FAKE, None, None, 0, FAKE, 16, None, 0, None, 0, None) == INVALID
     assert call(dtype=L.F32) == UNSUPPORTED and call(dtype=7) == UNSUPPORTED
     for bad in (dict(activation=4), dict(in_width=0), dict(out_width=0), dict(x=None), dict(w=None), dict(y=None), dict(xs=31), dict(ys=15), dict(r=FAKE, rs=15),
                 dict(z=FAKE, zs=3), dict(x=FAKE + 1), dict(w=FAKE + 1), dict(b=FAKE + 1), dict(y=FAKE + 1), dict(r=FAKE + 1, rs=16)):
         assert call(**bad) == INVALID, bad
     assert call(n=0, x=None, y=None) == 0
+    need = C.c_uint64(7)
+    d = L.LinearDesc(500, 33, 16, L.F16, 0)
+    assert f.neus2b_linear_forward_workspace(C.byref(d), 0, C.byref(need)) == 0 and need.value == 0
+    assert f.neus2b_linear_forward_workspace(C.byref(d), 1, C.byref(need)) == 0 and need.value >= (500 + 16) * 40 * 2
+    assert f.neus2b_linear_forward_workspace(C.byref(d), 1, None) == INVALID
+    for bad in (dict(), dict(ws=FAKE), dict(ws=FAKE, wsb=need.value - 1), dict(ws=FAKE + 8, wsb=need.value)):  # copies of x and W need room
+        assert call(n=500, in_width=33, xs=33, **bad) == INVALID, bad
 
 
 def test_linear_backward(lib):
@@ -43,7 +50,7 @@ def test_linear_backward(lib):
         d = L.LinearDesc(a["n"], 32, 16, a["dtype"], a["activation"])
         if a["ws"] is None and "wsb" not in kw:
             need = C.c_uint64(0)
-            if f.neus2b_linear_backward_workspace(C.byref(d), C.byref(need)) == 0:
+            if f.neus2b_linear_backward_workspace(C.byref(d), 0, C.byref(need)) == 0:
                 a["ws"], a["wsb"] = FAKE, need.value
         return f.neus2b_linear_backward(C.byref(d), a["x"], a["xs"], a["w"], a["z"], a["zs"], a["dy"], a["dys"], a["below"], a["bz"], a["bzs"], a["skip"],
                                         a["ss"], a["dx"], a["dxs"], a["dw"], a["db"], a["mode"], a["ws"], a["wsb"], None)
@@ -53,7 +60,8 @@ def test_linear_backward(lib):
                 dict(activation=2, z=FAKE, zs=15), dict(activation=2, z=FAKE, zs=16, ws=FAKE, wsb=4), dict(activation=2, z=FAKE, zs=16, ws=FAKE + 8, wsb=1 << 30)):
         assert call(**bad) == INVALID, bad
     d = L.LinearDesc(4, 32, 16, L.BF16, 0)
-    assert f.neus2b_linear_backward_workspace(C.byref(d), None) == INVALID
+    assert f.neus2b_linear_backward_workspace(C.byref(d), 0, None) == INVALID
+    assert call(dy=FAKE + 2) == INVALID and call(x=FAKE + 2) == INVALID  # the workspace has no room for their copies
 
 
 def test_layer_norm(lib):

@@ -123,7 +123,7 @@ def test_bias_gradient_alone_and_frozen_inputs(ops, n):
         only = ops.linear_backward(x, w, dy, want_din=False, want_bias=False)
         assert only[0] is None and only[2] is None and torch.equal(only[1], dw)
         d, need = L.LinearDesc(n, i, o, L.BF16, 0), C.c_uint64(0)
-        L.check(L.lib().neus2b_linear_backward_workspace(C.byref(d), C.byref(need)))
+        L.check(L.lib().neus2b_linear_backward_workspace(C.byref(d), 1, C.byref(need)))
         ws, out = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda"), torch.full((o,), 7.0, device="cuda")
         L.check(L.lib().neus2b_linear_backward(C.byref(d), None, 0, None, None, 0, dy.data_ptr(), o, 0, None, 0, None, 0, None, 0, None, out.data_ptr(),
                                                L.GRAD_ACCUMULATE, ws.data_ptr(), need.value, L.cur_stream()))
