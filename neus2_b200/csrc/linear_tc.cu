@@ -25,6 +25,7 @@ struct alignas(64) Args {
 	uint32_t bf16;
 	float *partial, *column_sums;  // splits > 1: [splits][M][N] and [splits][M]
 	uint32_t want_sums;
+	uint32_t stages, chunks;
 	Epilogue e;
 };
 
@@ -105,11 +106,12 @@ struct Shape {
 	static constexpr int kHalves = kTurns || GATHER ? 1 : kMany ? 4 : 2, kGroups = kTurns ? 4 : 1, kBufs = kTurns ? 4 : 2;
 	static constexpr int kEpiWarps = 4 * kHalves * kGroups, kMmaWarp = kEpiWarps, kLoadWarp = kEpiWarps + 1;
 	static constexpr int kThreads = (GATHER ? kLoadWarp + kGatherWarps : kLoadWarp + 1) * 32;
-	static constexpr int kBounce = SWAP || WGRAD ? 0 : kEpiWarps * 3 * kChunkBytes;  // a result, a slope and an addend chunk for every epilogue warp
-	static constexpr int kFixed = kBounce + 2048 + 1024;                         // ones tile and barriers; alignment of the base
-	static constexpr int kRoom = (kSmemMost - kFixed) / kStage;
-	static constexpr int kStages = kRoom < kMaxStages ? kRoom : kMaxStages;
-	static constexpr int kSmem = kStages * kStage + kFixed;
+	// Shared memory behind the operand stages: chunks of the epilogue (`chunks` for every warp), ones tile and barriers; alignment of the base.
+	static constexpr int fixed(int chunks) { return (SWAP || WGRAD ? 0 : kEpiWarps * chunks * kChunkBytes) + 2048 + 1024; }
+	static constexpr int stages(int chunks) {
+		const int room = (kSmemMost - fixed(chunks)) / kStage;
+		return room < kMaxStages ? room : kMaxStages;
+	}
 	static constexpr int kCols = kBufs * BN + (WGRAD && !PAIR ? 32 : 0);
 	static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
@@ -175,8 +177,9 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
 	extern __shared__ unsigned char smem_raw[];
 	unsigned char* smem = smem_raw + ((1024u - (sptr(smem_raw) & 1023u)) & 1023u);
-	unsigned char* bounces = smem + S::kStages * S::kStage;
-	unsigned char* ones = bounces + S::kBounce;  // 512 bytes: a [16][16] tile of 1.0
+	const uint32_t stages = p.stages;
+	unsigned char* ones = smem + stages * S::kStage;  // 512 bytes: a [16][16] tile of 1.0
+	unsigned char* chunks = ones + 2048;              // p.chunks for every epilogue warp
 	uint64_t* bars = reinterpret_cast<uint64_t*>(ones + 1024);
 	uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(ones + 2048 - 16);
 	const uint32_t full = sptr(bars), empty = full + 8 * kMaxStages, tfull = empty + 8 * kMaxStages, tempty = tfull + 8 * 4;
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	let_next_start();
 
 	if (tid == 0) {
-		for (int i = 0; i < S::kStages; ++i) {
+		for (uint32_t i = 0; i < stages; ++i) {
 			tc::mbar_init(full + 8 * i, GATHER ? kGatherWarps * 32 : 1);
 			tc::mbar_init(empty + 8 * i, 1);
 		}
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 				}
 				tc::fence_async_smem();
 				arrive(full + 8 * stage);
-				if (++stage == S::kStages) stage = 0, phase ^= 1u;
+				if (++stage == stages) stage = 0, phase ^= 1u;
 			}
 		}
 		__syncwarp();
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 				} else {
 					tma_load<PAIR>(sb, &p.tb, kb * kBK, n0, bar);
 				}
-				if (++stage == S::kStages) stage = 0, phase ^= 1u;
+				if (++stage == stages) stage = 0, phase ^= 1u;
 			}
 		}
 		__syncwarp();
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 								tc::mma_f16(tmem + S::kBufs * BN + buf * 16, da + k * kStepA, tc::smem_desc(sptr(ones), 128, 256), id_ones, kb > c0 || k > 0);
 						}
 						commit<PAIR>(empty + 8 * stage);
-						if (++stage == S::kStages) stage = 0, phase ^= 1u;
+						if (++stage == stages) stage = 0, phase ^= 1u;
 					}
 					if (!ok) break;
 					commit<PAIR>(tfull + 8 * buf);
@@ -349,9 +352,10 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 		const uint32_t q = warp & 3, half = (warp >> 2) % S::kHalves, group = (warp >> 2) / S::kHalves;
 		const uint32_t lanes = tmem + ((q * 32u) << 16);
 		constexpr int kCols = BN / S::kHalves;  // columns half * kCols .. of the tile
-		unsigned char* const result = bounces + warp * 3 * kChunkBytes;
-		unsigned char* const slope = result + kChunkBytes;
-		unsigned char* const addend = slope + kChunkBytes;
+		// the result of 32 columns goes out through the place that its last input came in by
+		unsigned char* const slope = chunks + warp * p.chunks * kChunkBytes;
+		unsigned char* const addend = slope + (p.chunks - 1) * kChunkBytes;
+		unsigned char* const result = addend;
 		uint32_t turn = 0, buf = 0, buf_phase = 0;
 		auto next_buf = [&] {
 			if (++buf == S::kBufs) buf = 0, buf_phase ^= 1u;
@@ -502,7 +506,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 					if (e.preact) {
 #pragma unroll
 						for (int i = 0; i < 16; ++i) other[i] = pack2(v[2 * i], v[2 * i + 1], bf);
-						chunk_store(other, e.preact, e.preact_ld, row0, p.M, col, p.N, result, e.vec, lane);
+						chunk_store(other, e.preact, e.preact_ld, row0, p.M, col, p.N, slope, e.vec, lane);
 					}
 					if (inputs) {
 						asm volatile("cp.async.wait_all;" ::: "memory");
@@ -529,14 +533,15 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 							v[2 * i + 1] += f.y;
 						}
 					}
-					if (inputs) {
-						__syncwarp();
-						if (c + 32 < kCols) fetch(col + 32);
-					}
 #pragma unroll
 					for (int i = 0; i < 16; ++i) other[i] = pack2(v[2 * i], v[2 * i + 1], bf);
 					chunk_store(other, e.out, e.out_ld, row0, p.M, col, p.N, result, e.vec, lane);
+					if (inputs && c + 32 < kCols) {
+						__syncwarp();
+						fetch(col + 32);
+					}
 				}
+				if (inputs) __syncwarp();  // before the next tile's inputs come in
 				next_buf();
 			}
 		}
@@ -602,11 +607,15 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 		if (int rc = AMN ? make_map(&a.ta, a.a, a.a_ld, a.K, a.M, 64, a.bf16) : make_map(&a.ta, a.a, a.a_ld, a.M, a.K, kBM, a.bf16)) return rc;
 		if (int rc = BMN ? make_map(&a.tb, a.b, a.b_ld, a.K, a.N, 64, a.bf16) : make_map(&a.tb, a.b, a.b_ld, a.N, a.K, S::kBRows, a.bf16)) return rc;
 	}
-	N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+	// one chunk for every epilogue input, and one for z where it does not go the same way as the result
+	a.chunks = (a.e.slope_z && a.e.add) || (a.e.preact && a.e.add) ? 2 : 1;
+	a.stages = S::stages((int)a.chunks);
+	const int smem = (int)a.stages * S::kStage + S::fixed((int)a.chunks);
+	N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
 	cudaLaunchConfig_t cfg{};
 	cfg.gridDim = dim3(ctas);
 	cfg.blockDim = dim3(S::kThreads);
-	cfg.dynamicSmemBytes = S::kSmem;
+	cfg.dynamicSmemBytes = smem;
 	cfg.stream = stream;
 	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
