@@ -23,23 +23,23 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 
 constexpr float kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;  // sqrt(2 / pi); the cubic term of the tanh form
 
-// The logistic function of t ln 2, from the hardware's 2^x and 1/x (2 and 1 units of the last place off): results are rounded to 16 bits.
-// 2^(-t) overflows to infinity on the far negative side, where the reciprocal is 0.
+// The logistic function of -t ln 2, from the hardware's 2^x and 1/x (2 and 1 units of the last place off): results are rounded to 16
+// bits.  2^t overflows to infinity on the far side, where the reciprocal is 0.
 __device__ __forceinline__ float logistic2(float t) {
 	float e, r;
-	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-t));
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
 	asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
 	return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
-// 2u log2(e), u = sqrt(2 / pi) (z + 0.044715 z^3)
+// -2u log2(e), u = sqrt(2 / pi) (z + 0.044715 z^3)
 __device__ __forceinline__ float gelu_argument(float z) {
-	return z * fmaf(2.f * kGeluC * kGeluA * kLog2e, z * z, 2.f * kGeluC * kLog2e);
+	return z * fmaf(-2.f * kGeluC * kGeluA * kLog2e, z * z, -2.f * kGeluC * kLog2e);
 }
 __device__ __forceinline__ float act_value(int act, float z) {
 	if (act == NEUS2B_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
 	if (act == NEUS2B_ACT_GELU) return z * logistic2(gelu_argument(z));
-	if (act == NEUS2B_ACT_SILU) return z * logistic2(kLog2e * z);
+	if (act == NEUS2B_ACT_SILU) return z * logistic2(-kLog2e * z);
 	return z;
 }
 // d act / dz.  gelu: s + z s (1 - s) 2u' with 2u' = 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2); where z^2 is held at 1e30, s (1 - s) is 0.
@@ -50,7 +50,7 @@ __device__ __forceinline__ float act_slope(int act, float z) {
 		return fmaf(z * fmaf(-s, s, s), fmaf(6.f * kGeluC * kGeluA, z2, 2.f * kGeluC), s);
 	}
 	if (act == NEUS2B_ACT_SILU) {
-		const float s = logistic2(kLog2e * z);
+		const float s = logistic2(-kLog2e * z);
 		return fmaf(z, fmaf(-s, s, s), s);
 	}
 	return 1.f;
