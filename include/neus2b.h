@@ -337,6 +337,8 @@ typedef struct {
 	 * treated as absent -- that parameter keeps its weight and moments this step, the gradient slot is cleared -- and the
 	 * number of such entries is added here, so that one bad value cannot reach the fp32 master weights unnoticed */
 	uint32_t* d_nonfinite;
+	/* optional device value that every gradient is multiplied by: the factor of neus2b_grad_norm (d_result + 1).  NULL: 1 */
+	const float* d_grad_scale;
 } neus2b_adam_cfg;
 /* Ema o ExponentialDecay o Adam (configs/nerf/dtu.json:5-27) over the flat parameter block.  Gradients: d_grad_mlp fp32
  * for [0, n_matrix), d_grad_grid fp16 for [n_matrix, n - 4), d_grad_variance fp32 for the last 4; all are zeroed after
@@ -500,6 +502,10 @@ typedef struct {
 	 * compacted batch and loss).  Cumulative window ends; n_forward_windows = 0 evaluates every sample like the reference. */
 	uint32_t n_forward_windows;
 	uint32_t forward_window_ends[6];
+	/* no counterpart in the reference: the canonical model's gradients (MLPs, grid, variance together, without the loss scale; after
+	 * the exchange in data-parallel training) are scaled so that their global norm is at most this; 0 = off.  Entries that are not
+	 * finite do not count (the optimizer does not use them either).  > 0 or 0. */
+	float max_grad_norm;
 } neus2b_testbed_config;
 /* "top_resolution" -> per_level_scale when the config gives none (src/testbed.cu:2173-2177):
  * exp(log(top_resolution * aabb_scale / base_resolution) / (n_levels - 1)). */
@@ -519,6 +525,8 @@ typedef struct {
 	uint32_t device_error;                         /* sticky device error bits at the end of the step (neus2b_device_error_flags) */
 	uint32_t n_samples_evaluated;                  /* samples the step's network pass evaluated (== ..._before_compaction without
 	                                                  forward windows) */
+	float grad_norm;                               /* global norm of the step's gradients before clipping; 0 when max_grad_norm is 0 or
+	                                                  the canonical model is frozen */
 } neus2b_train_stats;
 
 typedef struct neus2b_testbed neus2b_testbed;

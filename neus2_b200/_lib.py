@@ -72,7 +72,7 @@ class RenderRequest(C.Structure):
 class AdamCfg(C.Structure):
     _fields_ = [("learning_rate", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("epsilon", C.c_float),
                 ("l2_reg", C.c_float), ("ema_decay", C.c_float), ("loss_scale", C.c_float), ("step", C.c_uint32),
-                ("n_matrix", C.c_uint32), ("flags", C.c_uint32), ("d_nonfinite", C.c_void_p)]
+                ("n_matrix", C.c_uint32), ("flags", C.c_uint32), ("d_nonfinite", C.c_void_p), ("d_grad_scale", C.c_void_p)]
 
 
 class LinearDesc(C.Structure):
@@ -111,7 +111,7 @@ class TestbedConfig(C.Structure):
                 ("after_learning_rate", C.c_float), ("gm_learning_rate", C.c_float), ("gm_beta1", C.c_float), ("gm_beta2", C.c_float),
                 ("gm_epsilon", C.c_float), ("gm_l2_reg", C.c_float), ("gm_ema_decay", C.c_float), ("gm_lr_decay_start", C.c_uint32),
                 ("gm_lr_decay_interval", C.c_uint32), ("gm_lr_decay_base", C.c_float), ("first_frame_offset", C.c_float * 3),
-                ("n_forward_windows", C.c_uint32), ("forward_window_ends", C.c_uint32 * 6)]
+                ("n_forward_windows", C.c_uint32), ("forward_window_ends", C.c_uint32 * 6), ("max_grad_norm", C.c_float)]
 
 
 class TrainingState(C.Structure):
@@ -124,7 +124,7 @@ class TrainStats(C.Structure):
     _fields_ = [("training_step", C.c_uint32), ("rays_per_batch", C.c_uint32), ("n_rays_kept", C.c_uint32),
                 ("measured_batch_size_before_compaction", C.c_uint32), ("measured_batch_size", C.c_uint32),
                 ("overflow", C.c_uint32), ("loss", C.c_float), ("ek_loss", C.c_float), ("nonfinite_gradients", C.c_uint32),
-                ("device_error", C.c_uint32), ("n_samples_evaluated", C.c_uint32)]
+                ("device_error", C.c_uint32), ("n_samples_evaluated", C.c_uint32), ("grad_norm", C.c_float)]
 
 
 class Neus2bError(RuntimeError):

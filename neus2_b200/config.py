@@ -88,6 +88,10 @@ def testbed_config_from_json(cfg, aabb_scale=1, base=None):
     out.anneal_end = int(hp.get("anneal_end", 0))
     if "batch_size" in hp:
         out.batch_size = int(hp["batch_size"])
+    if "max_grad_norm" in hp:  # not a key of the reference: clipping of the gradients by their global norm
+        out.max_grad_norm = float(hp["max_grad_norm"])
+        if not 0.0 <= out.max_grad_norm < float("inf"):
+            raise ValueError("hyperparams.max_grad_norm has to be 0 (off) or a positive number")
     # dynamic sequences (src/testbed.cu:2108-2122; the frame counts are the caller's loop: dynamic_schedule below)
     out.predict_global_movement = int(bool(hp.get("predict_global_movement", False)))
     out.predict_global_movement_training_step = int(hp.get("predict_global_movement_training_step", 300)) if out.predict_global_movement else 0

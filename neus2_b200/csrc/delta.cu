@@ -118,6 +118,7 @@ __global__ void delta_optimizer_kernel(neus2b_adam_cfg c, float lr_t, float ema_
 			if (c.d_nonfinite) atomicAdd(c.d_nonfinite, 1u);
 			continue;
 		}
+		if (c.d_grad_scale) gk *= *c.d_grad_scale;
 		gk /= c.loss_scale;
 		float w = master[k];
 		if (gk != 0.f || (c.flags & NEUS2B_ADAM_UPDATE_UNTOUCHED)) {  // the unused slots never move

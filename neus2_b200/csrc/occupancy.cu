@@ -116,13 +116,13 @@ __global__ void occ_maxpool_kernel(uint32_t n, const uint8_t* __restrict__ prev,
 // ------------------------------------------------------------------------------------------------ Adam
 // One element of the Ema o Adam update.  Returns the new weight; m/v are updated in place.
 // A gradient that is NaN or infinite counts as absent (bad = true): the parameter keeps its weight and moments.
-__device__ __forceinline__ float adam_element(const neus2b_adam_cfg& c, float lr_t, bool matrix, float g, float w, float& m, float& v,
+__device__ __forceinline__ float adam_element(const neus2b_adam_cfg& c, float lr_t, bool matrix, float g, float scale, float w, float& m, float& v,
                                               bool& bad) {
 	if (!(fabsf(g) <= 3.402823466e+38f)) {
 		bad = true;
 		return w;
 	}
-	g = __fdividef(g, c.loss_scale);
+	g = __fdividef(g * scale, c.loss_scale);  // (a scale of 1 changes no bit)
 	bool upd = true;
 	if (matrix) g += c.l2_reg * w;
 	else {
@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(256, 8) adam_kernel(neus2b_adam_cfg c, float l
                                                       float* __restrict__ ema_master) {
 	const uint64_t stride = (uint64_t)gridDim.x * blockDim.x * 4u;
 	const uint64_t n_grid_end = n - 4u;
+	const float scale = c.d_grad_scale ? *c.d_grad_scale : 1.0f;
 	for (uint64_t i0 = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4u; i0 < n; i0 += stride) {
 		const bool matrix = i0 < c.n_matrix;
 		const bool var = i0 >= n_grid_end;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(256, 8) adam_kernel(neus2b_adam_cfg c, float l
 		}
 		bool bad = false;
 #pragma unroll
-		for (int e = 0; e < 4; ++e) w[e] = adam_element(c, lr_t, matrix, g[e], w[e], mm[e], vv[e], bad);
+		for (int e = 0; e < 4; ++e) w[e] = adam_element(c, lr_t, matrix, g[e], scale, w[e], mm[e], vv[e], bad);
 		if (bad && c.d_nonfinite) {
 			uint32_t nb = 0;
 #pragma unroll
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(256, 8) adam_packed_kernel(neus2b_adam_cfg c, 
                                                              __half* __restrict__ params, __half* __restrict__ params_ema) {
 	const uint64_t stride = (uint64_t)gridDim.x * blockDim.x * 2u;
 	const uint64_t n_grid_end = n - 4u;
+	const float scale = c.d_grad_scale ? *c.d_grad_scale : 1.0f;
 	for (uint64_t i0 = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) * 2u; i0 < n; i0 += stride) {
 		const bool matrix = i0 < c.n_matrix;
 		float g[2];
@@ -227,8 +229,8 @@ __global__ void __launch_bounds__(256, 8) adam_packed_kernel(neus2b_adam_cfg c, 
 		}
 		float4 s0 = state[i0], s1 = state[i0 + 1];
 		bool bad = false;
-		s0.x = adam_element(c, lr_t, matrix, g[0], s0.x, s0.y, s0.z, bad);
-		s1.x = adam_element(c, lr_t, matrix, g[1], s1.x, s1.y, s1.z, bad);
+		s0.x = adam_element(c, lr_t, matrix, g[0], scale, s0.x, s0.y, s0.z, bad);
+		s1.x = adam_element(c, lr_t, matrix, g[1], scale, s1.x, s1.y, s1.z, bad);
 		if (bad && c.d_nonfinite) atomicAdd(c.d_nonfinite, (uint32_t)!(fabsf(g[0]) <= 3.402823466e+38f) + (uint32_t)!(fabsf(g[1]) <= 3.402823466e+38f));
 		s0.w = ((1.0f - c.ema_decay) * s0.x + c.ema_decay * s0.w * ema_old) * ema_new_inv;
 		s1.w = ((1.0f - c.ema_decay) * s1.x + c.ema_decay * s1.w * ema_old) * ema_new_inv;

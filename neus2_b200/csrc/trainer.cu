@@ -17,6 +17,7 @@ struct TrainState {  // device resident, one per testbed
 	float loss, ek_loss;
 	uint32_t nonfinite;     // gradient entries the optimizer pass refused (cumulative; adam_kernel adds to it)
 	uint32_t device_error;  // copy of the sticky device error word, taken by the batch tuner
+	float grad_norm[2];     // max_grad_norm > 0: global norm of the step's gradients, and the factor that clips them
 	uint32_t evaluated;     // samples the network pass evaluated (counter 5; 0 = the full pass, which does not count)
 };
 
@@ -139,6 +140,10 @@ struct neus2b_testbed {
 	float *coords_compacted = nullptr, *loss = nullptr, *ek_loss = nullptr;
 	TrainState* state = nullptr;
 	TrainState* h_state = nullptr;  // pinned
+	// clipping: the table of the gradient buffers' pieces and the sums' workspace (max_grad_norm > 0 only)
+	uint64_t *grad_table = nullptr, *norm_workspace = nullptr;
+	uint64_t norm_workspace_bytes = 0;
+	uint32_t grad_pieces = 0;
 	const uint32_t* d_device_error = nullptr;  // the kernels' sticky error word on this device
 	// dataset
 	neus2b_dataset ds{};
@@ -291,13 +296,30 @@ static int reset_delta(neus2b_testbed* tb) {
 	return write_delta(tb, ident);
 }
 
+// The table of the gradient buffers (fp32 MLPs and variance, fp16 grid) for the norm, once: the buffers stay where they are.
+static int prepare_clipping(neus2b_testbed* tb) {
+	const neus2b_grad_tensor t[2] = {{tb->grad_mlp, nullptr, (uint64_t)NEUS2B_MLP_N + 4, NEUS2B_F32}, {tb->grad_grid, nullptr, tb->n_grid, NEUS2B_F16}};
+	uint64_t bytes = 0;
+	if (int rc = neus2b_grad_table(t, 2, nullptr, &bytes, &tb->grad_pieces)) return rc;
+	uint64_t* host = new (std::nothrow) uint64_t[bytes / 8];
+	if (!host) return NEUS2B_E_TOO_LARGE;
+	int rc = neus2b_grad_table(t, 2, host, &bytes, &tb->grad_pieces);
+	tb->norm_workspace_bytes = neus2b_grad_norm_workspace(tb->grad_pieces);
+	if (!rc) rc = dev_alloc(tb, &tb->grad_table, bytes / 8);
+	if (!rc) rc = dev_alloc(tb, &tb->norm_workspace, (tb->norm_workspace_bytes + 7) / 8);
+	if (!rc) rc = (int)cudaMemcpyAsync(tb->grad_table, host, bytes, cudaMemcpyHostToDevice, tb->stream);  // behind the allocation's clearing
+	if (!rc) rc = (int)cudaStreamSynchronize(tb->stream);
+	delete[] host;
+	return rc;
+}
+
 extern "C" int neus2b_testbed_create(const neus2b_testbed_config* cfg, neus2b_testbed** out) {
 	if (!cfg || !out) return NEUS2B_E_INVALID;
 	GridLevels lv;
 	int rc = make_levels(&cfg->grid, &lv);
 	if (rc) return rc;
 	if (cfg->batch_size == 0 || cfg->batch_size % 128u || cfg->n_cascades == 0 || cfg->n_cascades > NEUS2B_CASCADES ||
-	    cfg->world_size == 0 || cfg->rank >= cfg->world_size || !(cfg->loss_scale > 0.f))
+	    cfg->world_size == 0 || cfg->rank >= cfg->world_size || !(cfg->loss_scale > 0.f) || !(cfg->max_grad_norm >= 0.f) || !isfinite(cfg->max_grad_norm))
 		return NEUS2B_E_INVALID;
 	int ndev = 0;
 	if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0) return NEUS2B_E_NO_DEVICE;
@@ -339,6 +361,13 @@ extern "C" int neus2b_testbed_create(const neus2b_testbed_config* cfg, neus2b_te
 	TB_ALLOC(tb->adam_v, tb->n_params);
 	TB_ALLOC(tb->grad_mlp, (size_t)NEUS2B_MLP_N + 4);  // the variance gradient sits right behind: one fp32 exchange for both
 	tb->grad_var = tb->grad_mlp + NEUS2B_MLP_N;
+	if (cfg->max_grad_norm > 0.f) {
+		rc = prepare_clipping(tb);
+		if (rc) {
+			neus2b_testbed_destroy(tb);
+			return rc;
+		}
+	}
 	const size_t cells = (size_t)NEUS2B_GRIDSIZE * NEUS2B_GRIDSIZE * NEUS2B_GRIDSIZE;
 	const size_t n_occ = cells * cfg->n_cascades;
 	TB_ALLOC(tb->density_grid, n_occ);
@@ -795,6 +824,12 @@ static int optimizer_enqueue(neus2b_testbed* tb, bool want_stats) {
 	ac.flags = c.adam_flags;
 	ac.d_nonfinite = &tb->state->nonfinite;
 	int rc = NEUS2B_OK;
+	if (tb->train_canonical && c.max_grad_norm > 0.f) {
+		rc = neus2b_grad_norm(tb->grad_table, tb->grad_pieces, 1.f / c.loss_scale, c.max_grad_norm, NEUS2B_NORM_SKIP_NONFINITE, tb->state->grad_norm, nullptr,
+		                      tb->norm_workspace, tb->norm_workspace_bytes, tb->stream);
+		if (rc) return rc;
+		ac.d_grad_scale = tb->state->grad_norm + 1;
+	}
 	if (tb->train_canonical) {  // src/testbed_nerf.cu:3497-3499
 		rc = neus2b_adam_step(&ac, tb->n_params, tb->grad_mlp, (uint16_t*)tb->grad_grid, tb->grad_var, tb->master, tb->adam_m, tb->adam_v,
 		                      (uint16_t*)tb->params, (uint16_t*)tb->params_ema, tb->ema_master, tb->stream);
@@ -852,6 +887,7 @@ extern "C" int neus2b_testbed_train_wait_stats(neus2b_testbed* tb, neus2b_train_
 	h_stats->ek_loss = tb->h_state->ek_loss;
 	h_stats->nonfinite_gradients = tb->h_state->nonfinite;
 	h_stats->device_error = tb->h_state->device_error;
+	h_stats->grad_norm = tb->cfg.max_grad_norm > 0.f && tb->train_canonical ? tb->h_state->grad_norm[0] : 0.f;
 	// a bounded wait inside a kernel ran out: that step's gradients are not to be trusted
 	return tb->h_state->device_error ? NEUS2B_E_DEVICE : NEUS2B_OK;
 }

@@ -224,6 +224,11 @@ class Testbed:
     def ek_loss(self):
         return float(self.stats.ek_loss)
 
+    @property
+    def grad_norm(self):
+        """Global norm of the last read step's gradients ahead of clipping (0 without max_grad_norm)."""
+        return float(self.stats.grad_norm)
+
     # --- device views (torch tensors over the library's buffers; for tests and for NCCL)
     def device_ptrs(self):
         names = ("params", "params_ema", "master", "grad_mlp", "grad_grid", "grad_variance", "bitfield", "density_grid")
