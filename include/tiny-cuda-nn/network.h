@@ -3,7 +3,8 @@
  * (configs/nerf/base.json:40-47, :63-69): a fully fused MLP of 64 ReLU neurons with 1 or 2 hidden layers, no output
  * activation and 16 padded outputs, bound to the C interface's MLP kernels.  NerfNetwork holds two of them
  * (include/neural-graphics-primitives/nerf_network.h:57, :65) and calls forward, backward and, for the eikonal term,
- * backward_backward_input on the first (:212, :229, :402, :560-571). */
+ * backward_backward_input on the first (:212, :229, :402, :560-571).  Beside it, for widths of the caller's choice, ResidualMLP
+ * (networks/residual_mlp.h). */
 #pragma once
 #include <tiny-cuda-nn/object.h>
 
@@ -26,7 +27,7 @@ public:
 /* the input alignment a network type asks of the encoding that feeds it */
 inline uint32_t minimum_alignment(const json& network) {
 	const std::string otype = to_lower(network.value("otype", "FullyFusedMLP"));
-	if (otype == "fullyfusedmlp" || otype == "megakernelmlp") return 16u;
+	if (otype == "fullyfusedmlp" || otype == "megakernelmlp" || otype == "residualmlp") return 16u;
 	return 8u;
 }
 
@@ -217,14 +218,23 @@ private:
 	GPUMemory<float> m_grad_scratch;
 };
 
+TCNN_NAMESPACE_END
+
+#include <tiny-cuda-nn/networks/residual_mlp.h>
+
+TCNN_NAMESPACE_BEGIN
+
 template <typename T>
 Network<T>* create_network(const json& network) {
 	const std::string otype = to_lower(network.value("otype", "FullyFusedMLP"));
-	if (otype != "fullyfusedmlp" && otype != "megakernelmlp")
-		throw std::runtime_error("create_network: network \"" + network.value("otype", "") + "\" is not part of this library (FullyFusedMLP is)");
+	if (otype != "fullyfusedmlp" && otype != "megakernelmlp" && otype != "residualmlp")
+		throw std::runtime_error("create_network: network \"" + network.value("otype", "") + "\" is not part of this library (FullyFusedMLP and ResidualMLP are)");
 	if constexpr (!std::is_same<T, __half>::value) {
 		throw std::runtime_error("create_network: the MLP kernels of this library compute in fp16");
 	} else {
+		if (otype == "residualmlp")
+			return new ResidualMLP<T>{network["n_input_dims"], network["n_output_dims"], network.value("n_neurons", 128u), network.value("n_hidden_layers", 2u),
+			                          network.value("activation", "GELU"), string_to_activation(network.value("output_activation", "None"))};
 		if (network.value("n_neurons", 128u) != 64) throw std::runtime_error("create_network: FullyFusedMLP with 64 neurons only");
 		return new FullyFusedMLP<T>{network["n_input_dims"], network["n_output_dims"], network.value("n_hidden_layers", 5u),
 		                            string_to_activation(network.value("activation", "ReLU")), string_to_activation(network.value("output_activation", "None"))};
