@@ -230,19 +230,19 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 		}
 	}
 	Raw cur[VPT], ahead[kAhead ? VPT : 1];
-	auto fetch = [&](Raw* raw, uint32_t r) {
+	auto fetch = [&](Raw* raw, const T* row, bool there) {
 #pragma unroll
-		for (int k = 0; k < VPT; ++k) {
-			const uint32_t c = (k * TPR + t) * VEC;
-			raw[k] = r < d.n && c < W ? *reinterpret_cast<const Raw*>(x + r * x_ld + c) : zero<Raw>();
-		}
+		for (int k = 0; k < VPT; ++k) raw[k] = there && (k * TPR + t) * VEC < W ? *reinterpret_cast<const Raw*>(row + k * TPR * VEC) : zero<Raw>();
 	};
 	int turn = 0, slot = 0;
 	uint32_t parity = 0, r = blockIdx.x * G + group;
 	const uint32_t step = gridDim.x * G;
 	const uint32_t row_bytes = W * (uint32_t)sizeof(T);
 	unsigned char* const ring = reinterpret_cast<unsigned char*>(params4) + (F::kStaged ? 2 * VEC * TPR * VPT * sizeof(float) : 0) + (size_t)group * depth * row_bytes;
-	if (kAhead) fetch(ahead, r);
+	const T* xp = x + (uint64_t)r * x_ld + t * VEC;  // the thread's first access of the row, and of the row it writes
+	T* yp = y + (uint64_t)r * y_ld + t * VEC;
+	const uint64_t x_step = (uint64_t)step * x_ld, y_step = (uint64_t)step * y_ld;
+	if (kAhead) fetch(ahead, xp, r < d.n);
 	if (RING && t == 0) {
 		for (int i = 0; i < depth; ++i) init_barrier(sptr(&bars[group * kMaxDepth + i]));
 		for (int i = 0; i < depth; ++i) {
@@ -255,11 +255,11 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 	}
 	if (RING) __syncthreads();
 	// every group of the block runs the same number of rounds: the shuffles of narrow groups take the whole warp
-	for (uint32_t r0 = blockIdx.x * G; r0 < d.n; r0 += step, r += step) {
+	for (uint32_t r0 = blockIdx.x * G; r0 < d.n; r0 += step, r += step, xp += x_step, yp += y_step) {
 		if (kAhead) {
 #pragma unroll
 			for (int k = 0; k < VPT; ++k) cur[k] = ahead[kAhead ? k : 0];
-			fetch(ahead, r + step);
+			fetch(ahead, xp + x_step, (uint64_t)r + step < d.n);
 		} else if (RING) {
 			const uint32_t bar = sptr(&bars[group * kMaxDepth + slot]);
 			unsigned char* const row = ring + (size_t)slot * row_bytes;
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 			}
 			if (++slot == depth) slot = 0, parity ^= 1u;
 		} else {
-			fetch(cur, r);
+			fetch(cur, xp, r < d.n);
 		}
 		float s = 0.f;
 #pragma unroll
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 #pragma unroll
 				for (int i = 0; i < VEC; ++i)
 					e[i] = fmaf((e[i] - mean) * rstd, F::kStaged ? g[i] : ga[F::kStaged ? 0 : k * VEC + i], F::kStaged ? b[i] : be[F::kStaged ? 0 : k * VEC + i]);
-				if (c < W) *reinterpret_cast<Raw*>(y + r * y_ld + c) = P::put(e);
+				if (c < W) *reinterpret_cast<Raw*>(yp + k * TPR * VEC) = P::put(e);
 			}
 			if (mean_out && t == 0) mean_out[r] = mean, rstd_out[r] = rstd;
 		}

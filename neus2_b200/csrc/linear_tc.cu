@@ -109,7 +109,8 @@ struct Shape {
 	// Shared memory behind the operand stages: chunks of the epilogue (`chunks` for every warp), ones tile and barriers; alignment of the base.
 	static constexpr int fixed(int chunks) { return (SWAP || WGRAD ? 0 : kEpiWarps * chunks * kChunkBytes) + 2048 + 1024; }
 	static constexpr int stages(int chunks) {
-		const int room = (kSmemMost - fixed(chunks)) / kStage;
+		// few samples: room for a second CTA on the SM
+		const int room = ((SWAP && !GATHER ? kSmemMost / 2 - 1024 : kSmemMost) - fixed(chunks)) / kStage;
 		return room < kMaxStages ? room : kMaxStages;
 	}
 	static constexpr int kCols = kBufs * BN + (WGRAD && !PAIR ? 32 : 0);
@@ -173,7 +174,7 @@ __device__ __forceinline__ void chunk_store(const uint32_t (&row)[16], void* bas
 	}
 }
 template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
-__global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>::kThreads, 1) product_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>::kThreads, SWAP && !GATHER ? 2 : 1) product_kernel(const __grid_constant__ Args p) {
 	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
 	extern __shared__ unsigned char smem_raw[];
 	unsigned char* smem = smem_raw + ((1024u - (sptr(smem_raw) & 1023u)) & 1023u);
@@ -631,10 +632,10 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 	return NEUS2B_OK;
 }
 
-// over how many CTAs of a cluster a tile's sum is split: as many as the SMs can take, with at least four steps of 64 for each
-static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks) {
+// over how many CTAs of a cluster a tile's sum is split: as many as the SMs can take (`each` at a time), with at least four steps of 64 for each
+static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks, uint32_t each) {
 	uint32_t c = 1;
-	while (c < 8 && tiles * c * 2 <= (uint64_t)kSMs && kblocks >= c * 2 * 4) c *= 2;
+	while (c < 8 && tiles * c * 2 <= (uint64_t)kSMs * each && kblocks >= c * 2 * 4) c *= 2;
 	return c;
 }
 
@@ -647,17 +648,17 @@ static int product_of(const Product& p, cudaStream_t stream) {
 	a.splits = a.cluster = 1;
 	const uint32_t kblocks = tiles_of(p.K, kBK);
 	// grid of one-CTA tiles; may_split: the kernel can join a cluster's parts
-	auto grid = [&](uint32_t bn, bool may_split) -> uint32_t {
+	auto grid = [&](uint32_t bn, bool may_split, uint32_t each) -> uint32_t {
 		a.tiles_m = tiles_of(a.M, kBM);
 		a.tiles_n = tiles_of(a.N, bn);
 		const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
 		if (tiles >= (1ull << 31)) return 0;
-		a.cluster = a.splits = may_split ? cluster_for(tiles, kblocks) : 1u;
-		return (uint32_t)(a.cluster > 1 ? tiles * a.cluster : tiles < (uint64_t)kSMs ? tiles : (uint64_t)kSMs);
+		a.cluster = a.splits = may_split ? cluster_for(tiles, kblocks, each) : 1u;
+		return (uint32_t)(a.cluster > 1 ? tiles * a.cluster : tiles < (uint64_t)kSMs * each ? tiles : (uint64_t)kSMs * each);
 	};
 #define N2B_GO(BN, AMN, BMN_, SWAP, GATHER)                                                          \
 	do {                                                                                             \
-		const uint32_t ctas = grid(BN, BN <= 128);                                                   \
+		const uint32_t ctas = grid(BN, BN <= 128, SWAP && !GATHER ? 2 : 1);                                       \
 		if (!ctas) return NEUS2B_E_TOO_LARGE;                                                        \
 		return launch<BN, AMN, BMN_, SWAP, false, GATHER, false>(a, ctas, stream);                   \
 	} while (0)
