@@ -276,49 +276,53 @@ def _refuse(what):
     raise L.Neus2bError("neus2b: " + what)
 
 
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _home(t, name):
-    """The device all tensors of a call have to be on: the current one, whose current stream the call is enqueued on."""
-    if not t.is_cuda:
+    """Index of the device all tensors of a call have to be on: the current one, whose current stream the call is enqueued on."""
+    dev = t.get_device()
+    if dev < 0:
         _refuse(f"{name} has to be a CUDA tensor")
-    if t.device.index != torch.cuda.current_device():
-        _refuse(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return t.device
+    if dev != _current_device():
+        _refuse(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
+    return dev
 
 
-def _rows(t, name, n, width, dtype, device):
+def _rows(t, name, n, width, dtype, dev):
     """(address, row stride in entries) of a [n][width] tensor with contiguous rows; (None, 0) for None."""
     if t is None:
         return None, 0
-    if t.device != device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
-        _refuse(f"{name} has to be {dtype} [{n}][{width}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != (n, width):
+        _refuse(f"{name} has to be {dtype} [{n}][{width}] on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
     row, col = t.stride()
     if (col != 1 and width > 1) or (row < width and n > 1):
         _refuse(f"{name}: the entries of a row have to be contiguous and the rows apart, got strides ({row}, {col})")
     return t.data_ptr(), row if n > 1 else width
 
 
-def _vector(t, name, width, dtype, device):
+def _vector(t, name, width, dtype, dev):
     if t is None:
         return None
-    if t.device != device or t.dtype != dtype or t.shape != (width,) or not t.is_contiguous():
-        _refuse(f"{name} has to be contiguous {dtype} [{width}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != (width,) or not t.is_contiguous():
+        _refuse(f"{name} has to be contiguous {dtype} [{width}] on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _weights(w, dtype, device):
-    if w.dim() != 2 or w.dtype != dtype or w.device != device or not w.is_contiguous():
-        _refuse(f"the weights have to be contiguous {dtype} [out][in] on {device}, got {w.dtype} {list(w.shape)} on {w.device}")
+def _weights(w, dtype, dev):
+    if w.dtype is not dtype or w.get_device() != dev or w.dim() != 2 or not w.is_contiguous():
+        _refuse(f"the weights have to be contiguous {dtype} [out][in] on cuda:{dev}, got {w.dtype} {list(w.shape)} on {w.device}")
     return w.shape
 
 
-def _workspace(need, given, device):
+def _workspace(need, given, like):
     """(tensor that keeps it alive, address, bytes)"""
     if not need:
         return None, None, 0
     if given is None:
-        given = torch.empty(need, dtype=torch.uint8, device=device)
-    elif given.device != device or not given.is_contiguous() or given.numel() * given.element_size() < need:
-        _refuse(f"the workspace has to be {need} contiguous bytes on {device}")
+        given = like.new_empty(need, dtype=torch.uint8)
+    elif given.get_device() != like.get_device() or not given.is_contiguous() or given.numel() * given.element_size() < need:
+        _refuse(f"the workspace has to be {need} contiguous bytes on {like.device}")
     return given, given.data_ptr(), given.numel() * given.element_size()
 
 
@@ -328,14 +332,13 @@ def _bytes(query, desc, *flags):
     return need.value
 
 
-def _gradient(t, name, shape, mode, device):
+def _gradient(t, name, shape, mode, like):
     """The fp32 tensor a parameter gradient goes to: the caller's, or a new one where there is nothing to add to."""
     if t is None:
-        if mode == L.GRAD_ACCUMULATE:
-            return torch.zeros(shape, dtype=torch.float32, device=device)
-        return torch.empty(shape, dtype=torch.float32, device=device)
-    if t.device != device or t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        _refuse(f"{name} has to be contiguous float32 {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+        new = like.new_zeros if mode == L.GRAD_ACCUMULATE else like.new_empty
+        return new(shape, dtype=torch.float32)
+    if t.get_device() != like.get_device() or t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
+        _refuse(f"{name} has to be contiguous float32 {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t
 
 
@@ -352,16 +355,16 @@ def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_p
     rp, rs = _rows(residual, "residual", n, n_out, t, dev)
     bp = _vector(bias, "bias", n_out, t, dev)
     if out is None:
-        out = torch.empty((n, n_out), dtype=t, device=dev)
+        out = x.new_empty((n, n_out))
     yp, ys = _rows(out, "out", n, n_out, t, dev)
-    z = torch.empty((n, n_out), dtype=t, device=dev) if want_preact else None
+    z = x.new_empty((n, n_out)) if want_preact else None
     d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
     lib, wp = L.lib(), w.data_ptr()
     keep, wsp, wsb = None, None, 0
     if (xp | wp | xs * 2 | n_in * 2) & 15:
-        keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_forward_workspace, d, 1), workspace, dev)
+        keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_forward_workspace, d, 1), workspace, x)
     L.check(lib.neus2b_linear_forward(C.byref(d), xp, xs, wp, bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out, wsp, wsb,
-                                      L.cur_stream()))
+                                      _raw_stream(dev)))
     return (out, z) if want_preact else out
 
 
@@ -385,17 +388,17 @@ def linear_backward(x, w, dL_dout, activation=L.ACT_NONE, preact=None, below_act
     zp, zs = _rows(preact, "preact", n, n_out, t, dev)
     bzp, bzs = _rows(below_preact, "below_preact", n, n_in, t, dev)
     sp, ss = _rows(skip, "skip", n, n_in, t, dev)
-    din = torch.empty((n, n_in), dtype=t, device=dev) if want_din else None
+    din = x.new_empty((n, n_in)) if want_din else None
     params = mode != L.GRAD_IGNORE
-    wgrad = _gradient(wgrad, "wgrad", (n_out, n_in), mode, dev) if params else None
-    bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, dev) if params and want_bias else None
+    wgrad = _gradient(wgrad, "wgrad", (n_out, n_in), mode, x) if params else None
+    bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, x) if params and want_bias else None
     d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
     lib = L.lib()
     unaligned = 1 if (xp | w.data_ptr() | dyp | xs * 2 | n_in * 2 | dys * 2) & 15 else 0
-    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_backward_workspace, d, unaligned), workspace, dev)
+    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_backward_workspace, d, unaligned), workspace, x)
     L.check(lib.neus2b_linear_backward(C.byref(d), xp, xs, w.data_ptr(), zp, zs, dyp, dys, below_activation, bzp, bzs, sp, ss,
                                        din.data_ptr() if want_din else None, n_in, wgrad.data_ptr() if params else None,
-                                       bgrad.data_ptr() if bgrad is not None else None, mode, wsp, wsb, L.cur_stream()))
+                                       bgrad.data_ptr() if bgrad is not None else None, mode, wsp, wsb, _raw_stream(dev)))
     return din, wgrad, bgrad
 
 
@@ -418,12 +421,14 @@ def layer_norm_forward(x, gamma, beta=None, eps=1e-5, want_stats=False, out=None
     xp, xs = _rows(x, "x", n, width, x.dtype, dev)
     gp, bp = _vector(gamma, "gamma", width, gamma.dtype, dev), _vector(beta, "beta", width, gamma.dtype, dev)
     if out is None:
-        out = torch.empty((n, width), dtype=x.dtype, device=dev)
+        out = x.new_empty((n, width))
     yp, ys = _rows(out, "out", n, width, x.dtype, dev)
-    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if want_stats else None
-    sp = stats.data_ptr() if want_stats else None
-    L.check(L.lib().neus2b_layer_norm_forward(C.byref(d), xp, xs, gp, bp, yp, ys, sp, sp + 4 * n if want_stats else None, L.cur_stream()))
-    return (out, stats[0], stats[1]) if want_stats else out
+    if not want_stats:
+        L.check(L.lib().neus2b_layer_norm_forward(C.byref(d), xp, xs, gp, bp, yp, ys, None, None, _raw_stream(dev)))
+        return out
+    mean, rstd = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
+    L.check(L.lib().neus2b_layer_norm_forward(C.byref(d), xp, xs, gp, bp, yp, ys, mean.data_ptr(), rstd.data_ptr(), _raw_stream(dev)))
+    return out, mean, rstd
 
 
 def layer_norm_backward(x, gamma, mean, rstd, dL_dout, skip=None, dgamma=None, dbeta=None, mode=L.GRAD_OVERWRITE, eps=1e-5, want_din=True,
@@ -437,15 +442,15 @@ def layer_norm_backward(x, gamma, mean, rstd, dL_dout, skip=None, dgamma=None, d
     sp, ss = _rows(skip, "skip", n, width, x.dtype, dev)
     gp = _vector(gamma, "gamma", width, gamma.dtype, dev)
     mp, rp = _vector(mean, "mean", n, torch.float32, dev), _vector(rstd, "rstd", n, torch.float32, dev)
-    din = torch.empty((n, width), dtype=x.dtype, device=dev) if want_din else None
+    din = x.new_empty((n, width)) if want_din else None
     params = mode != L.GRAD_IGNORE
-    dgamma = _gradient(dgamma, "dgamma", (width,), mode, dev) if params else None
-    dbeta = _gradient(dbeta, "dbeta", (width,), mode, dev) if params else None
+    dgamma = _gradient(dgamma, "dgamma", (width,), mode, x) if params else None
+    dbeta = _gradient(dbeta, "dbeta", (width,), mode, x) if params else None
     lib = L.lib()
-    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_layer_norm_backward_workspace, d) if params else 0, workspace, dev)
+    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_layer_norm_backward_workspace, d) if params else 0, workspace, x)
     L.check(lib.neus2b_layer_norm_backward(C.byref(d), xp, xs, gp, mp, rp, dyp, dys, sp, ss, din.data_ptr() if want_din else None, width,
                                            dgamma.data_ptr() if params else None, dbeta.data_ptr() if params else None, mode, wsp, wsb,
-                                           L.cur_stream()))
+                                           _raw_stream(dev)))
     return din, dgamma, dbeta
 
 
@@ -466,8 +471,8 @@ class GradientSet:
         rows = (L.GradTensor * len(grads))()
         for i, (g, o) in enumerate(zip(grads, out)):
             for t in (g, o):
-                if t.device != dev or t.dtype not in _DTYPES or t.dtype != g.dtype or t.numel() != g.numel() or not t.is_contiguous():
-                    _refuse(f"tensor {i}: gradients and outputs have to be contiguous float32, float16 or bfloat16 on {dev}, alike in type and size")
+                if t.get_device() != dev or t.dtype not in _DTYPES or t.dtype != g.dtype or t.numel() != g.numel() or not t.is_contiguous():
+                    _refuse(f"tensor {i}: gradients and outputs have to be contiguous float32, float16 or bfloat16 on cuda:{dev}, alike in type and size")
             rows[i] = L.GradTensor(g.data_ptr(), o.data_ptr(), g.numel(), _DTYPES[g.dtype])
         lib = L.lib()
         nbytes, pieces = C.c_uint64(0), C.c_uint32(0)
@@ -475,18 +480,18 @@ class GradientSet:
         host = torch.zeros(max(1, nbytes.value // 8), dtype=torch.int64)
         L.check(lib.neus2b_grad_table(rows, len(grads), host.data_ptr(), C.byref(nbytes), C.byref(pieces)))
         self.n_pieces = pieces.value
-        self.table = host.to(dev)
+        self.table = host.to(grads[0].device)
         self.workspace_bytes = int(lib.neus2b_grad_norm_workspace(self.n_pieces))
-        self.workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=dev)
+        self.workspace = self.table.new_empty(self.workspace_bytes, dtype=torch.uint8)
         self._keep = (grads, out)
 
     def _call(self, f, max_norm, scale, skip_nonfinite, nonfinite):
         dev = _home(self.table, "the gradient set")
-        if nonfinite is not None and (nonfinite.device != dev or nonfinite.dtype != torch.int32 or nonfinite.numel() != 1):
-            _refuse(f"nonfinite has to be one int32 on {dev}")
-        result = torch.empty(2, dtype=torch.float32, device=dev)
+        if nonfinite is not None and (nonfinite.get_device() != dev or nonfinite.dtype is not torch.int32 or nonfinite.numel() != 1):
+            _refuse(f"nonfinite has to be one int32 on cuda:{dev}")
+        result = self.table.new_empty(2, dtype=torch.float32)
         L.check(f(self.table.data_ptr(), self.n_pieces, scale, max_norm, L.NORM_SKIP_NONFINITE if skip_nonfinite else 0, result.data_ptr(),
-                  nonfinite.data_ptr() if nonfinite is not None else None, self.workspace.data_ptr(), self.workspace_bytes, L.cur_stream()))
+                  nonfinite.data_ptr() if nonfinite is not None else None, self.workspace.data_ptr(), self.workspace_bytes, _raw_stream(dev)))
         return result
 
     def norm(self, max_norm=float("inf"), scale=1.0, skip_nonfinite=False, nonfinite=None):
