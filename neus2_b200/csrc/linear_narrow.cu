@@ -344,10 +344,12 @@ static int launch_narrow(const Product& r, const Product* w, cudaStream_t stream
 
 using namespace lin;
 
-// More than two tiles of samples (below, spreading a tile's work over several SMs is faster), and every matrix readable by TMA.
+// More than two tiles of samples (below, spreading a tile's work over several SMs is faster), and every matrix readable by TMA.  Results
+// leave by TMA stores, which write whole 16-byte units of a row: their width has to be a multiple of 8, or the units would reach into
+// what the caller keeps behind the row.
 bool narrow_fits(const Product& r, bool backward, const Product* w) {
 	const Epilogue& e = r.e;
-	if (r.M <= 256 || r.N > 64 || r.K > 128) return false;
+	if (r.M <= 256 || r.N > 64 || r.K > 128 || (e.out && r.N % 8)) return false;
 	auto fine = [](const void* p, uint64_t ld) { return !p || tma_ok(p, ld); };
 	if (!tma_ok(r.a, r.a_ld)) return false;
 	if (e.out && !(tma_ok(r.b, r.b_ld) && tma_ok(e.out, e.out_ld) && fine(e.slope_z, e.slope_ld) && fine(e.add, e.add_ld) && fine(e.preact, e.preact_ld))) return false;

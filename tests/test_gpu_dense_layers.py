@@ -93,6 +93,34 @@ def test_linear_backward(ops, shape, t):
         R.within(f"db {k}", db, wb, eb)
 
 
+@pytest.mark.parametrize("shape", [(1000, 37, 64), (700, 64, 37), (300, 61, 33), (5000, 13, 9), (40, 37, 29), (500, 1001, 333), (2000, 100, 201)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_rows_on_16_byte_boundaries_with_odd_widths(ops, shape):
+    """Widths that fill no 16-byte unit in rows that start on 16-byte boundaries: what lies behind a row (NaN in the inputs, a marker
+    around the outputs) is neither used nor written."""
+    n, i, o = shape
+    t = torch.float16
+    g = gen(n + i)
+
+    def padded(rows_, width, scale=1.0):
+        full = torch.full((rows_, (width + 15) // 8 * 8), float("nan"), dtype=t, device="cuda")
+        full[:, :width] = rows(g, rows_, width, t, scale)
+        return full[:, :width]
+    x, r, dy, zb = padded(n, i), padded(n, o), padded(n, o, 0.1), padded(n, i)
+    w, b = rows(g, o, i, t, 0.3), rows(g, 1, o, t)[0]
+    y, untouched = framed(n, o, t, (o + 15) // 8 * 8 - o)
+    _, z = ops.linear_forward(x, w, b, r, R.GELU, want_preact=True, out=y)
+    wy, wz, ey, ez = R.linear(x, w, b, r, R.GELU, t)
+    R.within("y", y, wy, ey)
+    R.within("z", z, wz, ez)
+    assert untouched()
+    dx, dw, db = ops.linear_backward(x, w, dy, below_activation=R.SILU, below_preact=zb)
+    wx, ww, wb, ex, ew, eb = R.linear_backward(x, w, dy, R.SILU, zb, None, t)
+    R.within("dx", dx, wx, ex)
+    R.within("dw", dw, ww, ew)
+    R.within("db", db, wb, eb)
+
+
 @pytest.mark.parametrize("t", HALF, ids=["f16", "bf16"])
 def test_linear_backward_of_an_activated_layer(ops, t):
     """The layer's own activation: dz is rounded to the layer's type on the way, which the bound counts."""
