@@ -366,7 +366,8 @@ int neus2b_delta_optimizer_step(const neus2b_adam_cfg* cfg, float* d_sums, float
  * for networks beside them.  Values are fp16 or bf16 (layer norm: fp32 too), sums and statistics fp32.  Matrices are row-major,
  * one sample per row, rows a caller-given number of ENTRIES apart (*_stride, at least the width; entries of a row are contiguous).
  * Any width, stride and entry-aligned address is taken; rows that start on 16-byte boundaries are faster.  n == 0 is allowed.
- * Outputs may not overlap inputs unless a comment says so.  Parameter gradients are fp32 and follow grad_mode
+ * Outputs may not overlap inputs unless a comment says so (then with the same stride).  At most 2^30 samples and entries a row
+ * (layer norm: 2^31 samples).  Parameter gradients are fp32 and follow grad_mode
  * (NEUS2B_GRAD_*, IGNORE: the pointers are not used).  Every sum has a fixed order: the same call gives the same bits. */
 #define NEUS2B_F32 0
 #define NEUS2B_F16 1

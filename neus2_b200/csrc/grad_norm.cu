@@ -267,6 +267,7 @@ static int run(const void* d_table, uint32_t n_pieces, float scale, float max_no
                uint64_t workspace_bytes, bool clip, cudaStream_t s) {
 	if (!d_result || ((uintptr_t)d_result & 3) || ((uintptr_t)d_nonfinite & 3) || (flags & ~NEUS2B_NORM_SKIP_NONFINITE)) return NEUS2B_E_INVALID;
 	if (!(max_norm > 0.f) || !isfinite(scale)) return NEUS2B_E_INVALID;
+	if (n_pieces > 0x7fffffffu) return NEUS2B_E_TOO_LARGE;
 	if (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < neus2b_grad_norm_workspace(n_pieces)) return NEUS2B_E_INVALID;
 	if (n_pieces && (!d_table || ((uintptr_t)d_table & 15))) return NEUS2B_E_INVALID;
 	const uint32_t blocks = blocks_for(n_pieces);
@@ -296,7 +297,7 @@ extern "C" int neus2b_grad_table(const neus2b_grad_tensor* h_tensors, uint32_t n
 		if (g.n && (!g.d_in || (((uintptr_t)g.d_in | (uintptr_t)g.d_out) & (b - 1)))) return NEUS2B_E_INVALID;
 		if (g.n > (1ull << 60)) return NEUS2B_E_TOO_LARGE;
 		const uint64_t entries = kPieceBytes / b, pieces = (g.n + entries - 1) / entries;
-		if (count + pieces > 0xffffffffull) return NEUS2B_E_TOO_LARGE;
+		if (count + pieces > 0x7fffffffull) return NEUS2B_E_TOO_LARGE;
 		for (uint64_t k = 0; p && k < pieces; ++k) {
 			const uint64_t at = k * entries;
 			p[count + k] = Piece{(const char*)g.d_in + at * b, g.d_out ? (char*)g.d_out + at * b : nullptr, (uint32_t)(g.n - at < entries ? g.n - at : entries),

@@ -668,9 +668,12 @@ int write_layer_norm_error(uint32_t flags) {
 
 static int check_desc(const neus2b_layer_norm_desc* d) {
 	if (!d || d->width == 0 || !(d->epsilon > 0.f) || isinf(d->epsilon)) return NEUS2B_E_INVALID;
+	if (d->n > (1u << 31) || d->width > (1u << 30)) return NEUS2B_E_TOO_LARGE;
 	if (d->dtype > NEUS2B_BF16 || (d->param_dtype != NEUS2B_F32 && d->param_dtype != d->dtype)) return NEUS2B_E_UNSUPPORTED;
 	return NEUS2B_OK;
 }
+// An output in place of an input has to have its rows where the input has them.
+static bool clash(const void* out, uint64_t out_stride, const void* in, uint64_t in_stride, uint32_t n) { return out && out == in && n > 1 && out_stride != in_stride; }
 static bool bad_rows(const void* p, uint64_t stride, uint32_t width, size_t align) { return !p || stride < width || ((uintptr_t)p & (align - 1)); }
 
 }  // namespace n2b
@@ -685,6 +688,7 @@ extern "C" int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, con
 		return NEUS2B_E_INVALID;
 	if (desc->n == 0) return NEUS2B_OK;
 	if (bad_rows(d_x, x_stride, desc->width, b) || bad_rows(d_y, y_stride, desc->width, b)) return NEUS2B_E_INVALID;
+	if (clash(d_y, y_stride, d_x, x_stride, desc->n)) return NEUS2B_E_INVALID;
 	return with_float_type(desc->dtype, [&](auto t) {
 		using T = decltype(t);
 		constexpr int V = 16 / sizeof(T);
@@ -760,6 +764,7 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 	if (!d_mean || !d_rstd || bad_rows(d_x, x_stride, width, b) || bad_rows(d_dL_dy, dy_stride, width, b) ||
 	    (d_skip && bad_rows(d_skip, skip_stride, width, b)) || (d_dL_dx && bad_rows(d_dL_dx, dx_stride, width, b)))
 		return NEUS2B_E_INVALID;
+	if ((d_dL_dx && d_dL_dx == d_x) || clash(d_dL_dx, dx_stride, d_dL_dy, dy_stride, n) || clash(d_dL_dx, dx_stride, d_skip, skip_stride, n)) return NEUS2B_E_INVALID;
 	if (need && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need)) return NEUS2B_E_INVALID;
 	return with_float_type(desc->dtype, [&](auto t) {
 		using T = decltype(t);

@@ -17,6 +17,11 @@ __global__ void __launch_bounds__(256) slope_kernel(uint64_t n, uint32_t width, 
 static bool bad_desc(const neus2b_linear_desc* d) {
 	return !d || d->in_width == 0 || d->out_width == 0 || d->activation > NEUS2B_ACT_SILU;
 }
+constexpr uint32_t kMost = 1u << 30;  // samples and widths: tile coordinates are signed 32-bit numbers
+static bool too_large(const neus2b_linear_desc* d) { return d->n > kMost || d->in_width > kMost || d->out_width > kMost; }
+// An output that is an input, other than as the interface allows it: the same rows, read by the thread that writes them.
+static bool clash(const void* out, const void* in) { return out && out == in; }
+static bool clash(const void* out, uint64_t out_stride, const void* in, uint64_t in_stride, uint32_t n) { return out && out == in && n > 1 && out_stride != in_stride; }
 static bool bad_matrix(const void* p, uint64_t stride, uint32_t width, size_t align) { return !p || stride < width || ((uintptr_t)p & (align - 1)); }
 static bool bad_optional(const void* p, uint64_t stride, uint32_t width, size_t align) { return p && bad_matrix(p, stride, width, align); }
 
@@ -45,6 +50,7 @@ static void realigned(const void*& p, uint64_t& ld, uint32_t rows, uint32_t cols
 extern "C" int neus2b_linear_forward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes) {
 	if (bad_desc(desc) || !bytes) return NEUS2B_E_INVALID;
 	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
+	if (too_large(desc)) return NEUS2B_E_TOO_LARGE;
 	*bytes = unaligned && desc->n > kFewSamples ? copy_bytes(desc->n, desc->in_width) + copy_bytes(desc->out_width, desc->in_width) : 0;
 	return NEUS2B_OK;
 }
@@ -59,6 +65,9 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	if (desc->n == 0) return NEUS2B_OK;
 	if (bad_matrix(d_x, x_stride, in, 2) || bad_matrix(d_y, y_stride, out, 2) || bad_optional(d_residual, residual_stride, out, 2) ||
 	    bad_optional(d_preact, preact_stride, out, 2))
+		return NEUS2B_E_INVALID;
+	if (clash(d_y, d_x) || clash(d_y, d_w) || clash(d_y, d_preact) || clash(d_preact, d_x) || clash(d_preact, d_w) || clash(d_preact, d_residual) ||
+	    clash(d_y, y_stride, d_residual, residual_stride, desc->n))
 		return NEUS2B_E_INVALID;
 	Product p{};
 	p.a = d_x, p.a_ld = x_stride, p.b = d_w, p.b_ld = in;
@@ -89,6 +98,7 @@ static uint64_t copies_bytes(const neus2b_linear_desc* d) {
 extern "C" int neus2b_linear_backward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes) {
 	if (bad_desc(desc) || !bytes) return NEUS2B_E_INVALID;
 	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
+	if (too_large(desc)) return NEUS2B_E_TOO_LARGE;
 	uint64_t parts = 0;
 	if (desc->n) {
 		const uint64_t narrow = narrow_workspace(desc->out_width, desc->in_width, desc->n);
@@ -123,6 +133,9 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	if (desc->activation != NEUS2B_ACT_NONE && bad_matrix(d_preact, preact_stride, out, 2)) return NEUS2B_E_INVALID;
 	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE && bad_matrix(d_below_preact, below_stride, in, 2)) return NEUS2B_E_INVALID;
 	if (need && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need)) return NEUS2B_E_INVALID;
+	if (clash(d_dL_dx, d_x) || clash(d_dL_dx, d_w) || clash(d_dL_dx, d_dL_dy) || clash(d_dL_dx, d_preact) || clash(d_dL_dx, d_below_preact) ||
+	    clash(d_dL_dx, dx_stride, d_skip, skip_stride, n))
+		return NEUS2B_E_INVALID;
 	const void *dz = d_dL_dy, *xs = d_x, *ws = d_w;
 	uint64_t dz_ld = dy_stride, xs_ld = x_stride, ws_ld = in;
 	char* at = (char*)d_workspace;

@@ -73,7 +73,6 @@ __global__ void __launch_bounds__(Narrow<BACKWARD>::kThreads, 1) narrow_kernel(c
 	               wempty = wfull + 16, wload = wempty + 16;
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 	const bool bf = p.bf16 != 0;
-	let_next_start();
 
 	if (tid == 0) {
 		for (uint32_t i = 0; i < p.stages; ++i) {
@@ -94,6 +93,7 @@ __global__ void __launch_bounds__(Narrow<BACKWARD>::kThreads, 1) narrow_kernel(c
 	__syncthreads();
 	tc::fence_after_sync();
 	const uint32_t tmem = *tmem_ptr;
+	let_next_start();  // (the next kernel's blocks may take tensor memory: only now that this one has its own)
 	const uint32_t tiles = (p.n + 127u) / 128u;
 	const uint32_t x_at = slabs * kTile, slope_at = x_at + (p.params ? kTile : 0), add_at = slope_at + (p.slope ? kTile : 0);
 	bool ok = true;

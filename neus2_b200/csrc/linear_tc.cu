@@ -187,7 +187,6 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 	const bool bf = p.bf16 != 0;
 	const uint32_t rank = PAIR || p.cluster > 1 ? cluster_rank() : 0u;
-	let_next_start();
 
 	if (tid == 0) {
 		for (uint32_t i = 0; i < stages; ++i) {
@@ -209,6 +208,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	else __syncthreads();
 	tc::fence_after_sync();
 	const uint32_t tmem = *tmem_ptr;
+	let_next_start();     // (the next kernel's blocks may take tensor memory: only now that this one has its own)
 	wait_for_previous();  // the set-up above runs beside the end of the kernel ahead
 
 	// A cluster that splits k computes one tile; a pair, or a CTA by itself, takes every `step`-th.

@@ -13,13 +13,14 @@ def lib():
     return L, L.lib()
 
 
-FAKE = 4096  # never dereferenced
-INVALID, UNSUPPORTED = -1, -2
+FAKE = 4096  # addresses that are never dereferenced
+X, W, Y, DY, DX = (FAKE * k for k in (3, 5, 7, 11, 13))
+INVALID, UNSUPPORTED, TOO_LARGE = -1, -2, -5
 
 
 def test_linear_forward(lib):
     L, f = lib
-    ok = dict(n=4, in_width=32, out_width=16, dtype=L.F16, activation=0, x=FAKE, xs=32, w=FAKE, b=None, r=None, rs=0, y=FAKE, ys=16, z=None, zs=0, ws=None, wsb=0)
+    ok = dict(n=4, in_width=32, out_width=16, dtype=L.F16, activation=0, x=X, xs=32, w=W, b=None, r=None, rs=0, y=Y, ys=16, z=None, zs=0, ws=None, wsb=0)
 
     def call(**kw):
         a = dict(ok, **kw)
@@ -28,8 +29,13 @@ def test_linear_forward(lib):
     assert f.neus2b_linear_forward(None, FAKE, 32, FAKE, None, None, 0, FAKE, 16, None, 0, None, 0, None) == INVALID
     assert call(dtype=L.F32) == UNSUPPORTED and call(dtype=7) == UNSUPPORTED
     for bad in (dict(activation=4), dict(in_width=0), dict(out_width=0), dict(x=None), dict(w=None), dict(y=None), dict(xs=31), dict(ys=15), dict(r=FAKE, rs=15),
-                dict(z=FAKE, zs=3), dict(x=FAKE + 1), dict(w=FAKE + 1), dict(b=FAKE + 1), dict(y=FAKE + 1), dict(r=FAKE + 1, rs=16)):
+                dict(z=FAKE, zs=3), dict(x=X + 1), dict(w=W + 1), dict(b=FAKE + 1), dict(y=Y + 1), dict(r=FAKE + 1, rs=16)):
         assert call(**bad) == INVALID, bad
+    B = FAKE * 2
+    for bad in (dict(y=X, ys=32), dict(y=W), dict(z=Y, zs=16), dict(z=X, zs=32), dict(z=W, zs=16), dict(r=B, rs=16, z=B, zs=16),
+                dict(r=Y, rs=24)):  # outputs on inputs
+        assert call(**bad) == INVALID, bad
+    assert call(n=(1 << 30) + 1) == TOO_LARGE and call(in_width=(1 << 30) + 1, xs=1 << 31) == TOO_LARGE
     assert call(n=0, x=None, y=None) == 0
     need = C.c_uint64(7)
     d = L.LinearDesc(500, 33, 16, L.F16, 0)
@@ -42,7 +48,7 @@ def test_linear_forward(lib):
 
 def test_linear_backward(lib):
     L, f = lib
-    ok = dict(n=4, dtype=L.BF16, activation=0, x=FAKE, xs=32, w=FAKE, z=None, zs=0, dy=FAKE, dys=16, below=0, bz=None, bzs=0, skip=None, ss=0, dx=FAKE,
+    ok = dict(n=4, dtype=L.BF16, activation=0, x=X, xs=32, w=W, z=None, zs=0, dy=DY, dys=16, below=0, bz=None, bzs=0, skip=None, ss=0, dx=DX,
               dxs=32, dw=FAKE, db=FAKE, mode=1, ws=None, wsb=0)
 
     def call(**kw):
@@ -55,13 +61,16 @@ def test_linear_backward(lib):
         return f.neus2b_linear_backward(C.byref(d), a["x"], a["xs"], a["w"], a["z"], a["zs"], a["dy"], a["dys"], a["below"], a["bz"], a["bzs"], a["skip"],
                                         a["ss"], a["dx"], a["dxs"], a["dw"], a["db"], a["mode"], a["ws"], a["wsb"], None)
     assert call(dtype=L.F32) == UNSUPPORTED
-    for bad in (dict(dy=None), dict(dys=15), dict(x=None), dict(w=None), dict(dx=FAKE + 1), dict(dxs=31), dict(dw=FAKE + 2), dict(db=FAKE + 1), dict(mode=3),
+    for bad in (dict(dy=None), dict(dys=15), dict(x=None), dict(w=None), dict(dx=DX + 1), dict(dxs=31), dict(dw=FAKE + 2), dict(db=FAKE + 1), dict(mode=3),
                 dict(mode=-1), dict(below=4), dict(below=2), dict(below=2, bz=FAKE, bzs=31), dict(skip=FAKE, ss=31), dict(activation=2),
                 dict(activation=2, z=FAKE, zs=15), dict(activation=2, z=FAKE, zs=16, ws=FAKE, wsb=4), dict(activation=2, z=FAKE, zs=16, ws=FAKE + 8, wsb=1 << 30)):
         assert call(**bad) == INVALID, bad
+    for bad in (dict(dx=X), dict(dx=DY), dict(dx=W), dict(below=1, bz=DX, bzs=32), dict(activation=1, z=DX, zs=16), dict(skip=DX, ss=40)):  # outputs on inputs
+        assert call(**bad) == INVALID, bad
+    assert call(n=(1 << 30) + 1) == TOO_LARGE
     d = L.LinearDesc(4, 32, 16, L.BF16, 0)
     assert f.neus2b_linear_backward_workspace(C.byref(d), 0, None) == INVALID
-    assert call(dy=FAKE + 2) == INVALID and call(x=FAKE + 2) == INVALID  # the workspace has no room for their copies
+    assert call(dy=DY + 2) == INVALID and call(x=X + 2) == INVALID  # the workspace has no room for their copies
 
 
 def test_layer_norm(lib):
@@ -75,15 +84,17 @@ def test_layer_norm(lib):
                 dict(xs=31), dict(ys=31), dict(x=FAKE + 1), dict(g=FAKE + 1), dict(pdtype=L.F32, g=FAKE + 2), dict(mean=FAKE), dict(rstd=FAKE),
                 dict(mean=FAKE, rstd=FAKE + 1)):
         assert fwd(**bad) == INVALID, bad
+    assert fwd(xs=40) == INVALID  # in place, rows elsewhere
+    assert fwd(n=(1 << 31) + 1, y=FAKE * 2) == TOO_LARGE
     assert fwd(n=0, x=None, y=None) == 0
 
-    def bwd(n=4, x=FAKE, xs=32, g=FAKE, mean=FAKE, rstd=FAKE, dy=FAKE, dys=32, skip=None, ss=0, dx=FAKE, dxs=32, dg=FAKE, db=FAKE, mode=1, short=0):
+    def bwd(n=4, x=X, xs=32, g=FAKE, mean=FAKE, rstd=FAKE, dy=DY, dys=32, skip=None, ss=0, dx=DX, dxs=32, dg=FAKE, db=FAKE, mode=1, short=0):
         d = L.LayerNormDesc(n, 32, L.F16, L.F16, 1e-5)
         need = C.c_uint64(0)
         assert f.neus2b_layer_norm_backward_workspace(C.byref(d), C.byref(need)) == 0
         return f.neus2b_layer_norm_backward(C.byref(d), x, xs, g, mean, rstd, dy, dys, skip, ss, dx, dxs, dg, db, mode, FAKE, need.value - short, None)
     for bad in (dict(x=None), dict(g=None), dict(mean=None), dict(rstd=None), dict(dy=None), dict(xs=31), dict(dys=31), dict(skip=FAKE, ss=31), dict(dxs=31),
-                dict(dg=FAKE + 1), dict(mode=5), dict(mean=FAKE + 1), dict(dx=FAKE + 1)):
+                dict(dx=X), dict(dx=DY, dxs=40), dict(skip=DX, ss=40), dict(dg=FAKE + 1), dict(mode=5), dict(mean=FAKE + 1), dict(dx=FAKE + 1)):
         assert bwd(**bad) == INVALID, bad
 
 

@@ -45,7 +45,7 @@ def framed(n, width, t, pad):
 SHAPES = [(1, 1, 1), (1, 16, 16), (2, 7, 5), (1, 4096, 264), (7, 1024, 129), (16, 2048, 64), (17, 48, 64), (33, 333, 77), (64, 520, 1000),
           (65, 128, 256), (128, 64, 128), (129, 1000, 333), (200, 8, 2048), (257, 72, 520), (700, 31, 3), (1000, 4100, 24), (3000, 48, 64),
           (5000, 64, 16), (512, 2048, 1536), (2600, 136, 2100), (9472, 23, 512), (100, 40, 37888), (1500, 128, 40),
-          (1111, 56, 120), (300, 8, 100), (100000, 64, 64)]
+          (1111, 56, 120), (300, 8, 100), (100000, 64, 64), (3, 24, 40000), (50, 7, 38000)]
 
 
 @pytest.mark.parametrize("t", HALF, ids=["f16", "bf16"])
@@ -388,6 +388,52 @@ def test_clip_extreme_and_nonfinite(ops):
     assert ops.GradientSet([z]).clip(1.0).tolist() == [0.0, 1.0]
     v = torch.full((4,), 3.0, device="cuda")
     assert ops.GradientSet([v]).norm(max_norm=1.5, scale=-0.5).tolist() == [3.0, 0.5]
+
+
+def test_tensors_of_another_device_are_refused(ops, monkeypatch):
+    from neus2_b200 import _lib as L
+    x = torch.ones((8, 16), dtype=torch.float16, device="cuda")
+    w, s, g = torch.ones((16, 16), dtype=torch.float16, device="cuda"), torch.ones(8, device="cuda"), torch.ones(16, device="cuda")
+    gset = ops.GradientSet([g])
+    monkeypatch.setattr(ops, "_current_device", lambda: x.get_device() + 1)
+    for call in (lambda: ops.linear_forward(x, w), lambda: ops.linear_backward(x, w, x), lambda: ops.layer_norm_forward(x, g),
+                 lambda: ops.layer_norm_backward(x, g, s, s, x), lambda: ops.GradientSet([g]), lambda: gset.clip(1.0)):
+        with pytest.raises(L.Neus2bError, match="current device"):
+            call()
+
+
+FIRST_CALLS_IN_A_CAPTURE = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from neus2_b200 import ops
+t = torch.float16
+x, w, wide, gamma = (torch.ones(s, dtype=t, device="cuda") for s in ((300, 64), (64, 64), (320, 64), (64,)))
+few, odd = torch.ones((3, 64), dtype=t, device="cuda"), torch.ones((300, 63), dtype=t, device="cuda")
+wodd, grad = torch.ones((40, 63), dtype=t, device="cuda"), torch.ones(1000, device="cuda")
+gset = ops.GradientSet([grad])
+torch.cuda.synchronize()
+g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(g, stream=s):
+    y = ops.linear_forward(x, w, activation=2)
+    out = [y, ops.linear_forward(x, wide), ops.linear_forward(few, w), ops.linear_forward(odd, wodd), *ops.linear_backward(x, w, y), *ops.linear_backward(few, w, few)]
+    h, mean, rstd = ops.layer_norm_forward(x, gamma, want_stats=True)
+    out += [h, *ops.layer_norm_backward(x, gamma, mean, rstd, y), gset.clip(1.0)]
+g.replay()
+torch.cuda.synchronize()
+assert float(y[0, 0]) == 64 and float(out[1][299, 319]) == 64 and float(out[2][2, 0]) == 64 and float(out[3][299, 39]) == 63
+assert float(grad[0]) < 0.04 and all(bool(torch.isfinite(o.float()).all()) for o in out)
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS_IN_A_CAPTURE.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
 
 
 def test_streams_and_graph(ops):
