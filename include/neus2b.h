@@ -389,8 +389,8 @@ typedef struct {
  * NULL, d_residual [n][out_width] or NULL, d_y [n][out_width], d_preact [n][out_width] or NULL: receives z, which the backward
  * pass of an activated layer reads.  The sum and the epilogue are fp32, y and z are rounded once.  d_residual may be d_y (with the
  * same stride).  d_workspace: neus2b_linear_forward_workspace bytes, 16-byte aligned; NULL and 0 where that is 0.  `unaligned`: whether
- * rows of x or W may start off 16-byte boundaries (the address, or the stride, or in_width for W, times 2 bytes): with more than a few
- * samples they are then copied to where they do.  Nothing in a workspace is kept between calls; calls that may run at the same time
+ * rows of x or W may start off 16-byte boundaries (the address, or the stride, or in_width for W, times 2 bytes): they are
+ * then copied to where they do.  Nothing in a workspace is kept between calls; calls that may run at the same time
  * need workspaces of their own. */
 int neus2b_linear_forward_workspace(const neus2b_linear_desc* desc, int unaligned, uint64_t* bytes);
 int neus2b_linear_forward(const neus2b_linear_desc* desc, const void* d_x, uint64_t x_stride, const void* d_w, const void* d_bias,

@@ -51,7 +51,7 @@ extern "C" int neus2b_linear_forward_workspace(const neus2b_linear_desc* desc, i
 	if (bad_desc(desc) || !bytes) return NEUS2B_E_INVALID;
 	if (!is_half_type(desc->dtype)) return NEUS2B_E_UNSUPPORTED;
 	if (too_large(desc)) return NEUS2B_E_TOO_LARGE;
-	*bytes = unaligned && desc->n > kFewSamples ? copy_bytes(desc->n, desc->in_width) + copy_bytes(desc->out_width, desc->in_width) : 0;
+	*bytes = unaligned ? copy_bytes(desc->n, desc->in_width) + copy_bytes(desc->out_width, desc->in_width) : 0;
 	return NEUS2B_OK;
 }
 
@@ -72,7 +72,7 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	Product p{};
 	p.a = d_x, p.a_ld = x_stride, p.b = d_w, p.b_ld = in;
 	p.M = desc->n, p.N = out, p.K = in, p.bf16 = desc->dtype == NEUS2B_BF16;
-	if (desc->n > kFewSamples && !(operand_aligned(p.a, p.a_ld) && operand_aligned(p.b, p.b_ld))) {
+	if (!(operand_aligned(p.a, p.a_ld) && operand_aligned(p.b, p.b_ld))) {
 		if (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need) return NEUS2B_E_INVALID;
 		Operand ops[2];
 		int count = 0;
@@ -153,9 +153,8 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		at += dz_bytes(desc);
 	}
 	const bool params = d_wgrad || d_bgrad;
-	// the input gradient of a few samples reads rows anywhere, the weight gradient does not
-	const bool copy_dz = !operand_aligned(dz, dz_ld) && (params || (d_dL_dx && n > kFewSamples)), copy_x = d_wgrad && !operand_aligned(xs, xs_ld),
-	           copy_w = d_dL_dx && n > kFewSamples && !operand_aligned(ws, ws_ld);
+	const bool copy_dz = !operand_aligned(dz, dz_ld) && (params || d_dL_dx), copy_x = d_wgrad && !operand_aligned(xs, xs_ld),
+	           copy_w = d_dL_dx && !operand_aligned(ws, ws_ld);
 	if (copy_dz || copy_x || copy_w) {
 		if (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need + copies_bytes(desc)) return NEUS2B_E_INVALID;
 		Operand ops[3];

@@ -34,30 +34,6 @@ __device__ __forceinline__ float h2f(uint16_t v, bool bf) { return bf ? __uint_a
 __device__ __forceinline__ uint16_t f2h(float v, bool bf) {
 	return bf ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
-// one sum, sample r, feature c
-__device__ __forceinline__ void finish_one(const Epilogue& e, bool bf, uint64_t r, uint32_t c, float v) {
-	if (e.out_f32) {
-		float* o = (float*)e.out + r * e.out_ld + c;
-		*o = e.accumulate ? *o + v : v;
-		return;
-	}
-	if (e.bias) v += h2f(((const uint16_t*)e.bias)[c], bf);
-	if (e.preact) ((uint16_t*)e.preact)[r * e.preact_ld + c] = f2h(v, bf);
-	v = e.slope_z ? v * act_slope(e.act, h2f(((const uint16_t*)e.slope_z)[r * e.slope_ld + c], bf)) : act_value(e.act, v);
-	if (e.add) v += h2f(((const uint16_t*)e.add)[r * e.add_ld + c], bf);
-	((uint16_t*)e.out)[r * e.out_ld + c] = f2h(v, bf);
-}
-
-// eight fp32 sums of a weight gradient's row, all of them inside and on a 16-byte boundary
-__device__ __forceinline__ void store_eight(const Epilogue& e, uint64_t r, uint32_t c, float (&v)[8]) {
-	float4* o = reinterpret_cast<float4*>((float*)e.out + r * e.out_ld + c);
-	if (e.accumulate) {
-		const float4 a = o[0], b = o[1];
-		v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-	}
-	o[0] = make_float4(v[0], v[1], v[2], v[3]);
-	o[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
 
 // width of the product that carries the column sums where no weight gradient is wanted (it is not stored)
 inline uint32_t sums_only_width(uint32_t out_width) { return out_width < 64u ? out_width : 64u; }
@@ -71,8 +47,7 @@ uint64_t narrow_workspace(uint32_t out_width, uint32_t in_width, uint32_t n);
 int run_narrow(const Product& rows, bool backward, const Product* weights, cudaStream_t stream);
 int read_narrow_error(uint32_t* flags);
 int write_narrow_error(uint32_t flags);
-// Rows on 16-byte boundaries, as the product kernels read them (with up to kFewSamples samples run_product takes any).
-constexpr uint32_t kFewSamples = 64;
+// Rows on 16-byte boundaries, as the product kernels read them.
 struct Operand {
 	const void* from;
 	uint64_t ld;

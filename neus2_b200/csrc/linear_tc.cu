@@ -1,10 +1,12 @@
 // The products of the linear layer on tcgen05: operands in 128-byte-swizzled shared-memory tiles, sums in tensor memory.
 //
-// A CTA computes 128 x BN tiles of sum_k a(m, k) b(n, k), 64 k at a time.  Warps 0-7 take finished sums out of tensor memory and run
-// the epilogue while the MMA warp fills the other accumulator; one warp issues the MMAs; operand tiles are brought in by TMA, or,
-// where rows do not start on 16-byte boundaries, by warps that shift them into place (GATHER).  Both layouts of an operand are
-// read as they lie in memory: [m][k] is a K-major tile (128 rows of 64 k), [k][m] an MN-major one (slabs of 64 k x 64 m), so neither
-// backward product transposes anything.
+// A CTA computes 128 x BN tiles of sum_k a(m, k) b(n, k), 64 k at a time.  One warp brings in operand tiles by TMA, one issues the MMAs,
+// 8 or 16 warps take finished sums out of tensor memory and run the epilogue while the MMA warp fills another accumulator.  Both
+// layouts of an operand are read as they lie in memory: [m][k] is a K-major tile (128 rows of 64 k), [k][m] an MN-major one (slabs of
+// 64 k x 64 m), so neither backward product transposes anything.  Operands whose rows do not start on 16-byte boundaries, which TMA
+// cannot read, are copied once ahead of the product (realign_kernel).
+#include <algorithm>
+
 #include "linear_tc.cuh"
 
 namespace n2b {
@@ -12,7 +14,6 @@ namespace lin {
 
 static __device__ uint32_t g_error;  // bit 0: a bounded wait ran out
 
-constexpr int kGatherWarps = 11;
 constexpr int kChunkBytes = 32 * 64;  // 32 x 32 values on their way between the epilogue and global memory
 constexpr int kChunk = 8;  // weight gradient: k blocks (512 samples) summed in tensor memory before the sum moves to registers
 
@@ -29,35 +30,38 @@ struct alignas(64) Args {
 	Epilogue e;
 };
 
-// One 16-byte unit of an operand tile, eight values that start at any even address of a [rows][cols] matrix: two aligned 16-byte loads and
-// a shift; zeros outside of the matrix.  The loads may reach up to 14 bytes around the values: they are used only where that stays inside
-// the matrix's extent in memory, which is the caller's.
+// Eight values of a row of a [rows][cols] matrix that start at any even address: two aligned 16-byte loads and a shift; zeros behind the
+// row's end.  The loads may reach up to 14 bytes around the values: they are used only where that stays inside the matrix's extent in
+// memory, which is the caller's.
 struct Unit {
 	uint4 lo, hi;
-	uint32_t shift;
+	const uint16_t* p;
+	uint32_t shift, n;
+	bool wide;
 };
+__device__ __noinline__ uint4 unit_by_entries(const uint16_t* p, uint32_t n) {  // at the matrix's two ends
+	uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+	for (uint32_t i = 0; i < 8; ++i)
+		if (i < n) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+	return make_uint4(w[0], w[1], w[2], w[3]);
+}
 __device__ __forceinline__ void unit_fetch(Unit& v, const uint16_t* base, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t row, uint32_t col) {
-	v.lo = v.hi = make_uint4(0, 0, 0, 0);
-	v.shift = 0;
-	if (row >= rows || col >= cols) return;
+	v.n = min(8u, cols - col);
 	const char *begin = reinterpret_cast<const char*>(base), *end = begin + ((uint64_t)(rows - 1) * ld + cols) * 2;
 	const uint16_t* p = base + (uint64_t)row * ld + col;
 	const char* q = reinterpret_cast<const char*>(p);
+	v.p = p;
 	v.shift = (uint32_t)(uintptr_t)q & 15u;
 	const char* down = q - v.shift;
-	if (col + 8 <= cols && down >= begin && down + 32 <= end) {
+	v.wide = down >= begin && down + 32 <= end;
+	if (v.wide) {
 		v.lo = __ldg(reinterpret_cast<const uint4*>(down));
 		v.hi = __ldg(reinterpret_cast<const uint4*>(down) + 1);
-	} else {  // at the matrix's edges: entry by entry
-		uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-		for (int i = 0; i < 8; ++i)
-			if (col + i < cols) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-		v.lo = make_uint4(w[0], w[1], w[2], w[3]);
-		v.shift = 0;
 	}
 }
 __device__ __forceinline__ uint4 unit_value(const Unit& v) {
+	if (!v.wide) return unit_by_entries(v.p, v.n);
 	uint32_t w[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
 	if (v.shift & 8u) {
 #pragma unroll
@@ -68,7 +72,13 @@ __device__ __forceinline__ uint4 unit_value(const Unit& v) {
 		for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
 	}
 	const uint32_t b = (v.shift & 2u) * 8u;
-	return make_uint4(__funnelshift_r(w[0], w[1], b), __funnelshift_r(w[1], w[2], b), __funnelshift_r(w[2], w[3], b), __funnelshift_r(w[3], w[4], b));
+	uint32_t y[4];
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		y[i] = __funnelshift_r(w[i], w[i + 1], b);
+		if (2 * i + 1 >= (int)v.n) y[i] = 2 * i < (int)v.n ? y[i] & 0xffffu : 0u;
+	}
+	return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
 // Copies of up to three matrices with rows on 16-byte boundaries, for operands that have none: thread = 16 bytes of a copy.
@@ -79,38 +89,53 @@ struct Realign {
 	uint32_t rows[3], cols[3];
 	uint64_t units[4];  // first unit of each, and behind the last
 };
-__global__ void __launch_bounds__(256) realign_kernel(const Realign r) {
+constexpr uint32_t kRealign = 2;  // units of a thread that are on their way together
+__global__ void __launch_bounds__(256, 4) realign_kernel(const Realign r) {
 	let_next_start();
 	wait_for_previous();
-	for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < r.units[3]; i += gridDim.x * 256ull) {
-		const int k = i >= r.units[2] ? 2 : i >= r.units[1] ? 1 : 0;
-		const uint64_t u = i - r.units[k];
-		const uint32_t per = (r.cols[k] + 7) / 8, row = (uint32_t)(u / per), col = (uint32_t)(u - (uint64_t)row * per) * 8;
-		Unit v;
-		unit_fetch(v, r.from[k], r.from_ld[k], r.rows[k], r.cols[k], row, col);
-		*reinterpret_cast<uint4*>(r.to[k] + (uint64_t)row * per * 8 + col) = unit_value(v);
+#pragma unroll 1
+	for (int k = 0; k < 3; ++k) {
+		// a thread's units lie a grid's width apart: (row, column) moves on by one division's worth, taken once
+		const uint64_t units = r.units[k + 1] - r.units[k], width = (uint64_t)gridDim.x * 256;
+		uint64_t u = blockIdx.x * 256ull + threadIdx.x;
+		if (u >= units) continue;
+		const uint32_t per = (r.cols[k] + 7) / 8, step_row = (uint32_t)(width / per), step_col = (uint32_t)(width - (uint64_t)step_row * per);
+		uint32_t row = (uint32_t)(u / per), col = (uint32_t)(u - (uint64_t)row * per);
+		while (u < units) {
+			Unit v[kRealign];
+			uint4* to[kRealign];
+#pragma unroll
+			for (uint32_t j = 0; j < kRealign; ++j) {
+				to[j] = u < units ? reinterpret_cast<uint4*>(r.to[k]) + u : nullptr;
+				if (to[j]) unit_fetch(v[j], r.from[k], r.from_ld[k], r.rows[k], r.cols[k], row, col * 8);
+				u += width, row += step_row, col += step_col;
+				if (col >= per) col -= per, ++row;
+			}
+#pragma unroll
+			for (uint32_t j = 0; j < kRealign; ++j)
+				if (to[j]) *to[j] = unit_value(v[j]);
+		}
 	}
 }
 
 // What a block of one variant is made of.  PAIR: two CTAs of a cluster compute a 256 x BN tile together, each with 128 of its rows in its
 // tensor memory and half of B's tile in its shared memory.  The epilogue is a long chain of dependent steps, so that it takes 16 warps to
 // keep up with the MMAs: on wide tiles they share the columns, narrow ones (BN 64) go to four groups in turn, each with an accumulator.
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
+template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool PAIR>
 struct Shape {
-	static_assert(!GATHER || SWAP, "operands of larger products are realigned ahead of them");
 	static constexpr int kBRows = PAIR ? BN / 2 : BN;  // of B's tile in this CTA
 	static constexpr int kABytes = kBM * 128;
 	static constexpr int kBBytes = (BMN && kBRows < 64 ? 64 : kBRows) * 128;
 	static constexpr int kStage = kABytes + kBBytes;
 	static constexpr bool kTurns = BN == 64 && !SWAP && !WGRAD, kMany = !SWAP && !WGRAD && (PAIR || BN <= 128);
-	static constexpr int kHalves = kTurns || GATHER ? 1 : kMany ? 4 : 2, kGroups = kTurns ? 4 : 1, kBufs = kTurns ? 4 : 2;
+	static constexpr int kHalves = kTurns ? 1 : kMany ? 4 : 2, kGroups = kTurns ? 4 : 1, kBufs = kTurns ? 4 : 2;
 	static constexpr int kEpiWarps = 4 * kHalves * kGroups, kMmaWarp = kEpiWarps, kLoadWarp = kEpiWarps + 1;
-	static constexpr int kThreads = (GATHER ? kLoadWarp + kGatherWarps : kLoadWarp + 1) * 32;
+	static constexpr int kThreads = (kLoadWarp + 1) * 32;
 	// Shared memory behind the operand stages: chunks of the epilogue (`chunks` for every warp), ones tile and barriers; alignment of the base.
-	static constexpr int fixed(int chunks) { return (SWAP || WGRAD ? 0 : kEpiWarps * chunks * kChunkBytes) + 2048 + 1024; }
+	static constexpr int fixed(int chunks) { return (SWAP ? 0 : kEpiWarps * (WGRAD ? 4096 : chunks * kChunkBytes)) + 2048 + 1024; }
 	static constexpr int stages(int chunks) {
 		// few samples: room for a second CTA on the SM
-		const int room = ((SWAP && !GATHER ? kSmemMost / 2 - 1024 : kSmemMost) - fixed(chunks)) / kStage;
+		const int room = ((SWAP ? kSmemMost / 2 - 1024 : kSmemMost) - fixed(chunks)) / kStage;
 		return room < kMaxStages ? room : kMaxStages;
 	}
 	static constexpr int kCols = kBufs * BN + (WGRAD && !PAIR ? 32 : 0);
@@ -133,10 +158,13 @@ __device__ __forceinline__ void chunk_fetch(uint32_t chunk, const void* base, ui
 				asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(chunk + unit_at(i * 8 + (lane >> 2), lane & 3)), "l"(q) : "memory");
 	} else {
 		const uint16_t* q = p + (uint64_t)row0 * ld + col0 + lane;
-#pragma unroll 8
-		for (int i = 0; i < 32; ++i, q += ld) {
-			const uint16_t v = row0 + i < rows && col0 + lane < cols ? *q : (uint16_t)0;
-			asm volatile("st.shared.u16 [%0], %1;" ::"r"(chunk + unit_at(i, lane >> 3) + (lane & 7) * 2), "h"(v) : "memory");
+#pragma unroll
+		for (int h = 0; h < 32; h += 16) {  // 16 on their way together
+			uint16_t v[16];
+#pragma unroll
+			for (int i = 0; i < 16; ++i, q += ld) v[i] = row0 + h + i < rows && col0 + lane < cols ? *q : (uint16_t)0;
+#pragma unroll
+			for (int i = 0; i < 16; ++i) asm volatile("st.shared.u16 [%0], %1;" ::"r"(chunk + unit_at(h + i, lane >> 3) + (lane & 7) * 2), "h"(v[i]) : "memory");
 		}
 	}
 }
@@ -173,9 +201,47 @@ __device__ __forceinline__ void chunk_store(const uint32_t (&row)[16], void* bas
 		}
 	}
 }
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
-__global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>::kThreads, SWAP && !GATHER ? 2 : 1) product_kernel(const __grid_constant__ Args p) {
-	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
+// 32 x 32 fp32 sums of a weight gradient, a row a thread, to global memory in row segments (128 bytes) through 4 KB of a warp: written
+// a row a thread they would take 32 accesses of a few bytes an instruction (8 us a tile where rows are unaligned).
+__device__ __forceinline__ void sums_store(const float (&v)[32], const Epilogue& e, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols, unsigned char* chunk,
+                                           int lane) {
+	__syncwarp();  // what was here before has been read
+#pragma unroll
+	for (int u = 0; u < 8; ++u)
+		*reinterpret_cast<float4*>(chunk + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+	__syncwarp();
+	if (e.vec && col0 + 32 <= cols) {
+		float* o = (float*)e.out + (uint64_t)(row0 + (lane >> 3)) * e.out_ld + col0 + (lane & 7) * 4;
+#pragma unroll 4
+		for (int r = lane >> 3; r < 32; r += 4, o += 4 * e.out_ld) {
+			float4 s = *reinterpret_cast<const float4*>(chunk + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+			if (row0 + r >= rows) continue;
+			if (e.accumulate) {
+				const float4 a = *reinterpret_cast<const float4*>(o);
+				s.x += a.x, s.y += a.y, s.z += a.z, s.w += a.w;
+			}
+			*reinterpret_cast<float4*>(o) = s;
+		}
+	} else {
+		float* o = (float*)e.out + (uint64_t)row0 * e.out_ld + col0 + lane;
+#pragma unroll 8
+		for (int r = 0; r < 32; ++r, o += e.out_ld) {
+			const float s = *reinterpret_cast<const float*>(chunk + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+			if (row0 + r < rows && col0 + lane < cols) *o = e.accumulate ? *o + s : s;
+		}
+	}
+}
+
+// Place of sum (m, n) of a tile in shared memory.  Features are contiguous, as they are in the result: what a warp reads of another
+// CTA's tile has to be (spread over 32 lines it takes 8 us instead of 1.5).
+template <int BN, bool SWAP>
+__device__ __forceinline__ uint32_t joined_at(uint32_t m, uint32_t n) {
+	return SWAP ? n * (kBM + 1) + m : m * (BN + 1) + n;
+}
+
+template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool PAIR>
+__global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThreads, SWAP ? 2 : 1) product_kernel(const __grid_constant__ Args p) {
+	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>;
 	extern __shared__ unsigned char smem_raw[];
 	unsigned char* smem = smem_raw + ((1024u - (sptr(smem_raw) & 1023u)) & 1023u);
 	const uint32_t stages = p.stages;
@@ -190,7 +256,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 
 	if (tid == 0) {
 		for (uint32_t i = 0; i < stages; ++i) {
-			tc::mbar_init(full + 8 * i, GATHER ? kGatherWarps * 32 : 1);
+			tc::mbar_init(full + 8 * i, 1);
 			tc::mbar_init(empty + 8 * i, 1);
 		}
 		for (int i = 0; i < S::kBufs; ++i) {
@@ -211,11 +277,12 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	let_next_start();     // (the next kernel's blocks may take tensor memory: only now that this one has its own)
 	wait_for_previous();  // the set-up above runs beside the end of the kernel ahead
 
-	// A cluster that splits k computes one tile; a pair, or a CTA by itself, takes every `step`-th.
+	// With few samples, or where a cluster splits k, a CTA computes one tile; otherwise a pair, or a CTA by itself, takes every `step`-th.
 	const uint32_t tiles = p.tiles_m * p.tiles_n, kblocks = (p.K + kBK - 1) / kBK;
 	const uint32_t first = PAIR ? blockIdx.x / 2 : p.cluster > 1 ? (blockIdx.x / p.cluster) + rank * tiles : blockIdx.x;
 	const uint32_t units = tiles * p.splits;
-	const uint32_t step = PAIR ? gridDim.x / 2 : p.cluster > 1 ? units : gridDim.x;
+	const bool single = !WGRAD && !PAIR && (SWAP || p.cluster > 1);
+	const uint32_t step = PAIR ? gridDim.x / 2 : single ? units : gridDim.x;
 	const uint32_t row_offset = PAIR ? rank * kBM : 0u;
 	constexpr int kTileM = PAIR ? 2 * kBM : kBM;
 	bool ok = true;
@@ -231,45 +298,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 		kb1 = (uint32_t)((uint64_t)(split + 1) * kblocks / p.splits);
 	};
 
-	if (GATHER && warp >= S::kLoadWarp) {
-		// ---------------------------------------------------------------- operand tiles, rows anywhere: the next tile's units are on their way
-		// while this one's are put into place
-		constexpr int kUnits = (kBM + BN) * 8, kEach = (kUnits + kGatherWarps * 32 - 1) / (kGatherWarps * 32);
-		const int t = tid - S::kLoadWarp * 32;
-		uint32_t stage = 0, phase = 0;
-		for (uint32_t u = first; u < units && ok; u += step) {
-			uint32_t mt, nt, split, kb0, kb1;
-			locate(u, mt, nt, split, kb0, kb1);
-			Unit now[kEach], next[kEach];
-			auto fetch = [&](Unit (&v)[kEach], uint32_t kb) {
-#pragma unroll
-				for (int j = 0; j < kEach; ++j) {
-					const int i = t + j * kGatherWarps * 32, r = i >> 3, c = (i & 7) * 8;
-					if (i >= kUnits) break;
-					if (r >= kBM) unit_fetch(v[j], p.b, p.b_ld, p.N, p.K, nt * BN + (r - kBM), kb * kBK + c);
-					else if (AMN) unit_fetch(v[j], p.a, p.a_ld, p.K, p.M, kb * kBK + (r & 63), mt * kBM + (r & 64) + c);
-					else unit_fetch(v[j], p.a, p.a_ld, p.M, p.K, mt * kBM + r, kb * kBK + c);
-				}
-			};
-			fetch(now, kb0);
-			for (uint32_t kb = kb0; kb < kb1; ++kb) {
-				ok = wait_phase(empty + 8 * stage, phase ^ 1u);
-				if (!ok) break;
-				if (kb + 1 < kb1) fetch(next, kb + 1);
-				unsigned char* const sa = smem + stage * S::kStage;  // A's 128 rows and B's behind them
-#pragma unroll
-				for (int j = 0; j < kEach; ++j) {
-					const int i = t + j * kGatherWarps * 32, r = i >> 3;
-					if (i < kUnits) *reinterpret_cast<uint4*>(sa + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = unit_value(now[j]);
-					now[j] = next[j];
-				}
-				tc::fence_async_smem();
-				arrive(full + 8 * stage);
-				if (++stage == stages) stage = 0, phase ^= 1u;
-			}
-		}
-		__syncwarp();
-	} else if (warp >= S::kLoadWarp) {
+	if (warp >= S::kLoadWarp) {
 		// ---------------------------------------------------------------- operand tiles by TMA, one thread
 		uint32_t stage = 0, phase = 0;
 		const uint32_t full_lead = PAIR ? peer_address(full, 0) : full;  // a pair's tiles are counted in by the first CTA
@@ -410,55 +439,38 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 					next_buf();
 				}
 				if (!ok) break;
-				if (m < p.M) {
-					Epilogue e = p.e;
-					if (p.splits > 1) {
-						e.out = p.partial + (uint64_t)split * p.M * p.N;
-						e.out_ld = p.N;
-						e.accumulate = 0;
-						e.vec = (p.N & 3u) == 0;
-					}
-#pragma unroll
-					for (int c = 0; c < kCols; c += 8) {
-						if (!p.e.out) break;
-						float v[8];
-#pragma unroll
-						for (int i = 0; i < 8; ++i) v[i] = acc[c + i];
-						if (e.vec && n0 + c + 8 <= p.N) {
-							store_eight(e, m, n0 + c, v);
-						} else {
-#pragma unroll
-							for (int i = 0; i < 8; ++i)
-								if (n0 + c + i < p.N) finish_one(e, bf, m, n0 + c + i, v[i]);
-						}
-					}
-					if (sums) {
-						if (p.splits > 1) p.partial[(uint64_t)p.splits * p.M * p.N + (uint64_t)split * p.M + m] = sum;
-						else p.column_sums[m] = p.e.accumulate ? p.column_sums[m] + sum : sum;
-					}
+				Epilogue e = p.e;
+				if (p.splits > 1) {
+					e.out = p.partial + (uint64_t)split * p.M * p.N;
+					e.out_ld = p.N;
+					e.accumulate = 0;
+					e.vec = (p.N & 3u) == 0;
 				}
-			} else if (SWAP || p.cluster > 1) {
+#pragma unroll
+				for (int c = 0; c < kCols; c += 32) {
+					if (!p.e.out || n0 + c >= p.N) break;
+					float v[32];
+#pragma unroll
+					for (int i = 0; i < 32; ++i) v[i] = acc[c + i];
+					sums_store(v, e, row0, p.M, n0 + c, p.N, chunks + warp * 4096, lane);
+				}
+				if (sums && m < p.M) {
+					if (p.splits > 1) p.partial[(uint64_t)p.splits * p.M * p.N + (uint64_t)split * p.M + m] = sum;
+					else p.column_sums[m] = p.e.accumulate ? p.column_sums[m] + sum : sum;
+				}
+			} else if (single) {
 				ok = wait_phase(tfull + 8 * buf, buf_phase);
 				if (!ok) break;
 				tc::fence_after_sync();
-				float* joined = reinterpret_cast<float*>(smem);  // cluster: [BN][129]; every tile of this CTA's only unit has been consumed
+				float* joined = reinterpret_cast<float*>(smem);  // every operand tile of this CTA's only unit has been consumed
 #pragma unroll 1
-				for (int c = 0; c < kCols; c += 16) {
+				for (uint32_t c = half * kCols; c < (half + 1) * kCols && nt * BN + c < p.N; c += 16) {
 					uint32_t r[16];
-					tmem_ld16_raw(lanes + buf * BN + half * kCols + c, r);
+					tmem_ld16_raw(lanes + buf * BN + c, r);
 					tmem_wait16(r);
-					if (p.cluster > 1) {
 #pragma unroll
-						for (int i = 0; i < 16; ++i) joined[(half * kCols + c + i) * 129 + q * 32 + lane] = __uint_as_float(r[i]);
-					} else {
-						// m is the feature, the tile's columns are samples
-#pragma unroll
-						for (int i = 0; i < 16; ++i)
-							if (m < p.M && n0 + c + i < p.N) finish_one(p.e, bf, n0 + c + i, m, __uint_as_float(r[i]));
-					}
+					for (int i = 0; i < 16; ++i) joined[joined_at<BN, SWAP>(q * 32 + lane, c + i)] = __uint_as_float(r[i]);
 				}
-				release();
-				next_buf();
 			} else {
 				const Epilogue& e = p.e;
 				// the inputs' next 32 columns are on their way while the sums are still being computed
@@ -498,10 +510,10 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 									v[8 * i + 2 * j + 1] += f.y;
 								}
 							}
-						} else {
+						} else {  // a column a thread, handed round
+							const float mine = col + lane < p.N ? h2f(b[col + lane], bf) : 0.f;
 #pragma unroll
-							for (int i = 0; i < 32; ++i)
-								if (col + i < p.N) v[i] += h2f(b[col + i], bf);
+							for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, mine, i);
 						}
 					}
 					if (e.preact) {
@@ -548,24 +560,57 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 		}
 	}
 	if (!ok) atomicOr(&g_error, 1u);
-	if (!WGRAD && !PAIR && p.cluster > 1) {
-		// every CTA adds up its share of the tile over the cluster's partial sums, in rank order, and finishes it
+	if (single) {
+		// every CTA adds up its share of the tile over the cluster's sums, in rank order, and finishes it: two entries at a time, whose
+		// inputs are on their way together
 		__syncwarp();
-		cluster_sync();
+		if (p.cluster > 1) cluster_sync();
+		else __syncthreads();
 		uint32_t mt, nt, split, kb0, kb1;
 		locate(first, mt, nt, split, kb0, kb1);
-		const uint32_t joined = sptr(smem), count = kBM * BN / p.cluster;
-		for (uint32_t i = tid; i < count; i += S::kThreads) {
-			const uint32_t idx = rank * count + i;
-			const uint32_t m = SWAP ? idx % kBM : idx / BN, n = SWAP ? idx / kBM : idx % BN;
-			if (mt * kBM + m >= p.M || nt * BN + n >= p.N) continue;
-			float v = 0.f;
-			for (uint32_t s = 0; s < p.cluster; ++s) v += load_peer(joined + (n * 129 + m) * 4, s);
-			if (SWAP) finish_one(p.e, bf, nt * BN + n, mt * kBM + m, v);
-			else finish_one(p.e, bf, mt * kBM + m, nt * BN + n, v);
+		const uint32_t joined = sptr(smem), rows = min((uint32_t)kBM, p.M - mt * kBM), cols = min((uint32_t)BN, p.N - nt * BN);
+		const uint32_t count = rows * cols, stride = p.cluster * S::kThreads;
+		const Epilogue& e = p.e;
+		for (uint32_t base = rank * S::kThreads + tid; base < count; base += 2 * stride) {
+			float v[2];
+			uint32_t at[2], feature[2];
+			uint64_t sample[2];
+			bool in[2];
+			uint16_t z[2], add[2], bias[2];
+#pragma unroll
+			for (int k = 0; k < 2; ++k) {
+				const uint32_t idx = base + k * stride, slow = idx / (SWAP ? rows : cols), fast = idx - slow * (SWAP ? rows : cols);
+				const uint32_t m = SWAP ? fast : slow, n = SWAP ? slow : fast;
+				in[k] = idx < count;
+				at[k] = in[k] ? joined + joined_at<BN, SWAP>(m, n) * 4 : joined;
+				feature[k] = SWAP ? mt * kBM + m : nt * BN + n;
+				sample[k] = SWAP ? nt * BN + n : mt * kBM + m;
+				v[k] = 0.f;
+				z[k] = add[k] = bias[k] = 0;
+				if (in[k] && e.bias) bias[k] = ((const uint16_t*)e.bias)[feature[k]];
+				if (in[k] && e.slope_z) z[k] = ((const uint16_t*)e.slope_z)[sample[k] * e.slope_ld + feature[k]];
+				if (in[k] && e.add) add[k] = ((const uint16_t*)e.add)[sample[k] * e.add_ld + feature[k]];
+			}
+			if (p.cluster > 1) {
+				for (uint32_t s = 0; s < p.cluster; ++s)
+#pragma unroll
+					for (int k = 0; k < 2; ++k) v[k] += load_peer(at[k], s);
+			} else {
+#pragma unroll
+				for (int k = 0; k < 2; ++k) v[k] = load_peer(at[k], 0);
+			}
+#pragma unroll
+			for (int k = 0; k < 2; ++k) {
+				if (!in[k]) continue;
+				float y = v[k] + (e.bias ? h2f(bias[k], bf) : 0.f);
+				if (e.preact) ((uint16_t*)e.preact)[sample[k] * e.preact_ld + feature[k]] = f2h(y, bf);
+				y = e.slope_z ? y * act_slope(e.act, h2f(z[k], bf)) : act_value(e.act, y);
+				if (e.add) y += h2f(add[k], bf);
+				((uint16_t*)e.out)[sample[k] * e.out_ld + feature[k]] = f2h(y, bf);
+			}
 		}
 		__syncwarp();
-		cluster_sync();
+		if (p.cluster > 1) cluster_sync();
 	}
 	tc::fence_before_sync();
 	__syncwarp();
@@ -575,39 +620,64 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>
 	if (warp == 0) tmem_dealloc<PAIR>(tmem, S::kTmem);
 }
 
-// Sums of the splits' parts.  A block takes 32 neighbouring entries; its 8 or 32 rows of threads share the splits and are joined in order.
-template <int ROWS>
-__global__ void __launch_bounds__(32 * ROWS) join_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, float* __restrict__ out,
-                                                         float* __restrict__ sums, int accumulate) {
-	__shared__ float s[ROWS][33];
+// Sums of the splits' parts.  A thread takes VEC neighbouring entries; the rows of a block's threads share the splits and are joined in
+// order.
+template <int VEC>
+__global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, float* __restrict__ out,
+                                                    float* __restrict__ sums, int accumulate) {
+	extern __shared__ float s[];  // [blockDim.y][VEC][blockDim.x]
 	wait_for_previous();
-	const uint64_t n = (uint64_t)M * N, total = n + (sums ? M : 0), i = (out ? 0 : n) + blockIdx.x * 32ull + threadIdx.x;
-	const bool is_sum = i >= n;
-	float v = 0.f;
-	if (i < total) {
-		const float* q = is_sum ? partial + splits * n + (i - n) : partial + i;
-		const uint64_t pitch = is_sum ? M : n;
+	const uint64_t n = (uint64_t)M * N, groups = n / VEC, first = out ? 0 : groups, total = groups + (sums ? M : 0);
+	for (uint64_t base = first + (uint64_t)blockIdx.x * blockDim.x; base < total; base += (uint64_t)gridDim.x * blockDim.x) {
+		const uint64_t i = base + threadIdx.x;
+		const bool is_sum = i >= groups;
+		float v[VEC] = {};
+		if (i < total) {
+			if (is_sum) {
+				const float* q = partial + splits * n + (i - groups);
 #pragma unroll 4
-		for (uint32_t k = threadIdx.y; k < splits; k += ROWS) v += q[k * pitch];
-	}
-	s[threadIdx.y][threadIdx.x] = v;
-	__syncthreads();
-	if (threadIdx.y == 0 && i < total) {
+				for (uint32_t k = threadIdx.y; k < splits; k += blockDim.y) v[0] += q[(uint64_t)k * M];
+			} else if (VEC == 4) {
+				const float4* q = reinterpret_cast<const float4*>(partial) + i;
+#pragma unroll 4
+				for (uint32_t k = threadIdx.y; k < splits; k += blockDim.y) {
+					const float4 a = q[k * groups];
+					v[0] += a.x, v[1 % VEC] += a.y, v[2 % VEC] += a.z, v[3 % VEC] += a.w;
+				}
+			} else {
+#pragma unroll 4
+				for (uint32_t k = threadIdx.y; k < splits; k += blockDim.y) v[0] += partial[k * n + i];
+			}
+		}
+		if (blockDim.y > 1) {
 #pragma unroll
-		for (int k = 1; k < ROWS; ++k) v += s[k][threadIdx.x];
-		float* o = is_sum ? sums + (i - n) : out + i;
-		*o = accumulate ? *o + v : v;
+			for (int e = 0; e < VEC; ++e) s[(threadIdx.y * VEC + e) * blockDim.x + threadIdx.x] = v[e];
+			__syncthreads();
+			if (threadIdx.y == 0)
+				for (uint32_t k = 1; k < blockDim.y; ++k)
+#pragma unroll
+					for (int e = 0; e < VEC; ++e) v[e] += s[(k * VEC + e) * blockDim.x + threadIdx.x];
+			__syncthreads();
+		}
+		if (threadIdx.y == 0 && i < total) {
+			if (VEC == 4 && !is_sum) {
+				float4* o = reinterpret_cast<float4*>(out) + i;
+				const float4 a = accumulate ? *o : make_float4(0.f, 0.f, 0.f, 0.f);
+				*o = make_float4(a.x + v[0], a.y + v[1 % VEC], a.z + v[2 % VEC], a.w + v[3 % VEC]);
+			} else {
+				float* o = is_sum ? sums + (i - groups) : out + i;
+				*o = accumulate ? *o + v[0] : v[0];
+			}
+		}
 	}
 }
 
-template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool GATHER, bool PAIR>
+template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool PAIR>
 static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
-	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
-	auto kernel = product_kernel<BN, AMN, BMN, SWAP, WGRAD, GATHER, PAIR>;
-	if (!GATHER) {
-		if (int rc = AMN ? make_map(&a.ta, a.a, a.a_ld, a.K, a.M, 64, a.bf16) : make_map(&a.ta, a.a, a.a_ld, a.M, a.K, kBM, a.bf16)) return rc;
-		if (int rc = BMN ? make_map(&a.tb, a.b, a.b_ld, a.K, a.N, 64, a.bf16) : make_map(&a.tb, a.b, a.b_ld, a.N, a.K, S::kBRows, a.bf16)) return rc;
-	}
+	using S = Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>;
+	auto kernel = product_kernel<BN, AMN, BMN, SWAP, WGRAD, PAIR>;
+	if (int rc = AMN ? make_map(&a.ta, a.a, a.a_ld, a.K, a.M, 64, a.bf16) : make_map(&a.ta, a.a, a.a_ld, a.M, a.K, kBM, a.bf16)) return rc;
+	if (int rc = BMN ? make_map(&a.tb, a.b, a.b_ld, a.K, a.N, 64, a.bf16) : make_map(&a.tb, a.b, a.b_ld, a.N, a.K, S::kBRows, a.bf16)) return rc;
 	// one chunk for every epilogue input, and one for z where it does not go the same way as the result
 	a.chunks = (a.e.slope_z && a.e.add) || (a.e.preact && a.e.add) ? 2 : 1;
 	a.stages = S::stages((int)a.chunks);
@@ -632,11 +702,16 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 	return NEUS2B_OK;
 }
 
-// over how many CTAs of a cluster a tile's sum is split: as many as the SMs can take (`each` at a time), with at least four steps of 64 for each
-static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks, uint32_t each) {
-	uint32_t c = 1;
-	while (c < 8 && tiles * c * 2 <= (uint64_t)kSMs * each && kblocks >= c * 2 * 4) c *= 2;
-	return c;
+// Over how many CTAs of a cluster a tile's sum is split: as many as run at one time.  A cluster lies within a GPC, so that fewer SMs can
+// be used the larger it is (cudaOccupancyMaxActiveClusters with one and two CTAs on an SM); one cluster too many takes the time of a
+// second round.  Splitting pays from so many steps of 64 on: with few samples from two for each CTA; with 128 samples a tile the join
+// takes 3 us where two CTAs share it and 1.5 where eight do (100 samples, 512 -> 512: 7.4 us over clusters, 8.0 without; 1000 samples: 9.7
+// over clusters of two, 8.6 without).
+static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks, bool swap) {
+	constexpr uint32_t kFit[2][3] = {{148, 132, 120}, {296, 284, 264}}, kSteps[2][3] = {{16, 8, 16}, {4, 8, 16}};
+	for (int c = 2; c >= 0; --c)
+		if ((tiles << (c + 1)) <= kFit[swap][c] && kblocks >= kSteps[swap][c]) return 2u << c;
+	return 1;
 }
 
 template <bool BMN>
@@ -647,30 +722,27 @@ static int product_of(const Product& p, cudaStream_t stream) {
 	a.e = p.e;
 	a.splits = a.cluster = 1;
 	const uint32_t kblocks = tiles_of(p.K, kBK);
-	// grid of one-CTA tiles; may_split: the kernel can join a cluster's parts
-	auto grid = [&](uint32_t bn, bool may_split, uint32_t each) -> uint32_t {
+	// grid of one-CTA tiles
+	auto grid = [&](uint32_t bn, bool swap) -> uint32_t {
 		a.tiles_m = tiles_of(a.M, kBM);
 		a.tiles_n = tiles_of(a.N, bn);
 		const uint64_t tiles = (uint64_t)a.tiles_m * a.tiles_n;
 		if (tiles >= (1ull << 31)) return 0;
-		a.cluster = a.splits = may_split ? cluster_for(tiles, kblocks, each) : 1u;
-		return (uint32_t)(a.cluster > 1 ? tiles * a.cluster : tiles < (uint64_t)kSMs * each ? tiles : (uint64_t)kSMs * each);
+		a.cluster = a.splits = bn <= 128 ? cluster_for(tiles, kblocks, swap) : 1u;
+		return (uint32_t)(swap || tiles < kSMs ? tiles * a.cluster : kSMs);
 	};
-#define N2B_GO(BN, AMN, BMN_, SWAP, GATHER)                                                          \
-	do {                                                                                             \
-		const uint32_t ctas = grid(BN, BN <= 128, SWAP && !GATHER ? 2 : 1);                                       \
-		if (!ctas) return NEUS2B_E_TOO_LARGE;                                                        \
-		return launch<BN, AMN, BMN_, SWAP, false, GATHER, false>(a, ctas, stream);                   \
+#define N2B_GO(BN, AMN, BMN_, SWAP)                                         \
+	do {                                                                    \
+		const uint32_t ctas = grid(BN, SWAP);                               \
+		if (!ctas) return NEUS2B_E_TOO_LARGE;                               \
+		return launch<BN, AMN, BMN_, SWAP, false, false>(a, ctas, stream);  \
 	} while (0)
 	if (p.M <= 64) {
 		// few samples: the weights are the 128-row operand, the samples its columns
 		a.a = (const uint16_t*)p.b, a.a_ld = p.b_ld, a.M = p.N;
 		a.b = (const uint16_t*)p.a, a.b_ld = p.a_ld, a.N = p.M;
-		const bool tma = tma_ok(p.a, p.a_ld) && tma_ok(p.b, p.b_ld);
-		if (p.M <= 32 && tma) N2B_GO(32, BMN, false, true, false);
-		if (p.M <= 32) N2B_GO(32, BMN, false, true, true);
-		if (tma) N2B_GO(64, BMN, false, true, false);
-		N2B_GO(64, BMN, false, true, true);
+		if (p.M <= 32) N2B_GO(32, BMN, false, true);
+		N2B_GO(64, BMN, false, true);
 	}
 	a.a = (const uint16_t*)p.a, a.a_ld = p.a_ld, a.M = p.M;
 	a.b = (const uint16_t*)p.b, a.b_ld = p.b_ld, a.N = p.N;
@@ -684,22 +756,23 @@ static int product_of(const Product& p, cudaStream_t stream) {
 		a.tiles_m = tiles_of(a.M, 2 * kBM);
 		a.tiles_n = tiles_of(a.N, 256);
 		if (pairs >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
-		return launch<256, false, BMN, false, false, false, true>(a, 2 * (uint32_t)(pairs < kSMs / 2 ? pairs : kSMs / 2), stream);
+		return launch<256, false, BMN, false, false, true>(a, 2 * (uint32_t)(pairs < kSMs / 2 ? pairs : kSMs / 2), stream);
 	}
-	if (c256 < c128 && c256 < c64) N2B_GO(256, false, BMN, false, false);
-	if (c128 < c64) N2B_GO(128, false, BMN, false, false);
-	N2B_GO(64, false, BMN, false, false);
+	if (c256 < c128 && c256 < c64) N2B_GO(256, false, BMN, false);
+	if (c128 < c64) N2B_GO(128, false, BMN, false);
+	N2B_GO(64, false, BMN, false);
 #undef N2B_GO
 }
 
 // Weight gradient: tiles of out_width x in_width, k the samples.  Few tiles share the samples out over the SMs and are joined afterwards.
 // One CTA's 128 x 128 tile takes about 430 cycles for 64 samples (its operands' way through shared memory), a pair's 256 x 256 tile 512
-// (its MMAs); the plan with the fewest cycles is taken.
+// (its MMAs) and, where the column sums are wanted, the pass over dz that takes them and its join: 6 us and 4 TB/s.  The plan with the
+// fewest cycles is taken.
 struct WgradPlan {
 	bool pair;
 	uint32_t tiles_m, tiles_n, splits;
 };
-static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair) {  // (a pair's kernel always stores the product)
+static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair, bool sums) {  // (a pair's kernel always stores the product)
 	const uint32_t kblocks = tiles_of(K, kBK);
 	uint64_t best = 0;
 	WgradPlan plan{};
@@ -707,7 +780,7 @@ static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair) {
 		const uint32_t size = pair ? 256 : 128, slots = pair ? kSMs / 2 : kSMs;
 		const uint64_t tiles = (uint64_t)tiles_of(M, size) * tiles_of(N, size), fill = slots / tiles, most = kblocks / kChunk;
 		const uint64_t splits = fill < most ? (fill ? fill : 1) : (most ? most : 1);
-		const uint64_t cycles = (tiles * splits + slots - 1) / slots * ((kblocks + splits - 1) / splits) * (pair ? 512 : 430);
+		const uint64_t cycles = (tiles * splits + slots - 1) / slots * ((kblocks + splits - 1) / splits) * (pair ? 512 : 430) + (pair && sums ? 11000 + (uint64_t)K * M / 1000 : 0);
 		if (!pair || cycles < best) {
 			best = cycles;
 			plan = WgradPlan{pair != 0, tiles_of(M, size), tiles_of(N, size), (uint32_t)splits};
@@ -788,7 +861,7 @@ int run_realign(const Operand* ops, int count, cudaStream_t stream) {
 		r.units[k + 1] += (uint64_t)ops[k].rows * ((ops[k].cols + 7) / 8);
 	}
 	const uint64_t blocks = (r.units[3] + 255) / 256;
-	return launch_behind(realign_kernel, (uint32_t)(blocks < 16ull * kSMs ? blocks : 16 * kSMs), 256, 0, stream, r);
+	return launch_behind(realign_kernel, (uint32_t)(blocks < 4ull * kSMs ? blocks : 4 * kSMs), 256, 0, stream, r);
 }
 
 int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product_of<true>(p, stream) : product_of<false>(p, stream); }
@@ -796,19 +869,27 @@ int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product
 uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {
 	// whether the product or the column sums alone are wanted is not known here
 	const uint32_t alone = sums_only_width(out_width);
-	const uint64_t product = plan_bytes(wgrad_plan(out_width, in_width, n, true), out_width, in_width), sums = plan_bytes(wgrad_plan(out_width, alone, n, false), out_width, alone);
-	return product > sums ? product : sums;
+	const uint64_t bytes[3] = {plan_bytes(wgrad_plan(out_width, in_width, n, true, false), out_width, in_width),
+	                           plan_bytes(wgrad_plan(out_width, in_width, n, true, true), out_width, in_width),
+	                           plan_bytes(wgrad_plan(out_width, alone, n, false, true), out_width, alone)};
+	return std::max(std::max(bytes[0], bytes[1]), bytes[2]);
 }
 
 int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
-	const uint64_t entries = (out ? (uint64_t)M * N : 0) + (sums ? M : 0);
-	const uint32_t blocks = (uint32_t)((entries + 31) / 32);
-	if (splits >= 32) return launch_behind(join_kernel<32>, blocks, dim3(32, 32), 0, stream, partial, splits, M, N, out, sums, accumulate);
-	return launch_behind(join_kernel<8>, blocks, dim3(32, 8), 0, stream, partial, splits, M, N, out, sums, accumulate);
+	const uint64_t n = (uint64_t)M * N;
+	const bool vec = n % 4 == 0 && (((uintptr_t)partial | (uintptr_t)out) & 15u) == 0;
+	const uint64_t threads = (out ? (vec ? n / 4 : n) : 0) + (sums ? M : 0);
+	// threads for every part where the entries alone do not fill the SMs
+	const uint32_t rows = threads >= 512ull * kSMs || splits == 1 ? 1 : splits >= 32 && threads < 64ull * kSMs ? 32 : 8;
+	const dim3 block(rows == 1 ? 256 : 32, rows);
+	const uint64_t blocks = (threads + block.x - 1) / block.x, most = (uint64_t)kSMs * (rows == 32 ? 2 : 8);
+	const uint32_t grid = (uint32_t)(blocks < most ? blocks : most);
+	if (vec) return launch_behind(join_kernel<4>, grid, block, rows == 1 ? 0 : block.x * rows * 16, stream, partial, splits, M, N, out, sums, accumulate);
+	return launch_behind(join_kernel<1>, grid, block, rows == 1 ? 0 : block.x * rows * 4, stream, partial, splits, M, N, out, sums, accumulate);
 }
 
 int run_weight_gradient(const Product& p, cudaStream_t stream) {
-	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, p.e.out != nullptr);
+	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, p.e.out != nullptr, p.column_sums != nullptr);
 	if (p.workspace_bytes < plan_bytes(w, p.M, p.N)) return NEUS2B_E_INVALID;
 	Args a{};
 	a.bf16 = p.bf16;
@@ -830,13 +911,13 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 			if (int rc = run_join((const float*)p.workspace, by, p.M, 0, nullptr, p.column_sums, p.e.accumulate, stream)) return rc;
 		}
 		const uint32_t pairs = (uint32_t)(units < (uint64_t)(kSMs / 2) ? units : kSMs / 2);
-		if (int rc = launch<256, true, true, false, true, false, true>(a, 2 * pairs, stream)) return rc;
+		if (int rc = launch<256, true, true, false, true, true>(a, 2 * pairs, stream)) return rc;
 		return w.splits > 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, nullptr, p.e.accumulate, stream) : NEUS2B_OK;
 	}
 	a.column_sums = p.column_sums;
 	a.want_sums = p.column_sums != nullptr;
 	const uint32_t ctas = (uint32_t)(units < (uint64_t)kSMs ? units : kSMs);
-	if (int rc = launch<128, true, true, false, true, false, false>(a, ctas, stream)) return rc;
+	if (int rc = launch<128, true, true, false, true, false>(a, ctas, stream)) return rc;
 	return w.splits > 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate, stream) : NEUS2B_OK;
 }
 
