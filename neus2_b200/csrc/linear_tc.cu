@@ -30,14 +30,15 @@ struct alignas(64) Args {
 	Epilogue e;
 };
 
-// Eight values of a row of a [rows][cols] matrix that start at any even address: two aligned 16-byte loads and a shift; zeros behind the
-// row's end.  The loads may reach up to 14 bytes around the values: they are used only where that stays inside the matrix's extent in
-// memory, which is the caller's.
-struct Unit {
-	uint4 lo, hi;
-	const uint16_t* p;
-	uint32_t shift, n;
-	bool wide;
+// Copies of up to three matrices with rows on 16-byte boundaries, for operands that have none.  A thread's unit is 16 bytes of a copy, eight
+// values that start at any even address: two aligned 16-byte reads and a shift, zeros behind the row's end.  The reads may reach up to
+// 14 bytes around the values: they are used only where that stays inside the matrix's extent in memory, which is the caller's.
+struct Realign {
+	const uint16_t* from[3];
+	uint64_t from_ld[3];
+	uint16_t* to[3];
+	uint32_t rows[3], cols[3];
+	uint32_t blocks[4];  // first block of each, and behind the last
 };
 __device__ __noinline__ uint4 unit_by_entries(const uint16_t* p, uint32_t n) {  // at the matrix's two ends
 	uint32_t w[4] = {0, 0, 0, 0};
@@ -46,76 +47,81 @@ __device__ __noinline__ uint4 unit_by_entries(const uint16_t* p, uint32_t n) {  
 		if (i < n) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
 	return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void unit_fetch(Unit& v, const uint16_t* base, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t row, uint32_t col) {
-	v.n = min(8u, cols - col);
-	const char *begin = reinterpret_cast<const char*>(base), *end = begin + ((uint64_t)(rows - 1) * ld + cols) * 2;
-	const uint16_t* p = base + (uint64_t)row * ld + col;
-	const char* q = reinterpret_cast<const char*>(p);
-	v.p = p;
-	v.shift = (uint32_t)(uintptr_t)q & 15u;
-	const char* down = q - v.shift;
-	v.wide = down >= begin && down + 32 <= end;
-	if (v.wide) {
-		v.lo = __ldg(reinterpret_cast<const uint4*>(down));
-		v.hi = __ldg(reinterpret_cast<const uint4*>(down) + 1);
-	}
-}
-__device__ __forceinline__ uint4 unit_value(const Unit& v) {
-	if (!v.wide) return unit_by_entries(v.p, v.n);
-	uint32_t w[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
-	if (v.shift & 8u) {
+// the 16 bytes from byte `shift` (even, below 16) of two neighbouring units on, the first n values of them
+__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t shift, uint32_t n) {
+	uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+	if (shift & 8u) {
 #pragma unroll
 		for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
 	}
-	if (v.shift & 4u) {
+	if (shift & 4u) {
 #pragma unroll
 		for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
 	}
-	const uint32_t b = (v.shift & 2u) * 8u;
+	const uint32_t b = (shift & 2u) * 8u;
 	uint32_t y[4];
 #pragma unroll
 	for (int i = 0; i < 4; ++i) {
 		y[i] = __funnelshift_r(w[i], w[i + 1], b);
-		if (2 * i + 1 >= (int)v.n) y[i] = 2 * i < (int)v.n ? y[i] & 0xffffu : 0u;
+		if (2 * i + 1 >= (int)n) y[i] = 2 * i < (int)n ? y[i] & 0xffffu : 0u;
 	}
 	return make_uint4(y[0], y[1], y[2], y[3]);
 }
-
-// Copies of up to three matrices with rows on 16-byte boundaries, for operands that have none: thread = 16 bytes of a copy.
-struct Realign {
-	const uint16_t* from[3];
-	uint64_t from_ld[3];
-	uint16_t* to[3];
-	uint32_t rows[3], cols[3];
-	uint64_t units[4];  // first unit of each, and behind the last
-};
-constexpr uint32_t kRealign = 2;  // units of a thread that are on their way together
-__global__ void __launch_bounds__(256, 4) realign_kernel(const Realign r) {
+// A thread has kAhead units on their way in shared memory: registers for them would leave too few threads to fill the memory's latency.
+constexpr int kAhead = 8, kRealignSmem = kAhead * 2 * 256 * 16, kRealignBlocks = 3 * kSMs;
+__global__ void __launch_bounds__(256, 3) realign_kernel(const Realign r) {
+	extern __shared__ uint4 ring[];  // [kAhead][2][256]
 	let_next_start();
+	const int k = blockIdx.x >= r.blocks[2] ? 2 : blockIdx.x >= r.blocks[1] ? 1 : 0;
+	const uint32_t per = (r.cols[k] + 7) / 8, cols = r.cols[k];
+	const uint64_t units = (uint64_t)r.rows[k] * per, width = (uint64_t)(r.blocks[k + 1] - r.blocks[k]) * 256;
+	// a thread's units lie `width` apart: (row, column) moves on by one division's worth, taken once
+	struct Place {
+		uint64_t u;
+		uint32_t row, col;
+	};
+	Place ahead;
+	ahead.u = (uint64_t)(blockIdx.x - r.blocks[k]) * 256 + threadIdx.x;
+	ahead.row = (uint32_t)(ahead.u / per), ahead.col = (uint32_t)(ahead.u - (uint64_t)ahead.row * per);
+	Place now = ahead;
+	const uint32_t step_row = (uint32_t)(width / per), step_col = (uint32_t)(width - (uint64_t)step_row * per);
+	auto next = [&](Place& p) {
+		p.u += width, p.row += step_row, p.col += step_col;
+		if (p.col >= per) p.col -= per, ++p.row;
+	};
+	const char *begin = reinterpret_cast<const char*>(r.from[k]), *end = begin + ((uint64_t)(r.rows[k] - 1) * r.from_ld[k] + cols) * 2;
+	auto address = [&](const Place& p, const char*& down) {
+		const char* q = begin + ((uint64_t)p.row * r.from_ld[k] + p.col * 8u) * 2;
+		down = q - ((uintptr_t)q & 15u);
+		return q;
+	};
+	auto fetch = [&](uint32_t slot) {
+		const char* down;
+		address(ahead, down);
+		if (ahead.u < units && down >= begin && down + 32 <= end) {
+			const uint32_t s = sptr(ring + slot * 512 + threadIdx.x);
+			asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(s), "l"(down) : "memory");
+			asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(s + 256 * 16), "l"(down + 16) : "memory");
+		}
+		asm volatile("cp.async.commit_group;" ::: "memory");
+		next(ahead);
+	};
 	wait_for_previous();
 #pragma unroll 1
-	for (int k = 0; k < 3; ++k) {
-		// a thread's units lie a grid's width apart: (row, column) moves on by one division's worth, taken once
-		const uint64_t units = r.units[k + 1] - r.units[k], width = (uint64_t)gridDim.x * 256;
-		uint64_t u = blockIdx.x * 256ull + threadIdx.x;
-		if (u >= units) continue;
-		const uint32_t per = (r.cols[k] + 7) / 8, step_row = (uint32_t)(width / per), step_col = (uint32_t)(width - (uint64_t)step_row * per);
-		uint32_t row = (uint32_t)(u / per), col = (uint32_t)(u - (uint64_t)row * per);
-		while (u < units) {
-			Unit v[kRealign];
-			uint4* to[kRealign];
-#pragma unroll
-			for (uint32_t j = 0; j < kRealign; ++j) {
-				to[j] = u < units ? reinterpret_cast<uint4*>(r.to[k]) + u : nullptr;
-				if (to[j]) unit_fetch(v[j], r.from[k], r.from_ld[k], r.rows[k], r.cols[k], row, col * 8);
-				u += width, row += step_row, col += step_col;
-				if (col >= per) col -= per, ++row;
-			}
-#pragma unroll
-			for (uint32_t j = 0; j < kRealign; ++j)
-				if (to[j]) *to[j] = unit_value(v[j]);
-		}
+	for (int i = 0; i < kAhead; ++i) fetch(i);
+#pragma unroll 1
+	for (uint32_t slot = 0; now.u < units; slot = slot + 1 == kAhead ? 0 : slot + 1) {
+		asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+		const char *down, *q = address(now, down);
+		const uint32_t n = min(8u, cols - now.col * 8);
+		uint4 v;
+		if (down >= begin && down + 32 <= end) v = shifted(ring[slot * 512 + threadIdx.x], ring[slot * 512 + 256 + threadIdx.x], (uint32_t)(q - down), n);
+		else v = unit_by_entries(reinterpret_cast<const uint16_t*>(q), n);
+		reinterpret_cast<uint4*>(r.to[k])[now.u] = v;
+		next(now);
+		fetch(slot);
 	}
+	asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // What a block of one variant is made of.  PAIR: two CTAs of a cluster compute a 256 x BN tile together, each with 128 of its rows in its
@@ -854,14 +860,18 @@ int write_linear_error(uint32_t flags) {
 bool operand_aligned(const void* p, uint64_t ld) { return tma_ok(p, ld); }
 int run_realign(const Operand* ops, int count, cudaStream_t stream) {
 	Realign r{};
+	uint64_t units[3] = {}, total = 0;
+	for (int k = 0; k < count; ++k) total += units[k] = (uint64_t)ops[k].rows * ((ops[k].cols + 7) / 8);
 	for (int k = 0; k < 3; ++k) {
-		r.units[k + 1] = r.units[k];
+		r.blocks[k + 1] = r.blocks[k];
 		if (k >= count) continue;
 		r.from[k] = (const uint16_t*)ops[k].from, r.from_ld[k] = ops[k].ld, r.to[k] = (uint16_t*)ops[k].to, r.rows[k] = ops[k].rows, r.cols[k] = ops[k].cols;
-		r.units[k + 1] += (uint64_t)ops[k].rows * ((ops[k].cols + 7) / 8);
+		// all blocks run at one time and have alike work
+		const uint64_t share = (uint64_t)((double)kRealignBlocks * (double)units[k] / (double)total), need = (units[k] + 255) / 256;
+		r.blocks[k + 1] += (uint32_t)std::max<uint64_t>(1, std::min(share, need));
 	}
-	const uint64_t blocks = (r.units[3] + 255) / 256;
-	return launch_behind(realign_kernel, (uint32_t)(blocks < 4ull * kSMs ? blocks : 4 * kSMs), 256, 0, stream, r);
+	N2B_CHECK_CUDA(cudaFuncSetAttribute(realign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRealignSmem));
+	return launch_behind(realign_kernel, r.blocks[3], 256, kRealignSmem, stream, r);
 }
 
 int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product_of<true>(p, stream) : product_of<false>(p, stream); }
