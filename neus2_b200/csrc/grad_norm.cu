@@ -200,10 +200,12 @@ __global__ void __launch_bounds__(kThreads) norm_final_kernel(const double* __re
 }
 
 // Launched so that it may start while the sums are still being taken: each block fetches its first piece before it waits for them.
+// The pieces are taken from the end: those that the norm read last are still in the L2 (40 M bf16 in 400 tensors: 38.3 us, from the
+// beginning 40.5).
 __global__ void __launch_bounds__(kThreads, 5) clip_kernel(const Piece* __restrict__ pieces, uint32_t n_pieces, const double* __restrict__ partial,
                                                             uint32_t n_partial, float scale, float max_norm, float* __restrict__ result) {
 	uint4 r[4];
-	Piece p = pieces[blockIdx.x];
+	Piece p = pieces[n_pieces - 1 - blockIdx.x];
 	auto load = [&](const Piece& q) {
 		by_type(q.dtype, [&](auto t) {
 			using T = typename std::remove_const<typename std::remove_pointer<decltype(t)>::type>::type;
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 5) clip_kernel(const Piece* __restri
 				scale_piece<T>(p, View(p, t, (((uintptr_t)p.in ^ (uintptr_t)p.out) & 15u) == 0), r, c);
 			});
 		if (k + gridDim.x < n_pieces) {
-			p = pieces[k + gridDim.x];
+			p = pieces[n_pieces - 1 - k - gridDim.x];
 			if (!(p.out == p.in && c == 1.f)) load(p);
 		}
 	}

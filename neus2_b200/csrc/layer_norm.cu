@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 
 template <int TPR, int E, bool RING>
 struct Backward {
-	static constexpr int kThreads = RING ? 512 : TPR > 128 ? TPR : 128, kGroups = kThreads / TPR;
-	static constexpr int kBlocks = (!RING && E <= 8 ? 1024 : 512) / kThreads;
+	static constexpr int kThreads = RING ? (E <= 8 ? 1024 : 512) : TPR > 128 ? TPR : 128, kGroups = kThreads / TPR;
+	static constexpr int kBlocks = (E <= 8 ? 1024 : 512) / kThreads;
 	static constexpr int kGrid = kSMs * kBlocks;
 };
 
@@ -638,6 +638,9 @@ template <typename T, int VEC, typename F>
 int with_backward_ring(uint32_t width, F f) {
 	const uint32_t u = (width + VEC - 1) / VEC;
 	constexpr int M = VEC == 8 ? 2 : 4;  // 16 entries a thread
+	if constexpr (VEC == 8) {
+		if (u <= 32) return f(Variant<T, VEC, 32, 1>());  // 8, and twice the threads: 65536 rows of 256 bf16 32 us, before 40
+	}
 	if (u <= 32 * M) return f(Variant<T, VEC, 32, M>());
 	if (u <= 64 * M) return f(Variant<T, VEC, 64, M>());
 	if (u <= 128 * M) return f(Variant<T, VEC, 128, M>());
