@@ -169,7 +169,8 @@ __device__ __forceinline__ void by_type(uint32_t dtype, F f) {
 __global__ void __launch_bounds__(kThreads, 6) norm_partial_kernel(const Piece* __restrict__ pieces, uint32_t n_pieces, uint32_t flags,
                                                                     double* __restrict__ partial, uint32_t* __restrict__ nonfinite) {
 	__shared__ double s[kThreads / 32];
-	let_next_start();  // the clipping kernel may start on what does not depend on the sums
+	wait_for_previous();
+	let_next_start();  // the clipping kernel may start on what does not depend on the sums: the gradients, which are complete from here on
 	Sum sum;
 	sum.skip = flags & NEUS2B_NORM_SKIP_NONFINITE;
 	Piece p{};
@@ -274,8 +275,7 @@ static int run(const void* d_table, uint32_t n_pieces, float scale, float max_no
 	if (n_pieces && (!d_table || ((uintptr_t)d_table & 15))) return NEUS2B_E_INVALID;
 	const uint32_t blocks = blocks_for(n_pieces);
 	if (blocks) {
-		norm_partial_kernel<<<blocks, kThreads, 0, s>>>((const Piece*)d_table, n_pieces, flags, (double*)d_workspace, d_nonfinite);
-		N2B_CHECK_LAUNCH();
+		if (int rc = launch_behind(norm_partial_kernel, blocks, kThreads, 0, s, (const Piece*)d_table, n_pieces, flags, (double*)d_workspace, d_nonfinite)) return rc;
 	}
 	if (clip && blocks) {
 		return launch_behind(clip_kernel, n_pieces < kClipBlocks ? n_pieces : kClipBlocks, kThreads, 0, s, (const Piece*)d_table, n_pieces,

@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 	const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
 	const uint32_t W = d.width;
 	const float inv_w = 1.f / (float)W;
+	let_next_start();
+	wait_for_previous();
 	float ga[F::kStaged ? 1 : VPT * VEC], be[F::kStaged ? 1 : VPT * VEC];
 	if (F::kStaged) {
 		stage_param<VEC, TPR, VPT>(sg, gamma, d.param_dtype, W, F::kThreads);
@@ -351,6 +353,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 	const uint32_t W = d.width;
 	const float inv_w = 1.f / (float)W;
 	let_next_start();
+	wait_for_previous();
 	float ga[E];
 #pragma unroll
 	for (int k = 0; k < E; ++k) {
@@ -468,6 +471,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ partial, uint32_t parts, uint32_t width, float* __restrict__ dgamma,
                                                      float* __restrict__ dbeta, int accumulate) {
 	__shared__ float s[32][33];
+	let_next_start();
 	wait_for_previous();
 	const uint32_t c = blockIdx.x * 32 + threadIdx.x;
 	float v = 0.f;
@@ -717,9 +721,8 @@ extern "C" int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, con
 				resident = most;
 			}
 			const uint32_t need = (desc->n + F::kGroups - 1) / F::kGroups, most = kSMs * resident;
-			kernel<<<need < most ? need : most, F::kThreads, smem, stream>>>(*desc, depth, (const T*)d_x, x_stride, d_gamma, d_beta, (T*)d_y, y_stride, d_mean, d_rstd);
-			N2B_CHECK_LAUNCH();
-			return NEUS2B_OK;
+			return launch_behind(kernel, need < most ? need : most, F::kThreads, smem, stream, *desc, depth, (const T*)d_x, x_stride, d_gamma, d_beta, (T*)d_y, y_stride,
+			                     d_mean, d_rstd);
 		};
 		const bool vec = rows16(d_x, x_stride, b) && rows16(d_y, y_stride, b) && desc->width % V == 0;
 		int rc = kTooWide;
@@ -793,9 +796,9 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 			smem = smem > kSums ? smem : kSums;
 			auto kernel = backward_kernel<T, K::kVec, K::kTpr, K::kVpt, decltype(ring)::value>;
 			if (smem > 32 * 1024) N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-			kernel<<<blocks, B::kThreads, smem, stream>>>(*desc, depth, (const T*)d_x, x_stride, d_gamma, d_mean, d_rstd, (const T*)d_dL_dy, dy_stride,
-			                                              (const T*)d_skip, skip_stride, (T*)d_dL_dx, dx_stride, params ? (float*)d_workspace : nullptr);
-			N2B_CHECK_LAUNCH();
+			if (int rc = launch_behind(kernel, blocks, B::kThreads, smem, stream, *desc, depth, (const T*)d_x, x_stride, d_gamma, d_mean, d_rstd, (const T*)d_dL_dy, dy_stride,
+			                           (const T*)d_skip, skip_stride, (T*)d_dL_dx, dx_stride, params ? (float*)d_workspace : nullptr))
+				return rc;
 			if (params) {
 				return launch_behind(join_kernel, (2 * width + 31) / 32, dim3(32, 32), 0, stream, (const float*)d_workspace, blocks, width, d_dgamma, d_dbeta,
 				                     accumulate);

@@ -7,6 +7,8 @@ namespace n2b {
 template <typename T>
 __global__ void __launch_bounds__(256) slope_kernel(uint64_t n, uint32_t width, int act, const T* __restrict__ z, uint64_t z_ld,
                                                      const T* __restrict__ dy, uint64_t dy_ld, T* __restrict__ dz, uint64_t dz_ld) {
+	wait_for_previous();
+	let_next_start();
 	for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n * width; i += gridDim.x * 256ull) {
 		const uint64_t r = i / width;
 		const uint32_t c = (uint32_t)(i - r * width);
@@ -143,10 +145,8 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		const uint64_t ld = (out + 7) / 8 * 8;
 		const int rc = with_half_type(desc->dtype, [&](auto t) {
 			using T = decltype(t);
-			slope_kernel<T><<<kSMs * 8, 256, 0, stream>>>(n, out, (int)desc->activation, (const T*)d_preact, preact_stride, (const T*)d_dL_dy, dy_stride,
-			                                           (T*)d_workspace, ld);
-			N2B_CHECK_LAUNCH();
-			return NEUS2B_OK;
+			return launch_behind(slope_kernel<T>, kSMs * 8, 256, 0, stream, n, out, (int)desc->activation, (const T*)d_preact, preact_stride, (const T*)d_dL_dy,
+			                     dy_stride, (T*)d_workspace, ld);
 		});
 		if (rc) return rc;
 		dz = d_workspace, dz_ld = ld;

@@ -632,6 +632,7 @@ template <int VEC>
 __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t M, uint32_t N, float* __restrict__ out,
                                                     float* __restrict__ sums, int accumulate) {
 	extern __shared__ float s[];  // [blockDim.y][VEC][blockDim.x]
+	let_next_start();
 	wait_for_previous();
 	const uint64_t n = (uint64_t)M * N, groups = n / VEC, first = out ? 0 : groups, total = groups + (sums ? M : 0);
 	for (uint64_t base = first + (uint64_t)blockIdx.x * blockDim.x; base < total; base += (uint64_t)gridDim.x * blockDim.x) {
@@ -809,6 +810,8 @@ static uint64_t plan_bytes(const WgradPlan& w, uint32_t M, uint32_t N) {
 __global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ a, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t bf16,
                                                           float* __restrict__ partial) {
 	__shared__ float s[8][32][9];
+	wait_for_previous();
+	let_next_start();
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	const uint32_t c = blockIdx.x * 256 + lane * 8;
 	const bool bf = bf16 != 0;
@@ -916,8 +919,7 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 		// finds the matrix in the L2
 		if (p.column_sums) {
 			const uint32_t most = sum_blocks(p.M), need = tiles_of(p.K, 32), by = need < most ? need : most;
-			column_sums_kernel<<<dim3(tiles_of(p.M, 256), by), 256, 0, stream>>>(a.a, a.a_ld, p.K, p.M, a.bf16, (float*)p.workspace);
-			N2B_CHECK_LAUNCH();
+			if (int rc = launch_behind(column_sums_kernel, dim3(tiles_of(p.M, 256), by), 256, 0, stream, a.a, a.a_ld, p.K, p.M, a.bf16, (float*)p.workspace)) return rc;
 			if (int rc = run_join((const float*)p.workspace, by, p.M, 0, nullptr, p.column_sums, p.e.accumulate, stream)) return rc;
 		}
 		const uint32_t pairs = (uint32_t)(units < (uint64_t)(kSMs / 2) ? units : kSMs / 2);
