@@ -1,5 +1,6 @@
 """Tensor-level wrappers over the C ABI (torch is only the owner of device memory and streams)."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -332,11 +333,28 @@ def _bytes(query, desc, *flags):
     return need.value
 
 
-def _gradient(t, name, shape, mode, like):
-    """The fp32 tensor a parameter gradient goes to: the caller's, or a new one where there is nothing to add to."""
+# Short calls are bound by the host: what a call derives from its sizes alone is kept with them.
+@functools.lru_cache(maxsize=1024)
+def _linear_plan(n, n_in, n_out, dtype, activation, backward, unaligned):
+    """(descriptor, workspace bytes)"""
+    d = L.LinearDesc(n, n_in, n_out, _DTYPES[dtype], activation)
+    lib = L.lib()
+    return d, _bytes(lib.neus2b_linear_backward_workspace if backward else lib.neus2b_linear_forward_workspace, d, unaligned)
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_plan(n, width, dtype, param_dtype, eps):
+    d = L.LayerNormDesc(n, width, _DTYPES[dtype], _DTYPES[param_dtype], eps)
+    return d, _bytes(L.lib().neus2b_layer_norm_backward_workspace, d)
+
+
+def _gradient(t, name, shape, mode, param, like):
+    """The fp32 tensor a parameter gradient goes to: the caller's, or a new one where there is nothing to add to.  param: a contiguous tensor
+    of that shape, or None."""
     if t is None:
-        new = like.new_zeros if mode == L.GRAD_ACCUMULATE else like.new_empty
-        return new(shape, dtype=torch.float32)
+        if mode == L.GRAD_ACCUMULATE:
+            return like.new_zeros(shape, dtype=torch.float32)
+        return like.new_empty(shape, dtype=torch.float32) if param is None else torch.empty_like(param, dtype=torch.float32)
     if t.get_device() != like.get_device() or t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         _refuse(f"{name} has to be contiguous float32 {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t
@@ -355,15 +373,13 @@ def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_p
     rp, rs = _rows(residual, "residual", n, n_out, t, dev)
     bp = _vector(bias, "bias", n_out, t, dev)
     if out is None:
-        out = x.new_empty((n, n_out))
+        out = x.new_empty(n, n_out)
     yp, ys = _rows(out, "out", n, n_out, t, dev)
-    z = x.new_empty((n, n_out)) if want_preact else None
-    d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
-    lib, wp = L.lib(), w.data_ptr()
-    keep, wsp, wsb = None, None, 0
-    if (xp | wp | xs * 2 | n_in * 2) & 15:
-        keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_forward_workspace, d, 1), workspace, x)
-    L.check(lib.neus2b_linear_forward(C.byref(d), xp, xs, wp, bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out, wsp, wsb,
+    z = x.new_empty(n, n_out) if want_preact else None
+    wp = w.data_ptr()
+    d, need = _linear_plan(n, n_in, n_out, t, activation, False, 1 if (xp | wp | xs * 2 | n_in * 2) & 15 else 0)
+    keep, wsp, wsb = _workspace(need, workspace, x)
+    L.check(L.lib().neus2b_linear_forward(C.byref(d), xp, xs, wp, bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out, wsp, wsb,
                                       _raw_stream(dev)))
     return (out, z) if want_preact else out
 
@@ -388,40 +404,39 @@ def linear_backward(x, w, dL_dout, activation=L.ACT_NONE, preact=None, below_act
     zp, zs = _rows(preact, "preact", n, n_out, t, dev)
     bzp, bzs = _rows(below_preact, "below_preact", n, n_in, t, dev)
     sp, ss = _rows(skip, "skip", n, n_in, t, dev)
-    din = x.new_empty((n, n_in)) if want_din else None
+    din = x.new_empty(n, n_in) if want_din else None
     params = mode != L.GRAD_IGNORE
-    wgrad = _gradient(wgrad, "wgrad", (n_out, n_in), mode, x) if params else None
-    bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, x) if params and want_bias else None
-    d = L.LinearDesc(n, n_in, n_out, _DTYPES[t], activation)
-    lib = L.lib()
-    unaligned = 1 if (xp | w.data_ptr() | dyp | xs * 2 | n_in * 2 | dys * 2) & 15 else 0
-    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_linear_backward_workspace, d, unaligned), workspace, x)
-    L.check(lib.neus2b_linear_backward(C.byref(d), xp, xs, w.data_ptr(), zp, zs, dyp, dys, below_activation, bzp, bzs, sp, ss,
+    wgrad = _gradient(wgrad, "wgrad", (n_out, n_in), mode, w, x) if params else None
+    bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, None, x) if params and want_bias else None
+    wp = w.data_ptr()
+    d, need = _linear_plan(n, n_in, n_out, t, activation, True, 1 if (xp | wp | dyp | xs * 2 | n_in * 2 | dys * 2) & 15 else 0)
+    keep, wsp, wsb = _workspace(need, workspace, x)
+    L.check(L.lib().neus2b_linear_backward(C.byref(d), xp, xs, wp, zp, zs, dyp, dys, below_activation, bzp, bzs, sp, ss,
                                        din.data_ptr() if want_din else None, n_in, wgrad.data_ptr() if params else None,
                                        bgrad.data_ptr() if bgrad is not None else None, mode, wsp, wsb, _raw_stream(dev)))
     return din, wgrad, bgrad
 
 
-def _norm_desc(x, gamma, eps):
+def _norm_of(x, gamma, eps):
     if x.dtype not in _DTYPES:
         _refuse(f"layer norm takes float32, float16 and bfloat16, got {x.dtype}")
     if x.dim() != 2:
         _refuse(f"x has to be [n][width], got {list(x.shape)}")
     if gamma.dtype != x.dtype and gamma.dtype != torch.float32:
         _refuse(f"gamma has to be {x.dtype} or float32, got {gamma.dtype}")
-    return L.LayerNormDesc(x.shape[0], x.shape[1], _DTYPES[x.dtype], _DTYPES[gamma.dtype], eps)
+    return _norm_plan(x.shape[0], x.shape[1], x.dtype, gamma.dtype, eps)
 
 
 def layer_norm_forward(x, gamma, beta=None, eps=1e-5, want_stats=False, out=None):
     """gamma (x - mean) rstd + beta over the rows of x [n][width] (fp32, fp16, bf16; gamma and beta of the same type or fp32).
     want_stats: returns (y, mean, rstd), which layer_norm_backward reads.  `out` may be x."""
     dev = _home(x, "x")
-    d = _norm_desc(x, gamma, eps)
+    d, _ = _norm_of(x, gamma, eps)
     n, width = x.shape
     xp, xs = _rows(x, "x", n, width, x.dtype, dev)
     gp, bp = _vector(gamma, "gamma", width, gamma.dtype, dev), _vector(beta, "beta", width, gamma.dtype, dev)
     if out is None:
-        out = x.new_empty((n, width))
+        out = x.new_empty(n, width)
     yp, ys = _rows(out, "out", n, width, x.dtype, dev)
     if not want_stats:
         L.check(L.lib().neus2b_layer_norm_forward(C.byref(d), xp, xs, gp, bp, yp, ys, None, None, _raw_stream(dev)))
@@ -435,20 +450,19 @@ def layer_norm_backward(x, gamma, mean, rstd, dL_dout, skip=None, dgamma=None, d
                         workspace=None):
     """(dL/dx, dgamma, dbeta) of layer_norm_forward; skip [n][width] is added to dL/dx (a residual connection around the norm)."""
     dev = _home(x, "x")
-    d = _norm_desc(x, gamma, eps)
+    d, need = _norm_of(x, gamma, eps)
     n, width = x.shape
     xp, xs = _rows(x, "x", n, width, x.dtype, dev)
     dyp, dys = _rows(dL_dout, "dL_dout", n, width, x.dtype, dev)
     sp, ss = _rows(skip, "skip", n, width, x.dtype, dev)
     gp = _vector(gamma, "gamma", width, gamma.dtype, dev)
     mp, rp = _vector(mean, "mean", n, torch.float32, dev), _vector(rstd, "rstd", n, torch.float32, dev)
-    din = x.new_empty((n, width)) if want_din else None
+    din = x.new_empty(n, width) if want_din else None
     params = mode != L.GRAD_IGNORE
-    dgamma = _gradient(dgamma, "dgamma", (width,), mode, x) if params else None
-    dbeta = _gradient(dbeta, "dbeta", (width,), mode, x) if params else None
-    lib = L.lib()
-    keep, wsp, wsb = _workspace(_bytes(lib.neus2b_layer_norm_backward_workspace, d) if params else 0, workspace, x)
-    L.check(lib.neus2b_layer_norm_backward(C.byref(d), xp, xs, gp, mp, rp, dyp, dys, sp, ss, din.data_ptr() if want_din else None, width,
+    dgamma = _gradient(dgamma, "dgamma", (width,), mode, gamma, x) if params else None
+    dbeta = _gradient(dbeta, "dbeta", (width,), mode, gamma, x) if params else None
+    keep, wsp, wsb = _workspace(need if params else 0, workspace, x)
+    L.check(L.lib().neus2b_layer_norm_backward(C.byref(d), xp, xs, gp, mp, rp, dyp, dys, sp, ss, din.data_ptr() if want_din else None, width,
                                            dgamma.data_ptr() if params else None, dbeta.data_ptr() if params else None, mode, wsp, wsb,
                                            _raw_stream(dev)))
     return din, dgamma, dbeta
