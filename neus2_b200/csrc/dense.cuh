@@ -62,20 +62,48 @@ __device__ __forceinline__ float act_slope(int act, float z) {
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <typename... P, typename... A>
-int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+int launch_behind_in_clusters(uint32_t cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
 	cudaLaunchConfig_t cfg{};
 	cfg.gridDim = grid;
 	cfg.blockDim = block;
 	cfg.dynamicSmemBytes = smem;
 	cfg.stream = stream;
-	cudaLaunchAttribute attr[1];
+	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
 	attr[0].val.programmaticStreamSerializationAllowed = 1;
+	attr[1].id = cudaLaunchAttributeClusterDimension;
+	attr[1].val.clusterDim.x = cluster;
+	attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
 	cfg.attrs = attr;
-	cfg.numAttrs = 1;
+	cfg.numAttrs = cluster > 1 ? 2 : 1;
 	N2B_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, (P)args...));
 	N2B_CHECK_LAUNCH();
 	return NEUS2B_OK;
+}
+
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+	return launch_behind_in_clusters(1, kernel, grid, block, smem, stream, args...);
+}
+
+// Blocks of a cluster and each other's shared memory
+__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
+	uint32_t p;
+	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+	return p;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+	uint32_t r;
+	asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+	return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
+	float v;
+	asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(addr, rank)) : "memory");
+	return v;
 }
 
 template <typename F>

@@ -689,7 +689,7 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 	a.chunks = (a.e.slope_z && a.e.add) || (a.e.preact && a.e.add) ? 2 : 1;
 	a.stages = S::stages((int)a.chunks);
 	const int smem = (int)a.stages * S::kStage + S::fixed((int)a.chunks);
-	N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+	N2B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));  // (the same from every thread)
 	cudaLaunchConfig_t cfg{};
 	cfg.gridDim = dim3(ctas);
 	cfg.blockDim = dim3(S::kThreads);

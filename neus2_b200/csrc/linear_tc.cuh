@@ -54,11 +54,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 		             "r"(x), "r"(y), "r"(bar)
 		             : "memory");
 }
-__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
-	uint32_t p;
-	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-	return p;
-}
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
 	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -116,20 +111,6 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
 	             : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
 	               "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
-	uint32_t r;
-	asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-	return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
-	float v;
-	asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(addr, rank)) : "memory");
-	return v;
-}
-
 __device__ __forceinline__ float2 unpack2(uint32_t w, bool bf) {
 	return bf ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
