@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 	const uint32_t tiles = p.tiles_m * p.tiles_n, kblocks = (p.K + kBK - 1) / kBK;
 	const uint32_t first = PAIR ? blockIdx.x / 2 : p.cluster > 1 ? (blockIdx.x / p.cluster) + rank * tiles : blockIdx.x;
 	const uint32_t units = tiles * p.splits;
-	const bool single = !WGRAD && !PAIR && (SWAP || p.cluster > 1);
+	const bool single = !PAIR && (SWAP || p.cluster > 1);
 	const uint32_t step = PAIR ? gridDim.x / 2 : single ? units : gridDim.x;
 	const uint32_t row_offset = PAIR ? rank * kBM : 0u;
 	constexpr int kTileM = PAIR ? 2 * kBM : kBM;
@@ -445,6 +445,13 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 					next_buf();
 				}
 				if (!ok) break;
+				if (p.cluster > 1) {  // (every operand tile of this CTA's only unit has been consumed)
+					float* const joined = reinterpret_cast<float*>(smem);
+#pragma unroll
+					for (int i = 0; i < kCols; ++i) joined[joined_at<BN, SWAP>(q * 32 + lane, half * kCols + i)] = acc[i];
+					if (sums) joined[kBM * (BN + 1) + q * 32 + lane] = sum;
+					continue;
+				}
 				Epilogue e = p.e;
 				if (p.splits > 1) {
 					e.out = p.partial + (uint64_t)split * p.M * p.N;
@@ -574,6 +581,12 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 		else __syncthreads();
 		uint32_t mt, nt, split, kb0, kb1;
 		locate(first, mt, nt, split, kb0, kb1);
+		if (WGRAD && p.want_sums && nt == 0 && rank == 0 && tid < kBM && mt * kBM + tid < p.M) {
+			float v = 0.f;
+			for (uint32_t s = 0; s < p.cluster; ++s) v += load_peer(sptr(smem) + (kBM * (BN + 1) + tid) * 4, s);
+			float* const o = p.column_sums + mt * kBM + tid;
+			*o = p.e.accumulate ? *o + v : v;
+		}
 		const uint32_t joined = sptr(smem), rows = min((uint32_t)kBM, p.M - mt * kBM), cols = min((uint32_t)BN, p.N - nt * BN);
 		const uint32_t count = rows * cols, stride = p.cluster * S::kThreads;
 		const Epilogue& e = p.e;
@@ -608,6 +621,12 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 #pragma unroll
 			for (int k = 0; k < 2; ++k) {
 				if (!in[k]) continue;
+				if (WGRAD) {
+					if (!e.out) continue;
+					float* const o = (float*)e.out + sample[k] * e.out_ld + feature[k];
+					*o = e.accumulate ? *o + v[k] : v[k];
+					continue;
+				}
 				float y = v[k] + (e.bias ? h2f(bias[k], bf) : 0.f);
 				if (e.preact) ((uint16_t*)e.preact)[sample[k] * e.preact_ld + feature[k]] = f2h(y, bf);
 				y = e.slope_z ? y * act_slope(e.act, h2f(z[k], bf)) : act_value(e.act, y);
@@ -714,10 +733,11 @@ static int launch(Args& a, uint32_t ctas, cudaStream_t stream) {
 // second round.  Splitting pays from so many steps of 64 on: with few samples from two for each CTA; with 128 samples a tile the join
 // takes 3 us where two CTAs share it and 1.5 where eight do (100 samples, 512 -> 512: 7.4 us over clusters, 8.0 without; 1000 samples: 9.7
 // over clusters of two, 8.6 without).
+constexpr uint32_t kClusterFit[2][3] = {{148, 132, 120}, {296, 284, 264}};  // CTAs in clusters of 2, 4, 8
 static uint32_t cluster_for(uint64_t tiles, uint32_t kblocks, bool swap) {
-	constexpr uint32_t kFit[2][3] = {{148, 132, 120}, {296, 284, 264}}, kSteps[2][3] = {{16, 8, 16}, {4, 8, 16}};
+	constexpr uint32_t kSteps[2][3] = {{16, 8, 16}, {4, 8, 16}};
 	for (int c = 2; c >= 0; --c)
-		if ((tiles << (c + 1)) <= kFit[swap][c] && kblocks >= kSteps[swap][c]) return 2u << c;
+		if ((tiles << (c + 1)) <= kClusterFit[swap][c] && kblocks >= kSteps[swap][c]) return 2u << c;
 	return 1;
 }
 
@@ -774,10 +794,11 @@ static int product_of(const Product& p, cudaStream_t stream) {
 // Weight gradient: tiles of out_width x in_width, k the samples.  Few tiles share the samples out over the SMs and are joined afterwards.
 // One CTA's 128 x 128 tile takes about 430 cycles for 64 samples (its operands' way through shared memory), a pair's 256 x 256 tile 512
 // (its MMAs) and, where the column sums are wanted, the pass over dz that takes them and its join: 6 us and 4 TB/s.  The plan with the
-// fewest cycles is taken.
+// fewest cycles is taken.  Parts are joined by a pass of their own (6000 cycles with its launch), or, where a cluster's CTAs are enough parts,
+// through its shared memory (3000): 1328 samples, 160 -> 192: 14.1 us for the whole backward pass, 16.9 with a pass of its own.
 struct WgradPlan {
 	bool pair;
-	uint32_t tiles_m, tiles_n, splits;
+	uint32_t tiles_m, tiles_n, splits, cluster;
 };
 static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair, bool sums) {  // (a pair's kernel always stores the product)
 	const uint32_t kblocks = tiles_of(K, kBK);
@@ -787,10 +808,17 @@ static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair, b
 		const uint32_t size = pair ? 256 : 128, slots = pair ? kSMs / 2 : kSMs;
 		const uint64_t tiles = (uint64_t)tiles_of(M, size) * tiles_of(N, size), fill = slots / tiles, most = kblocks / kChunk;
 		const uint64_t splits = fill < most ? (fill ? fill : 1) : (most ? most : 1);
-		const uint64_t cycles = (tiles * splits + slots - 1) / slots * ((kblocks + splits - 1) / splits) * (pair ? 512 : 430) + (pair && sums ? 11000 + (uint64_t)K * M / 1000 : 0);
+		const uint64_t cycles = (tiles * splits + slots - 1) / slots * ((kblocks + splits - 1) / splits) * (pair ? 512 : 430) +
+		                        (splits > 1 ? 6000 : 0) + (pair && sums ? 11000 + (uint64_t)K * M / 1000 : 0);
 		if (!pair || cycles < best) {
 			best = cycles;
-			plan = WgradPlan{pair != 0, tiles_of(M, size), tiles_of(N, size), (uint32_t)splits};
+			plan = WgradPlan{pair != 0, tiles_of(M, size), tiles_of(N, size), (uint32_t)splits, 1};
+		}
+		for (int c = 0; !pair && c < 3; ++c) {
+			const uint64_t together = ((uint64_t)kblocks + (2u << c) - 1) / (2u << c) * 430 + 3000;
+			if ((tiles << (c + 1)) > kClusterFit[0][c] || together >= best) continue;
+			best = together;
+			plan = WgradPlan{false, tiles_of(M, size), tiles_of(N, size), 2u << c, 2u << c};
 		}
 	}
 	return plan;
@@ -801,7 +829,7 @@ static uint32_t sum_blocks(uint32_t cols) {
 	return by ? by : 1;
 }
 static uint64_t plan_bytes(const WgradPlan& w, uint32_t M, uint32_t N) {
-	const uint64_t partial = w.splits > 1 ? (uint64_t)w.splits * ((uint64_t)M * N + M) * 4 : 0, sums = w.pair ? (uint64_t)sum_blocks(M) * M * 4 : 0;
+	const uint64_t partial = w.splits > 1 && w.cluster == 1 ? (uint64_t)w.splits * ((uint64_t)M * N + M) * 4 : 0, sums = w.pair ? (uint64_t)sum_blocks(M) * M * 4 : 0;
 	return partial > sums ? partial : sums;
 }
 
@@ -909,8 +937,7 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 	a.M = p.M, a.N = p.N, a.K = p.K;
 	a.a = (const uint16_t*)p.a, a.a_ld = p.a_ld, a.b = (const uint16_t*)p.b, a.b_ld = p.b_ld;
 	a.e = p.e;
-	a.tiles_m = w.tiles_m, a.tiles_n = w.tiles_n, a.splits = w.splits;
-	a.cluster = 1;
+	a.tiles_m = w.tiles_m, a.tiles_n = w.tiles_n, a.splits = w.splits, a.cluster = w.cluster;
 	a.partial = (float*)p.workspace;
 	const uint64_t units = (uint64_t)a.tiles_m * a.tiles_n * a.splits;
 	if (units >= (1ull << 31)) return NEUS2B_E_TOO_LARGE;
@@ -930,7 +957,7 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 	a.want_sums = p.column_sums != nullptr;
 	const uint32_t ctas = (uint32_t)(units < (uint64_t)kSMs ? units : kSMs);
 	if (int rc = launch<128, true, true, false, true, false>(a, ctas, stream)) return rc;
-	return w.splits > 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate, stream) : NEUS2B_OK;
+	return w.splits > 1 && w.cluster == 1 ? run_join(a.partial, a.splits, p.M, p.N, (float*)p.e.out, p.column_sums, p.e.accumulate, stream) : NEUS2B_OK;
 }
 
 }  // namespace n2b
