@@ -3,17 +3,50 @@
 
 namespace n2b {
 
-// dz = dy * act'(z)
-template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(uint64_t n, uint32_t width, int act, const T* __restrict__ z, uint64_t z_ld,
-                                                     const T* __restrict__ dy, uint64_t dy_ld, T* __restrict__ dz, uint64_t dz_ld) {
+// dz = dy * act'(z), eight columns a thread; rows of dz start on 16-byte boundaries and hold whole units of eight.  VEC: rows of z and dy start
+// there, too.  Bound by memory: 8192 x 4096 fp16 in 35 us, 5.8 TB/s; entry by entry with a division each it took 100.
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(256) slope_kernel(uint32_t n, uint32_t width, const T* __restrict__ z, uint64_t z_ld, const T* __restrict__ dy, uint64_t dy_ld,
+                                                     T* __restrict__ dz) {
 	wait_for_previous();
 	let_next_start();
-	for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n * width; i += gridDim.x * 256ull) {
-		const uint64_t r = i / width;
-		const uint32_t c = (uint32_t)(i - r * width);
-		dz[r * dz_ld + c] = from_f<T>(to_f(dy[r * dy_ld + c]) * act_slope(act, to_f(z[r * z_ld + c])));
+	const uint32_t per = (width + 7) / 8;
+	const uint64_t units = (uint64_t)n * per, step = gridDim.x * 256ull;
+	const uint32_t step_row = (uint32_t)(step / per), step_col = (uint32_t)(step - (uint64_t)step_row * per);
+	uint64_t u = blockIdx.x * 256ull + threadIdx.x;
+	uint32_t row = (uint32_t)(u / per), col = (uint32_t)(u - (uint64_t)row * per);
+	for (; u < units; u += step) {
+		const T *zp = z + row * z_ld + col * 8u, *dp = dy + row * dy_ld + col * 8u;
+		const uint32_t count = width - col * 8u;  // 8 at least, but for the last ones of a row
+		union Eight {
+			uint4 q;
+			T v[8];
+		} a{}, b{};
+		if (VEC && count >= 8) {
+			a.q = *reinterpret_cast<const uint4*>(zp);
+			b.q = *reinterpret_cast<const uint4*>(dp);
+		} else {
+#pragma unroll
+			for (uint32_t k = 0; k < 8; ++k)
+				if (k < count) a.v[k] = zp[k], b.v[k] = dp[k];
+		}
+#pragma unroll
+		for (int k = 0; k < 8; ++k) b.v[k] = from_f<T>(to_f(b.v[k]) * act_slope(ACT, to_f(a.v[k])));
+		reinterpret_cast<uint4*>(dz)[u] = b.q;
+		row += step_row, col += step_col;
+		if (col >= per) col -= per, ++row;
 	}
+}
+template <typename T>
+static int run_slope(uint32_t n, uint32_t width, int act, const void* z, uint64_t z_ld, const void* dy, uint64_t dy_ld, void* dz, cudaStream_t stream) {
+	const bool vec = operand_aligned(z, z_ld) && operand_aligned(dy, dy_ld);
+	const uint64_t blocks = ((uint64_t)n * ((width + 7) / 8) + 255) / 256;
+	auto go = [&](auto kernel) {
+		return launch_behind(kernel, (uint32_t)(blocks < 8ull * kSMs ? blocks : 8 * kSMs), 256, 0, stream, n, width, (const T*)z, z_ld, (const T*)dy, dy_ld, (T*)dz);
+	};
+	if (act == NEUS2B_ACT_RELU) return vec ? go(slope_kernel<T, NEUS2B_ACT_RELU, true>) : go(slope_kernel<T, NEUS2B_ACT_RELU, false>);
+	if (act == NEUS2B_ACT_GELU) return vec ? go(slope_kernel<T, NEUS2B_ACT_GELU, true>) : go(slope_kernel<T, NEUS2B_ACT_GELU, false>);
+	return vec ? go(slope_kernel<T, NEUS2B_ACT_SILU, true>) : go(slope_kernel<T, NEUS2B_ACT_SILU, false>);
 }
 
 static bool bad_desc(const neus2b_linear_desc* d) {
@@ -145,8 +178,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		const uint64_t ld = (out + 7) / 8 * 8;
 		const int rc = with_half_type(desc->dtype, [&](auto t) {
 			using T = decltype(t);
-			return launch_behind(slope_kernel<T>, kSMs * 8, 256, 0, stream, n, out, (int)desc->activation, (const T*)d_preact, preact_stride, (const T*)d_dL_dy,
-			                     dy_stride, (T*)d_workspace, ld);
+			return run_slope<T>(n, out, (int)desc->activation, d_preact, preact_stride, d_dL_dy, dy_stride, d_workspace, stream);
 		});
 		if (rc) return rc;
 		dz = d_workspace, dz_ld = ld;

@@ -6,6 +6,9 @@
 // gradient in one pass over dz and x: the tile of dz is the K-major operand of dL/dx = dz W and, the same bytes, the MN-major operand of
 // dz^T x.  The weight gradient's sums stay in tensor memory for four tiles (512 samples), then in registers, and leave the CTA
 // once; the bias gradient is the product of dz^T with a tile of ones.
+//
+// 262144 samples, fp16: 48 -> 64 with ReLU 13.2 us (4.5 TB/s over what has to move), backward of 64 <- 64 with slopes, skip connection
+// and bias 36 us with its join (4.6 TB/s).  A tile's operands are 16 KB each, so that two to eight stages fit; one CTA on an SM.
 #include "linear_tc.cuh"
 
 namespace n2b {
