@@ -354,7 +354,7 @@ def _gradient(t, name, shape, mode, param, like):
     if t is None:
         if mode == L.GRAD_ACCUMULATE:
             return like.new_zeros(shape, dtype=torch.float32)
-        return like.new_empty(shape, dtype=torch.float32) if param is None else torch.empty_like(param, dtype=torch.float32)
+        return like.new_empty(*shape, dtype=torch.float32) if param is None else torch.empty_like(param, dtype=torch.float32)
     if t.get_device() != like.get_device() or t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         _refuse(f"{name} has to be contiguous float32 {list(shape)} on {like.device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t

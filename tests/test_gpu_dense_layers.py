@@ -470,6 +470,36 @@ def test_streams_and_graph(ops):
         first = [v.clone() for v in block()]
 
 
+def test_two_streams_at_once(ops):
+    """Calls of every kind issued to two streams in turn, without waiting in between, give the bits that they give one after another."""
+    g = gen(77)
+    t = torch.bfloat16
+    jobs = []
+    for n, i, o in [(5, 512, 300), (64, 1000, 1000), (300, 2056, 120), (2000, 131, 257), (5000, 64, 64), (1500, 512, 512), (3000, 1024, 2048)]:
+        x, dy, zb = rows(g, n, i, t), rows(g, n, o, t, 0.1), rows(g, n, i, t)
+        w, b = rows(g, o, i, t, 0.05), rows(g, 1, o, t)[0]
+        gamma = torch.ones(i, device="cuda")
+
+        def job(x=x, dy=dy, zb=zb, w=w, b=b, gamma=gamma):
+            y, z = ops.linear_forward(x, w, b, None, R.GELU, want_preact=True)
+            dx, dw, db = ops.linear_backward(x, w, dy, activation=R.GELU, preact=z, below_activation=R.SILU, below_preact=zb)
+            h, mean, rstd = ops.layer_norm_forward(x, gamma, want_stats=True)
+            dh, dg, dbeta = ops.layer_norm_backward(x, gamma, mean, rstd, dx, skip=h)
+            return [y, z, dx, dw, db, h, dh, dg, dbeta]
+        jobs.append(job)
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for turn in range(4):
+        for k, job in enumerate(jobs):
+            with torch.cuda.stream(streams[(k + turn) % 2]):
+                got.append((k, job()))
+    torch.cuda.synchronize()
+    for k, out in got:
+        assert all(torch.equal(u, v) for u, v in zip(out, want[k])), k
+
+
 def test_no_wait_ran_out(ops):
     from neus2_b200 import _lib as L
     torch.cuda.synchronize()
