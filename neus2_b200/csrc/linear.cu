@@ -60,12 +60,15 @@ static bool clash(const void* out, uint64_t out_stride, const void* in, uint64_t
 static bool bad_matrix(const void* p, uint64_t stride, uint32_t width, size_t align) { return !p || stride < width || ((uintptr_t)p & (align - 1)); }
 static bool bad_optional(const void* p, uint64_t stride, uint32_t width, size_t align) { return p && bad_matrix(p, stride, width, align); }
 
-static bool on16(const void* p, uint64_t ld, size_t bytes) { return !p || (((uintptr_t)p | (ld * bytes)) & 15) == 0; }
-// Whether the epilogue may move 16 bytes at a time: every row that it touches starts on a 16-byte boundary, and rows of 16-bit values
-// are whole numbers of accesses (an fp32 row's end is handled apart).
-static int whole_vectors(const Epilogue& e, uint32_t width) {
-	return (e.out_f32 || width % 8 == 0) && on16(e.out, e.out_ld, e.out_f32 ? 4 : 2) && on16(e.bias, 0, 2) && on16(e.add, e.add_ld, 2) && on16(e.slope_z, e.slope_ld, 2) &&
-	       on16(e.preact, e.preact_ld, 2);
+static bool starts_on(uint32_t at, const void* p, uint64_t ld, size_t bytes) { return !p || (((uintptr_t)p | (ld * bytes)) & (at - 1)) == 0; }
+// Bytes that the epilogue may move at a time: every row that it touches starts on such a boundary, and rows of 16-bit values are whole numbers
+// of accesses (an fp32 row's end is handled apart).
+static int widest_access(const Epilogue& e, uint32_t width) {
+	auto fits = [&](uint32_t at) {
+		return (e.out_f32 || width % (at / 2) == 0) && starts_on(at, e.out, e.out_ld, e.out_f32 ? 4 : 2) && starts_on(at, e.bias, 0, 2) &&
+		       starts_on(at, e.add, e.add_ld, 2) && starts_on(at, e.slope_z, e.slope_ld, 2) && starts_on(at, e.preact, e.preact_ld, 2);
+	};
+	return fits(16) ? 16 : fits(4) ? 4 : 2;
 }
 
 }  // namespace n2b
@@ -119,7 +122,7 @@ extern "C" int neus2b_linear_forward(const neus2b_linear_desc* desc, const void*
 	Epilogue& e = p.e;
 	e.out = d_y, e.out_ld = y_stride, e.bias = d_bias, e.add = d_residual, e.add_ld = residual_stride;
 	e.preact = d_preact, e.preact_ld = preact_stride, e.act = (int)desc->activation;
-	e.vec = whole_vectors(e, out);
+	e.vec = widest_access(e, out);
 	if (narrow_fits(p, false, nullptr)) return run_narrow(p, false, nullptr, stream);
 	return run_product(p, stream);
 }
@@ -205,7 +208,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 		w.M = out, w.N = d_wgrad ? in : sums_only_width(out), w.K = n;
 		w.a_mn = w.b_mn = true;
 		w.e.out = d_wgrad, w.e.out_ld = in, w.e.out_f32 = 1, w.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
-		w.e.vec = whole_vectors(w.e, in);
+		w.e.vec = widest_access(w.e, in);
 		w.column_sums = d_bgrad;
 		w.workspace = at, w.workspace_bytes = workspace_bytes - (uint64_t)(at - (char*)d_workspace);
 	}
@@ -214,7 +217,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	x.a_mn = false, x.b_mn = true;
 	x.e.out = d_dL_dx, x.e.out_ld = dx_stride, x.e.add = d_skip, x.e.add_ld = skip_stride;
 	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE) x.e.slope_z = d_below_preact, x.e.slope_ld = below_stride, x.e.act = (int)below_activation;
-	x.e.vec = whole_vectors(x.e, in);
+	x.e.vec = widest_access(x.e, in);
 	if ((params || d_dL_dx) && narrow_fits(x, true, params ? &w : nullptr)) return run_narrow(x, true, params ? &w : nullptr, stream);
 	if (params)
 		if (int rc = run_weight_gradient(w, stream)) return rc;

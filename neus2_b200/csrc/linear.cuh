@@ -14,7 +14,7 @@ struct Epilogue {
 	void* preact;
 	uint64_t preact_ld;
 	int act, out_f32, accumulate;
-	int vec;  // rows and bias start on 16-byte boundaries everywhere
+	int vec;  // bytes of an access that every row and the bias allow: 16, 4 (16-bit matrices) or less
 };
 
 // sum over k of a(m, k) b(n, k).  *_mn: the operand is stored with m (n) contiguous, [k][m], instead of [m][k].

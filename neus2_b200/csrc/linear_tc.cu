@@ -158,13 +158,21 @@ struct Shape {
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return (uint32_t)(row * 64 + ((unit ^ ((row >> 1) & 3)) << 4)); }
 __device__ __forceinline__ void chunk_fetch(uint32_t chunk, const void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols, int vec, int lane) {
 	const uint16_t* p = (const uint16_t*)base;
-	if (vec) {
+	if (vec == 16) {
 		const uint32_t r0 = row0 + (lane >> 2), c = col0 + (lane & 3) * 8;
 		const uint16_t* q = p + (uint64_t)r0 * ld + c;
 #pragma unroll
 		for (int i = 0; i < 4; ++i, q += 8 * ld)
 			if (r0 + 8 * i < rows && c < cols)
 				asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(chunk + unit_at(i * 8 + (lane >> 2), lane & 3)), "l"(q) : "memory");
+	} else if (vec == 4) {  // two rows an instruction
+		const uint32_t c = col0 + (lane & 15) * 2;
+		uint32_t r = lane >> 4;
+		const uint16_t* q = p + (uint64_t)(row0 + r) * ld + c;
+#pragma unroll 4
+		for (; r < 32; r += 2, q += 2 * ld)
+			if (row0 + r < rows && c < cols)
+				asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(chunk + unit_at(r, (lane & 15) >> 2) + (lane & 3) * 4), "l"(q) : "memory");
 	} else {
 		const uint16_t* q = p + (uint64_t)row0 * ld + col0 + lane;
 #pragma unroll
@@ -193,13 +201,22 @@ __device__ __forceinline__ void chunk_store(const uint32_t (&row)[16], void* bas
 	for (int u = 0; u < 4; ++u)
 		*reinterpret_cast<uint4*>(chunk + unit_at(lane, u)) = make_uint4(row[4 * u], row[4 * u + 1], row[4 * u + 2], row[4 * u + 3]);
 	__syncwarp();
-	if (vec) {
+	if (vec == 16) {
 		const uint32_t r0 = row0 + (lane >> 2), c = col0 + (lane & 3) * 8;
 		uint16_t* q = p + (uint64_t)r0 * ld + c;
 #pragma unroll
 		for (int i = 0; i < 4; ++i, q += 8 * ld) {
 			const uint4 v = *reinterpret_cast<const uint4*>(chunk + unit_at(i * 8 + (lane >> 2), lane & 3));
 			if (r0 + 8 * i < rows && c < cols) *reinterpret_cast<uint4*>(q) = v;
+		}
+	} else if (vec == 4) {
+		const uint32_t c = col0 + (lane & 15) * 2;
+		uint32_t r = lane >> 4;
+		uint16_t* q = p + (uint64_t)(row0 + r) * ld + c;
+#pragma unroll 4
+		for (; r < 32; r += 2, q += 2 * ld) {
+			const uint32_t v = *reinterpret_cast<const uint32_t*>(chunk + unit_at(r, (lane & 15) >> 2) + (lane & 3) * 4);
+			if (row0 + r < rows && c < cols) *reinterpret_cast<uint32_t*>(q) = v;
 		}
 	} else {
 		uint16_t* q = p + (uint64_t)row0 * ld + col0 + lane;
@@ -219,7 +236,7 @@ __device__ __forceinline__ void sums_store(const float (&v)[32], const Epilogue&
 	for (int u = 0; u < 8; ++u)
 		*reinterpret_cast<float4*>(chunk + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
 	__syncwarp();
-	if (e.vec && col0 + 32 <= cols) {
+	if (e.vec == 16 && col0 + 32 <= cols) {
 		float* o = (float*)e.out + (uint64_t)(row0 + (lane >> 3)) * e.out_ld + col0 + (lane & 7) * 4;
 #pragma unroll 4
 		for (int r = lane >> 3; r < 32; r += 4, o += 4 * e.out_ld) {
@@ -460,7 +477,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 					e.out = p.partial + (uint64_t)split * p.M * p.N;
 					e.out_ld = p.N;
 					e.accumulate = 0;
-					e.vec = (p.N & 3u) == 0;
+					e.vec = (p.N & 3u) == 0 ? 16 : 4;
 				}
 #pragma unroll
 				for (int c = 0; c < kCols; c += 32) {
@@ -514,7 +531,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 					if (c + 32 >= kCols) release();
 					if (e.bias) {
 						const uint16_t* b = (const uint16_t*)e.bias;
-						if (e.vec && col + 32 <= p.N) {
+						if (e.vec == 16 && col + 32 <= p.N) {
 #pragma unroll
 							for (int i = 0; i < 4; ++i) {
 								const uint4 w = __ldg(reinterpret_cast<const uint4*>(b + col) + i);
