@@ -55,7 +55,7 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
 		             : "memory");
 }
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+	asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
