@@ -470,6 +470,43 @@ def test_streams_and_graph(ops):
         first = [v.clone() for v in block()]
 
 
+@pytest.mark.parametrize("t", HALF, ids=["f16", "bf16"])
+def test_residual_block_and_clipping(ops, t):
+    """h + W2 gelu(W1 LN(h) + b1) + b2 forward and backward as a user chains the calls, then clipping, against autograd in 64 bits.  Norms of
+    differences: a result is behind at most six roundings to the type (u, z, a, dz, du, dh), each at most eps / 2 of its value; the factors
+    between them (slopes, projections of the norm) do not enlarge a norm, the slopes of a rounded z add one more."""
+    from neus2_b200 import _lib as L
+    g = gen(5)
+    n, width, hidden = 300, 256, 520
+    h, dh1 = rows(g, n, width, t), rows(g, n, width, t)
+    gamma, beta = 1 + 0.1 * torch.randn(width, device="cuda", generator=g), 0.1 * torch.randn(width, device="cuda", generator=g)
+    w1, w2 = rows(g, hidden, width, t, 0.06), rows(g, width, hidden, t, 0.04)
+    b1, b2 = rows(g, 1, hidden, t, 0.3)[0], rows(g, 1, width, t, 0.3)[0]
+    u, mean, rstd = ops.layer_norm_forward(h, gamma, beta, want_stats=True)
+    a, z = ops.linear_forward(u, w1, b1, activation=L.ACT_GELU, want_preact=True)
+    h1 = ops.linear_forward(a, w2, b2, residual=h)
+    dz, gw2, gb2 = ops.linear_backward(a, w2, dh1, below_activation=L.ACT_GELU, below_preact=z)
+    du, gw1, gb1 = ops.linear_backward(u, w1, dz)
+    dh, ggamma, gbeta = ops.layer_norm_backward(h, gamma, mean, rstd, du, skip=dh1)
+    leaves = [v.double().requires_grad_() for v in (h, gamma, beta, w1, b1, w2, b2)]
+    H, G, B, W1, B1, W2, B2 = leaves
+    centred = H - H.mean(1, keepdim=True)
+    U = centred / torch.sqrt((centred * centred).mean(1, keepdim=True) + 1e-5) * G + B
+    Z = U @ W1.T + B1
+    Y = 0.5 * Z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (Z + 0.044715 * Z ** 3))) @ W2.T + B2 + H
+    Y.backward(dh1.double())
+    bound = 7 * torch.finfo(t).eps / 2
+    for name, got, want in [("h1", h1, Y.detach()), ("dh", dh, H.grad), ("ggamma", ggamma, G.grad), ("gbeta", gbeta, B.grad), ("gw1", gw1, W1.grad),
+                            ("gb1", gb1, B1.grad), ("gw2", gw2, W2.grad), ("gb2", gb2, B2.grad)]:
+        assert float((got.double() - want).norm() / want.norm()) <= bound, name
+    grads = [gw2, gb2, gw1, gb1, ggamma, gbeta]
+    before = [v.clone() for v in grads]
+    norm = math.sqrt(sum(float((v.double() ** 2).sum()) for v in before))
+    got_norm, factor = ops.GradientSet(grads).clip(max_norm=norm / 3).tolist()
+    assert abs(got_norm / norm - 1) <= 2.0 ** -22 and abs(factor * 3 - 1) <= 2.0 ** -21
+    assert all(torch.equal(v, u * factor) for v, u in zip(grads, before))
+
+
 def test_two_streams_at_once(ops):
     """Calls of every kind issued to two streams in turn, without waiting in between, give the bits that they give one after another."""
     g = gen(77)
