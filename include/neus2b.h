@@ -425,7 +425,7 @@ int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, const void* d_
                               void* d_y, uint64_t y_stride, float* d_mean, float* d_rstd, neus2b_stream_t stream);
 /* d_dL_dx = rstd (a - mean(a) - xhat mean(a xhat)) + skip with a = gamma dL/dy, xhat = (x - mean) rstd; d_dgamma (+)= sum over n of
  * dL/dy xhat, d_dbeta (+)= sum over n of dL/dy.  d_dL_dx, d_dgamma, d_dbeta, d_skip may each be NULL; d_dL_dx may be d_dL_dy or d_skip.
- * The workspace is like that of neus2b_linear_backward. */
+ * The workspace is like that of neus2b_linear_backward; without d_dgamma and d_dbeta none is needed. */
 int neus2b_layer_norm_backward_workspace(const neus2b_layer_norm_desc* desc, uint64_t* bytes);
 int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, const void* d_x, uint64_t x_stride, const void* d_gamma, const float* d_mean,
                                const float* d_rstd, const void* d_dL_dy, uint64_t dy_stride, const void* d_skip, uint64_t skip_stride,

@@ -788,6 +788,7 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 	if (int rc = neus2b_layer_norm_backward_workspace(desc, &need)) return rc;
 	if (grad_mode < NEUS2B_GRAD_IGNORE || grad_mode > NEUS2B_GRAD_ACCUMULATE) return NEUS2B_E_INVALID;
 	if (grad_mode == NEUS2B_GRAD_IGNORE) d_dgamma = d_dbeta = nullptr;
+	if (!d_dgamma && !d_dbeta) need = 0;  // the workspace is theirs
 	const uint32_t n = desc->n, width = desc->width;
 	const size_t b = dtype_bytes(desc->dtype);
 	if (((uintptr_t)d_dgamma | (uintptr_t)d_dbeta | (uintptr_t)d_mean | (uintptr_t)d_rstd) & 3) return NEUS2B_E_INVALID;

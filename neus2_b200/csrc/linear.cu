@@ -157,6 +157,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	if (below_activation > NEUS2B_ACT_SILU || grad_mode < NEUS2B_GRAD_IGNORE || grad_mode > NEUS2B_GRAD_ACCUMULATE) return NEUS2B_E_INVALID;
 	const uint32_t n = desc->n, in = desc->in_width, out = desc->out_width;
 	if (grad_mode == NEUS2B_GRAD_IGNORE) d_wgrad = d_bgrad = nullptr;
+	if (!d_wgrad && !d_bgrad) need = dz_bytes(desc);
 	if (((uintptr_t)d_wgrad | (uintptr_t)d_bgrad) & 3) return NEUS2B_E_INVALID;
 	if (n == 0) {
 		if (grad_mode == NEUS2B_GRAD_OVERWRITE) {

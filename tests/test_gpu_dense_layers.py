@@ -294,6 +294,33 @@ def test_layer_norm(ops, shape, t):
         R.within(f"dbeta {k}", db, wb, eb)
 
 
+@pytest.mark.parametrize("shape", [(1, 100), (9, 1024), (32, 1111), (32, 4096), (33, 1111), (200, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_layer_norm_backward_parts(ops, shape):
+    """Parameter gradients without dL/dx, dL/dx without them, one of the two alone: the bits of the whole call."""
+    from neus2_b200 import _lib as L
+    n, width = shape
+    t = torch.bfloat16
+    g = gen(width)
+    x, dy = rows(g, n, width, t), rows(g, n, width, t)
+    gamma = torch.randn(width, device="cuda", generator=g)
+    _, mean, rstd = ops.layer_norm_forward(x, gamma, want_stats=True)
+    dx, dg, db = ops.layer_norm_backward(x, gamma, mean, rstd, dy)
+    none, dg1, db1 = ops.layer_norm_backward(x, gamma, mean, rstd, dy, want_din=False)
+    assert none is None and torch.equal(dg, dg1) and torch.equal(db, db1)
+    dx2, none, _ = ops.layer_norm_backward(x, gamma, mean, rstd, dy, mode=L.GRAD_IGNORE)
+    assert none is None and torch.equal(dx, dx2)
+    lib, d, need = L.lib(), L.LayerNormDesc(n, width, 2, 0, 1e-5), C.c_uint64(0)
+    L.check(lib.neus2b_layer_norm_backward_workspace(C.byref(d), C.byref(need)))
+    ws = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+    for which in (0, 1):
+        out = torch.full((width + 2,), 7.0, device="cuda")
+        at = out[1:].data_ptr()
+        L.check(lib.neus2b_layer_norm_backward(C.byref(d), x.data_ptr(), width, gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), width, None, 0,
+                                               None, 0, None if which else at, at if which else None, L.GRAD_OVERWRITE, ws.data_ptr(), need.value,
+                                               torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out[1:-1], db if which else dg) and float(out[0]) == float(out[-1]) == 7.0
+
+
 def test_layer_norm_rows_far_from_zero_and_constant(ops):
     """A mean a thousand times the spread costs no accuracy beyond the inputs' own; constant rows give beta."""
     g = gen(4)
