@@ -321,6 +321,49 @@ def test_layer_norm_backward_parts(ops, shape):
         assert torch.equal(out[1:-1], db if which else dg) and float(out[0]) == float(out[-1]) == 7.0
 
 
+@pytest.mark.parametrize("shape", [(9, 1024), (33, 1111), (300, 4096), (4000, 64), (5, 20001)], ids=lambda s: "x".join(map(str, s)))
+def test_layer_norm_backward_in_place(ops, shape):
+    """dL/dx in the place of dL/dy, or of the skip connection's gradient."""
+    from neus2_b200 import _lib as L
+    n, width = shape
+    g = gen(width + 1)
+    x, dy, skip = rows(g, n, width, torch.float16), rows(g, n, width, torch.float16), rows(g, n, width, torch.float16)
+    gamma = torch.randn(width, device="cuda", generator=g)
+    _, mean, rstd = ops.layer_norm_forward(x, gamma, want_stats=True)
+    want = ops.layer_norm_backward(x, gamma, mean, rstd, dy, skip=skip)
+    lib, d, need = L.lib(), L.LayerNormDesc(n, width, 1, 0, 1e-5), C.c_uint64(0)
+    L.check(lib.neus2b_layer_norm_backward_workspace(C.byref(d), C.byref(need)))
+    ws = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+    for k in (0, 1):
+        y, s = dy.clone(), skip.clone()
+        dg, db = torch.empty(width, device="cuda"), torch.empty(width, device="cuda")
+        out = s if k else y
+        L.check(lib.neus2b_layer_norm_backward(C.byref(d), x.data_ptr(), width, gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(), y.data_ptr(), width,
+                                               s.data_ptr(), width, out.data_ptr(), width, dg.data_ptr(), db.data_ptr(), L.GRAD_OVERWRITE, ws.data_ptr(),
+                                               need.value, torch.cuda.current_stream().cuda_stream))
+        assert all(torch.equal(u, v) for u, v in zip((out, dg, db), want)), k
+
+
+@pytest.mark.parametrize("shape", [(20, 300, 100), (1000, 64, 64), (1000, 512, 256), (500, 333, 77), (300, 2056, 120), (5000, 1024, 1024)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_linear_backward_in_place(ops, shape):
+    """dL/dx in the place of the skip connection's gradient."""
+    from neus2_b200 import _lib as L
+    n, i, o = shape
+    g = gen(i + o)
+    t = torch.bfloat16
+    x, dy, zb, skip, w = rows(g, n, i, t), rows(g, n, o, t, 0.1), rows(g, n, i, t), rows(g, n, i, t, 0.1), rows(g, o, i, t, 0.1)
+    want = ops.linear_backward(x, w, dy, below_activation=R.GELU, below_preact=zb, skip=skip)
+    lib, d, need = L.lib(), L.LinearDesc(n, i, o, 2, 0), C.c_uint64(0)
+    L.check(lib.neus2b_linear_backward_workspace(C.byref(d), 1, C.byref(need)))
+    ws = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+    out, dw, db = skip.clone(), torch.empty((o, i), device="cuda"), torch.empty(o, device="cuda")
+    L.check(lib.neus2b_linear_backward(C.byref(d), x.data_ptr(), i, w.data_ptr(), None, 0, dy.data_ptr(), o, L.ACT_GELU, zb.data_ptr(), i, out.data_ptr(), i,
+                                       out.data_ptr(), i, dw.data_ptr(), db.data_ptr(), L.GRAD_OVERWRITE, ws.data_ptr(), need.value,
+                                       torch.cuda.current_stream().cuda_stream))
+    assert all(torch.equal(u, v) for u, v in zip((out, dw, db), want))
+
+
 def test_layer_norm_rows_far_from_zero_and_constant(ops):
     """A mean a thousand times the spread costs no accuracy beyond the inputs' own; constant rows give beta."""
     g = gen(4)
