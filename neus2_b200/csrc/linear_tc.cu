@@ -153,8 +153,8 @@ struct Shape {
 
 // ---- 32 x 32 values of a matrix between global memory and registers, through 2 KB of shared memory of a warp.  Global memory is read
 // (asynchronously) and written in whole row segments (64 bytes), a thread computes on one row.  Where rows do not start on 16-byte
-// boundaries a thread moves one column's values one by one: still one segment of a row per instruction.  The 16-byte units of a row
-// are permuted so that neither side's accesses collide.
+// boundaries a thread moves two of its entries (rows on 4-byte boundaries) or one: still whole segments of rows per instruction.  The
+// 16-byte units of a row are permuted so that neither side's accesses collide.
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return (uint32_t)(row * 64 + ((unit ^ ((row >> 1) & 3)) << 4)); }
 __device__ __forceinline__ void chunk_fetch(uint32_t chunk, const void* base, uint64_t ld, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t cols, int vec, int lane) {
 	const uint16_t* p = (const uint16_t*)base;
@@ -813,7 +813,7 @@ static int product_of(const Product& p, cudaStream_t stream) {
 
 // Weight gradient: tiles of out_width x in_width, k the samples.  Few tiles share the samples out over the SMs and are joined afterwards.
 // One CTA's 128 x 128 tile takes about 430 cycles for 64 samples (its operands' way through shared memory), a pair's 256 x 256 tile 512
-// (its MMAs) and, where the column sums are wanted, the pass over dz that takes them and its join: 6 us and 4 TB/s.  The plan with the
+// (its MMAs) and, where the column sums are wanted, the pass over dz that takes them: 4 us and 4 TB/s.  The plan with the
 // fewest cycles is taken.  Parts are joined by a pass of their own (6000 cycles with its launch), or, where a cluster's CTAs are enough parts,
 // through its shared memory (3000): 1328 samples, 160 -> 192: 14.1 us for the whole backward pass, 16.9 with a pass of its own.
 struct WgradPlan {
@@ -829,7 +829,7 @@ static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair, b
 		const uint64_t tiles = (uint64_t)tiles_of(M, size) * tiles_of(N, size), fill = slots / tiles, most = kblocks / kChunk;
 		const uint64_t splits = fill < most ? (fill ? fill : 1) : (most ? most : 1);
 		const uint64_t cycles = (tiles * splits + slots - 1) / slots * ((kblocks + splits - 1) / splits) * (pair ? 512 : 430) +
-		                        (splits > 1 ? 6000 : 0) + (pair && sums ? 11000 + (uint64_t)K * M / 1000 : 0);
+		                        (splits > 1 ? 6000 : 0) + (pair && sums ? 8000 + (uint64_t)K * M / 1000 : 0);
 		if (!pair || cycles < best) {
 			best = cycles;
 			plan = WgradPlan{pair != 0, tiles_of(M, size), tiles_of(N, size), (uint32_t)splits, 1};
@@ -843,53 +843,75 @@ static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair, b
 	}
 	return plan;
 }
-// blocks of rows that the column sums of a pair's plan are taken in, at most
-static uint32_t sum_blocks(uint32_t cols) {
-	const uint32_t by = 4 * kSMs / tiles_of(cols, 256);
-	return by ? by : 1;
-}
 static uint64_t plan_bytes(const WgradPlan& w, uint32_t M, uint32_t N) {
-	const uint64_t partial = w.splits > 1 && w.cluster == 1 ? (uint64_t)w.splits * ((uint64_t)M * N + M) * 4 : 0, sums = w.pair ? (uint64_t)sum_blocks(M) * M * 4 : 0;
-	return partial > sums ? partial : sums;
+	return w.splits > 1 && w.cluster == 1 ? (uint64_t)w.splits * ((uint64_t)M * N + M) * 4 : 0;
 }
 
-// Column sums of a [rows][cols] matrix with rows on 16-byte boundaries: block (x, y) takes 256 columns and every gridDim.y-th group of 8
-// rows, a thread 8 columns; its 8 warps are joined in order.  partial [gridDim.y][cols].  8192 x 1024 bf16 with the join: 8 us, launches and the
-// read of 17 MB.
-__global__ void __launch_bounds__(256) column_sums_kernel(const uint16_t* __restrict__ a, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t bf16,
-                                                          float* __restrict__ partial) {
-	__shared__ float s[8][32][9];
+// Column sums of a [rows][cols] matrix with rows on 16-byte boundaries.  A cluster of 8 blocks takes COLS columns, its blocks every 8th group of
+// rows, a thread 8 columns; rows of a warp are joined by shuffles, warps and blocks in order through shared memory.  Bound by the read: 8192
+// x 1024 bf16 6 us (two launches with partial sums between them 7.6).
+template <int COLS>
+__global__ void __launch_bounds__(512) column_sums_kernel(const uint16_t* __restrict__ a, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t bf16,
+                                                          float* __restrict__ out, int accumulate) {
+	constexpr int kAcross = COLS / 8, kDown = 512 / kAcross;  // threads of a row, rows of a block
+	__shared__ float s[16][COLS], block[COLS];
 	wait_for_previous();
 	let_next_start();
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-	const uint32_t c = blockIdx.x * 256 + lane * 8;
+	const uint32_t first = blockIdx.x / 8 * COLS, c = first + threadIdx.x % kAcross * 8, rank = cluster_rank();
 	const bool bf = bf16 != 0;
 	float v[8] = {};
 	if (c + 8 <= cols) {
-#pragma unroll 4
-		for (uint32_t r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
-			const uint4 q = __ldg(reinterpret_cast<const uint4*>(a + (uint64_t)r * ld + c));
-			const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+		for (uint32_t r = rank * kDown + threadIdx.x / kAcross; r < rows; r += 8 * kDown * 8) {
+			uint4 q[8];  // on their way together
 #pragma unroll
-			for (int i = 0; i < 4; ++i) {
-				const float2 f = unpack2(w[i], bf);
-				v[2 * i] += f.x, v[2 * i + 1] += f.y;
+			for (uint32_t k = 0; k < 8; ++k) {
+				const uint32_t at = r + k * 8 * kDown;
+				q[k] = at < rows ? __ldg(reinterpret_cast<const uint4*>(a + (uint64_t)at * ld + c)) : make_uint4(0, 0, 0, 0);
+			}
+#pragma unroll
+			for (uint32_t k = 0; k < 8; ++k) {
+				const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+#pragma unroll
+				for (int i = 0; i < 4; ++i) {
+					const float2 f = unpack2(w[i], bf);
+					v[2 * i] += f.x, v[2 * i + 1] += f.y;
+				}
 			}
 		}
 	} else if (c < cols) {
-		for (uint32_t r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8)
-			for (uint32_t i = 0; c + i < cols; ++i) v[i] += h2f(a[(uint64_t)r * ld + c + i], bf);
-	}
+		for (uint32_t r = rank * kDown + threadIdx.x / kAcross; r < rows; r += 8 * kDown)
 #pragma unroll
-	for (int i = 0; i < 8; ++i) s[warp][lane][i] = v[i];
+			for (uint32_t i = 0; i < 8; ++i)
+				if (c + i < cols) v[i] += h2f(a[(uint64_t)r * ld + c + i], bf);
+	}
+	__syncwarp();
+#pragma unroll
+	for (int i = 0; i < 8; ++i) {
+#pragma unroll
+		for (int o = kAcross; o < 32; o *= 2) v[i] += __shfl_xor_sync(~0u, v[i], o);
+		if (lane < kAcross) s[warp][lane * 8 + i] = v[i];
+	}
 	__syncthreads();
-	const uint32_t col = threadIdx.x;
-	if (blockIdx.x * 256 + col < cols) {
+	if (threadIdx.x < COLS) {
 		float t = 0.f;
 #pragma unroll
-		for (int k = 0; k < 8; ++k) t += s[k][col >> 3][col & 7];
-		partial[(uint64_t)blockIdx.y * cols + blockIdx.x * 256 + col] = t;
+		for (int k = 0; k < 16; ++k) t += s[k][threadIdx.x];
+		block[threadIdx.x] = t;
 	}
+	__syncthreads();
+	cluster_sync();
+	if (rank == 0 && threadIdx.x < COLS && first + threadIdx.x < cols) {
+		float part[8], t = 0.f;
+#pragma unroll
+		for (int k = 0; k < 8; ++k) part[k] = load_peer(sptr(block + threadIdx.x), k);
+#pragma unroll
+		for (int k = 0; k < 8; ++k) t += part[k];
+		float* const o = out + first + threadIdx.x;
+		*o = accumulate ? *o + t : t;
+	}
+	__syncwarp();
+	cluster_sync();  // (before the other blocks' memory goes)
 }
 
 }  // namespace lin
@@ -966,9 +988,11 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 		// a pair's accumulators fill the tensor memory: the column sums are taken by a pass of their own, ahead of the product, which then
 		// finds the matrix in the L2
 		if (p.column_sums) {
-			const uint32_t most = sum_blocks(p.M), need = tiles_of(p.K, 32), by = need < most ? need : most;
-			if (int rc = launch_behind(column_sums_kernel, dim3(tiles_of(p.M, 256), by), 256, 0, stream, a.a, a.a_ld, p.K, p.M, a.bf16, (float*)p.workspace)) return rc;
-			if (int rc = run_join((const float*)p.workspace, by, p.M, 0, nullptr, p.column_sums, p.e.accumulate, stream)) return rc;
+			// narrow matrices are shared out over as many SMs by fewer columns a cluster
+			const uint32_t cols = p.M >= 1024 ? 64 : p.M >= 512 ? 32 : 16;
+			auto kernel = cols == 64 ? column_sums_kernel<64> : cols == 32 ? column_sums_kernel<32> : column_sums_kernel<16>;
+			if (int rc = launch_behind_in_clusters(8, kernel, 8 * tiles_of(p.M, cols), 512, 0, stream, a.a, a.a_ld, p.K, p.M, a.bf16, p.column_sums, p.e.accumulate))
+				return rc;
 		}
 		const uint32_t pairs = (uint32_t)(units < (uint64_t)(kSMs / 2) ? units : kSMs / 2);
 		if (int rc = launch<256, true, true, false, true, true>(a, 2 * pairs, stream)) return rc;

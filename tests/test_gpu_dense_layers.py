@@ -46,7 +46,7 @@ SHAPES = [(1, 1, 1), (1, 16, 16), (2, 7, 5), (1, 4096, 264), (7, 1024, 129), (16
           (65, 128, 256), (128, 64, 128), (129, 1000, 333), (200, 8, 2048), (257, 72, 520), (700, 31, 3), (1000, 4100, 24), (3000, 48, 64),
           (5000, 64, 16), (512, 2048, 1536), (2600, 136, 2100), (9472, 23, 512), (100, 40, 37888), (1500, 128, 40),
           (1111, 56, 120), (300, 8, 100), (100000, 64, 64), (3, 24, 40000), (50, 7, 38000), (100, 520, 512), (300, 2056, 120), (5000, 513, 947), (70, 40, 7000),
-          (20, 6000, 130)]
+          (20, 6000, 130), (6000, 8192, 300), (8192, 2100, 600), (8192, 2100, 1030)]
 
 
 @pytest.mark.parametrize("t", HALF, ids=["f16", "bf16"])
