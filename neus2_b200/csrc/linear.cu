@@ -203,10 +203,9 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	Product w{}, x{};  // the weight gradient, the input gradient
 	w.bf16 = x.bf16 = desc->dtype == NEUS2B_BF16;
 	w.a = x.a = dz, w.a_ld = x.a_ld = dz_ld;
-	if (params) {
-		// without a weight gradient the column sums ride on a product of dz with its own first columns that is not stored
-		w.b = d_wgrad ? xs : dz, w.b_ld = d_wgrad ? xs_ld : dz_ld;
-		w.M = out, w.N = d_wgrad ? in : sums_only_width(out), w.K = n;
+	if (d_wgrad) {
+		w.b = xs, w.b_ld = xs_ld;
+		w.M = out, w.N = in, w.K = n;
 		w.a_mn = w.b_mn = true;
 		w.e.out = d_wgrad, w.e.out_ld = in, w.e.out_f32 = 1, w.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
 		w.e.vec = widest_access(w.e, in);
@@ -219,8 +218,10 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	x.e.out = d_dL_dx, x.e.out_ld = dx_stride, x.e.add = d_skip, x.e.add_ld = skip_stride;
 	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE) x.e.slope_z = d_below_preact, x.e.slope_ld = below_stride, x.e.act = (int)below_activation;
 	x.e.vec = widest_access(x.e, in);
-	if ((params || d_dL_dx) && narrow_fits(x, true, params ? &w : nullptr)) return run_narrow(x, true, params ? &w : nullptr, stream);
-	if (params)
+	if (d_bgrad && !d_wgrad)
+		if (int rc = run_column_sums(dz, dz_ld, n, out, w.bf16, d_bgrad, grad_mode == NEUS2B_GRAD_ACCUMULATE, stream)) return rc;
+	if ((d_wgrad || d_dL_dx) && narrow_fits(x, true, d_wgrad ? &w : nullptr)) return run_narrow(x, true, d_wgrad ? &w : nullptr, stream);
+	if (d_wgrad)
 		if (int rc = run_weight_gradient(w, stream)) return rc;
 	if (d_dL_dx)
 		if (int rc = run_product(x, stream)) return rc;

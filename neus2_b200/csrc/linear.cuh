@@ -35,10 +35,10 @@ __device__ __forceinline__ uint16_t f2h(float v, bool bf) {
 	return bf ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// width of the product that carries the column sums where no weight gradient is wanted (it is not stored)
-inline uint32_t sums_only_width(uint32_t out_width) { return out_width < 64u ? out_width : 64u; }
+// sum over the rows of a [rows][cols] matrix with rows on 16-byte boundaries
+int run_column_sums(const void* a, uint64_t ld, uint32_t rows, uint32_t cols, bool bf16, float* out, int accumulate, cudaStream_t stream);
 uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n);
-// sums of `splits` parts [M][N] (to out, if not null) and, behind all of them, of `splits` parts [M] (to sums, if not null)
+// sums of `splits` parts [M][N] (to out) and, behind all of them, of `splits` parts [M] (to sums, if not null)
 int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream);
 // Results of up to 64 columns (linear_narrow.cu).  forward or input gradient: `rows` the product for dL/dx or y, `weights` null or the
 // weight gradient that shares its first operand.

@@ -356,7 +356,7 @@ bool narrow_fits(const Product& r, bool backward, const Product* w) {
 	auto fine = [](const void* p, uint64_t ld) { return !p || tma_ok(p, ld); };
 	if (!tma_ok(r.a, r.a_ld)) return false;
 	if (e.out && !(tma_ok(r.b, r.b_ld) && tma_ok(e.out, e.out_ld) && fine(e.slope_z, e.slope_ld) && fine(e.add, e.add_ld) && fine(e.preact, e.preact_ld))) return false;
-	if (w && !(tma_ok(w->b, w->b_ld) && w->e.out)) return false;
+	if (w && !tma_ok(w->b, w->b_ld)) return false;
 	return backward || !w;
 }
 uint64_t narrow_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {

@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 				}
 #pragma unroll
 				for (int c = 0; c < kCols; c += 32) {
-					if (!p.e.out || n0 + c >= p.N) break;
+					if (n0 + c >= p.N) break;
 					float v[32];
 #pragma unroll
 					for (int i = 0; i < 32; ++i) v[i] = acc[c + i];
@@ -642,7 +642,6 @@ __global__ void __launch_bounds__(Shape<BN, AMN, BMN, SWAP, WGRAD, PAIR>::kThrea
 			for (int k = 0; k < 2; ++k) {
 				if (!in[k]) continue;
 				if (WGRAD) {
-					if (!e.out) continue;
 					float* const o = (float*)e.out + sample[k] * e.out_ld + feature[k];
 					*o = e.accumulate ? *o + v[k] : v[k];
 					continue;
@@ -673,8 +672,8 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
 	extern __shared__ float s[];  // [blockDim.y][VEC][blockDim.x]
 	let_next_start();
 	wait_for_previous();
-	const uint64_t n = (uint64_t)M * N, groups = n / VEC, first = out ? 0 : groups, total = groups + (sums ? M : 0);
-	for (uint64_t base = first + (uint64_t)blockIdx.x * blockDim.x; base < total; base += (uint64_t)gridDim.x * blockDim.x) {
+	const uint64_t n = (uint64_t)M * N, groups = n / VEC, total = groups + (sums ? M : 0);
+	for (uint64_t base = (uint64_t)blockIdx.x * blockDim.x; base < total; base += (uint64_t)gridDim.x * blockDim.x) {
 		const uint64_t i = base + threadIdx.x;
 		const bool is_sum = i >= groups;
 		float v[VEC] = {};
@@ -820,11 +819,11 @@ struct WgradPlan {
 	bool pair;
 	uint32_t tiles_m, tiles_n, splits, cluster;
 };
-static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool may_pair, bool sums) {  // (a pair's kernel always stores the product)
+static WgradPlan wgrad_plan(uint32_t M, uint32_t N, uint32_t K, bool sums) {
 	const uint32_t kblocks = tiles_of(K, kBK);
 	uint64_t best = 0;
 	WgradPlan plan{};
-	for (int pair = 0; pair <= (may_pair ? 1 : 0); ++pair) {
+	for (int pair = 0; pair < 2; ++pair) {
 		const uint32_t size = pair ? 256 : 128, slots = pair ? kSMs / 2 : kSMs;
 		const uint64_t tiles = (uint64_t)tiles_of(M, size) * tiles_of(N, size), fill = slots / tiles, most = kblocks / kChunk;
 		const uint64_t splits = fill < most ? (fill ? fill : 1) : (most ? most : 1);
@@ -951,18 +950,21 @@ int run_realign(const Operand* ops, int count, cudaStream_t stream) {
 int run_product(const Product& p, cudaStream_t stream) { return p.b_mn ? product_of<true>(p, stream) : product_of<false>(p, stream); }
 
 uint64_t wgrad_workspace(uint32_t out_width, uint32_t in_width, uint32_t n) {
-	// whether the product or the column sums alone are wanted is not known here
-	const uint32_t alone = sums_only_width(out_width);
-	const uint64_t bytes[3] = {plan_bytes(wgrad_plan(out_width, in_width, n, true, false), out_width, in_width),
-	                           plan_bytes(wgrad_plan(out_width, in_width, n, true, true), out_width, in_width),
-	                           plan_bytes(wgrad_plan(out_width, alone, n, false, true), out_width, alone)};
-	return std::max(std::max(bytes[0], bytes[1]), bytes[2]);
+	// whether the bias gradient is wanted is not known here
+	return std::max(plan_bytes(wgrad_plan(out_width, in_width, n, false), out_width, in_width), plan_bytes(wgrad_plan(out_width, in_width, n, true), out_width, in_width));
+}
+
+int run_column_sums(const void* a, uint64_t ld, uint32_t rows, uint32_t cols, bool bf16, float* out, int accumulate, cudaStream_t stream) {
+	// narrow matrices are shared out over as many SMs by fewer columns a cluster
+	const uint32_t each = cols >= 1024 ? 64 : cols >= 512 ? 32 : 16;
+	auto kernel = each == 64 ? column_sums_kernel<64> : each == 32 ? column_sums_kernel<32> : column_sums_kernel<16>;
+	return launch_behind_in_clusters(8, kernel, 8 * tiles_of(cols, each), 512, 0, stream, (const uint16_t*)a, ld, rows, cols, bf16 ? 1u : 0u, out, accumulate);
 }
 
 int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, float* out, float* sums, int accumulate, cudaStream_t stream) {
 	const uint64_t n = (uint64_t)M * N;
 	const bool vec = n % 4 == 0 && (((uintptr_t)partial | (uintptr_t)out) & 15u) == 0;
-	const uint64_t threads = (out ? (vec ? n / 4 : n) : 0) + (sums ? M : 0);
+	const uint64_t threads = (vec ? n / 4 : n) + (sums ? M : 0);
 	// threads for every part where the entries alone do not fill the SMs
 	const uint32_t rows = threads >= 512ull * kSMs || splits == 1 ? 1 : splits >= 32 && threads < 64ull * kSMs ? 32 : 8;
 	const dim3 block(rows == 1 ? 256 : 32, rows);
@@ -973,7 +975,7 @@ int run_join(const float* partial, uint32_t splits, uint32_t M, uint32_t N, floa
 }
 
 int run_weight_gradient(const Product& p, cudaStream_t stream) {
-	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, p.e.out != nullptr, p.column_sums != nullptr);
+	const WgradPlan w = wgrad_plan(p.M, p.N, p.K, p.column_sums != nullptr);
 	if (p.workspace_bytes < plan_bytes(w, p.M, p.N)) return NEUS2B_E_INVALID;
 	Args a{};
 	a.bf16 = p.bf16;
@@ -988,11 +990,7 @@ int run_weight_gradient(const Product& p, cudaStream_t stream) {
 		// a pair's accumulators fill the tensor memory: the column sums are taken by a pass of their own, ahead of the product, which then
 		// finds the matrix in the L2
 		if (p.column_sums) {
-			// narrow matrices are shared out over as many SMs by fewer columns a cluster
-			const uint32_t cols = p.M >= 1024 ? 64 : p.M >= 512 ? 32 : 16;
-			auto kernel = cols == 64 ? column_sums_kernel<64> : cols == 32 ? column_sums_kernel<32> : column_sums_kernel<16>;
-			if (int rc = launch_behind_in_clusters(8, kernel, 8 * tiles_of(p.M, cols), 512, 0, stream, a.a, a.a_ld, p.K, p.M, a.bf16, p.column_sums, p.e.accumulate))
-				return rc;
+			if (int rc = run_column_sums(p.a, p.a_ld, p.K, p.M, p.bf16, p.column_sums, p.e.accumulate, stream)) return rc;
 		}
 		const uint32_t pairs = (uint32_t)(units < (uint64_t)(kSMs / 2) ? units : kSMs / 2);
 		if (int rc = launch<256, true, true, false, true, true>(a, 2 * pairs, stream)) return rc;
