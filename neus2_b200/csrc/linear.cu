@@ -206,7 +206,6 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	if (d_wgrad) {
 		w.b = xs, w.b_ld = xs_ld;
 		w.M = out, w.N = in, w.K = n;
-		w.a_mn = w.b_mn = true;
 		w.e.out = d_wgrad, w.e.out_ld = in, w.e.out_f32 = 1, w.e.accumulate = grad_mode == NEUS2B_GRAD_ACCUMULATE;
 		w.e.vec = widest_access(w.e, in);
 		w.column_sums = d_bgrad;
@@ -214,7 +213,7 @@ extern "C" int neus2b_linear_backward(const neus2b_linear_desc* desc, const void
 	}
 	x.b = ws, x.b_ld = ws_ld;
 	x.M = n, x.N = in, x.K = out;
-	x.a_mn = false, x.b_mn = true;
+	x.b_mn = true;
 	x.e.out = d_dL_dx, x.e.out_ld = dx_stride, x.e.add = d_skip, x.e.add_ld = skip_stride;
 	if (d_dL_dx && below_activation != NEUS2B_ACT_NONE) x.e.slope_z = d_below_preact, x.e.slope_ld = below_stride, x.e.act = (int)below_activation;
 	x.e.vec = widest_access(x.e, in);

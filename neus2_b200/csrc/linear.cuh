@@ -17,12 +17,12 @@ struct Epilogue {
 	int vec;  // bytes of an access that every row and the bias allow: 16, 4 (16-bit matrices) or less
 };
 
-// sum over k of a(m, k) b(n, k).  *_mn: the operand is stored with m (n) contiguous, [k][m], instead of [m][k].
+// sum over k of a(m, k) b(n, k).  b_mn: b is stored with n contiguous, [k][n], instead of [n][k] (the weight gradient: both are).
 struct Product {
 	const void *a, *b;
 	uint64_t a_ld, b_ld;
 	uint32_t M, N, K;
-	bool a_mn, b_mn, bf16;
+	bool b_mn, bf16;
 	Epilogue e;
 	float* column_sums;      // weight gradient: sum over k of a(m, k), or null
 	void* workspace;         // weight gradient: partial sums
