@@ -333,10 +333,18 @@ def _bytes(query, desc, *flags):
     return need.value
 
 
+def _at_most(most, **sizes):
+    """Sizes that the layers take; the 32-bit fields of a descriptor would hold what is left of a larger one."""
+    for name, size in sizes.items():
+        if size > most:
+            _refuse(f"at most {most} {name}, got {size}")
+
+
 # Short calls are bound by the host: what a call derives from its sizes alone is kept with them.
 @functools.lru_cache(maxsize=1024)
 def _linear_plan(n, n_in, n_out, dtype, activation, backward, unaligned):
     """(descriptor, workspace bytes)"""
+    _at_most(1 << 30, samples=n, inputs=n_in, outputs=n_out)
     d = L.LinearDesc(n, n_in, n_out, _DTYPES[dtype], activation)
     lib = L.lib()
     return d, _bytes(lib.neus2b_linear_backward_workspace if backward else lib.neus2b_linear_forward_workspace, d, unaligned)
@@ -344,6 +352,8 @@ def _linear_plan(n, n_in, n_out, dtype, activation, backward, unaligned):
 
 @functools.lru_cache(maxsize=1024)
 def _norm_plan(n, width, dtype, param_dtype, eps):
+    _at_most(1 << 31, samples=n)
+    _at_most(1 << 30, columns=width)
     d = L.LayerNormDesc(n, width, _DTYPES[dtype], _DTYPES[param_dtype], eps)
     return d, _bytes(L.lib().neus2b_layer_norm_backward_workspace, d)
 
@@ -372,12 +382,12 @@ def linear_forward(x, w, bias=None, residual=None, activation=L.ACT_NONE, want_p
     xp, xs = _rows(x, "x", n, n_in, t, dev)
     rp, rs = _rows(residual, "residual", n, n_out, t, dev)
     bp = _vector(bias, "bias", n_out, t, dev)
+    wp = w.data_ptr()
+    d, need = _linear_plan(n, n_in, n_out, t, activation, False, 1 if (xp | wp | xs * 2 | n_in * 2) & 15 else 0)
     if out is None:
         out = x.new_empty(n, n_out)
     yp, ys = _rows(out, "out", n, n_out, t, dev)
     z = x.new_empty(n, n_out) if want_preact else None
-    wp = w.data_ptr()
-    d, need = _linear_plan(n, n_in, n_out, t, activation, False, 1 if (xp | wp | xs * 2 | n_in * 2) & 15 else 0)
     keep, wsp, wsb = _workspace(need, workspace, x)
     L.check(L.lib().neus2b_linear_forward(C.byref(d), xp, xs, wp, bp, rp, rs, yp, ys, z.data_ptr() if want_preact else None, n_out, wsp, wsb,
                                       _raw_stream(dev)))
@@ -404,12 +414,12 @@ def linear_backward(x, w, dL_dout, activation=L.ACT_NONE, preact=None, below_act
     zp, zs = _rows(preact, "preact", n, n_out, t, dev)
     bzp, bzs = _rows(below_preact, "below_preact", n, n_in, t, dev)
     sp, ss = _rows(skip, "skip", n, n_in, t, dev)
+    wp = w.data_ptr()
+    d, need = _linear_plan(n, n_in, n_out, t, activation, True, 1 if (xp | wp | dyp | xs * 2 | n_in * 2 | dys * 2) & 15 else 0)
     din = x.new_empty(n, n_in) if want_din else None
     params = mode != L.GRAD_IGNORE
     wgrad = _gradient(wgrad, "wgrad", (n_out, n_in), mode, w, x) if params else None
     bgrad = _gradient(bgrad, "bgrad", (n_out,), mode, None, x) if params and want_bias else None
-    wp = w.data_ptr()
-    d, need = _linear_plan(n, n_in, n_out, t, activation, True, 1 if (xp | wp | dyp | xs * 2 | n_in * 2 | dys * 2) & 15 else 0)
     keep, wsp, wsb = _workspace(need, workspace, x)
     L.check(L.lib().neus2b_linear_backward(C.byref(d), xp, xs, wp, zp, zs, dyp, dys, below_activation, bzp, bzs, sp, ss,
                                        din.data_ptr() if want_din else None, n_in, wgrad.data_ptr() if params else None,
