@@ -42,14 +42,23 @@ __device__ __forceinline__ float act_value(int act, float z) {
 	if (act == NEUS2B_ACT_SILU) return z * logistic2(-kLog2e * z);
 	return z;
 }
-// d act / dz.  gelu: s + z s (1 - s) 2u' with 2u' = 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2); where z^2 is held at 1e30, s (1 - s) is 0.
+// v held to +-most, NaN as it is
+__device__ __forceinline__ float held(float v, float most) {
+	float r;
+	asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+	return r;
+}
+// d act / dz.  gelu: s + z s (1 - s) 2u' with 2u' = 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2).  Where z is held, s is exactly 0 or 1 and s (1 - s)
+// is 0: the slopes are 0 and 1 for infinite z, too (a preactivation beyond fp16's range is stored as one).
 __device__ __forceinline__ float act_slope(int act, float z) {
 	if (act == NEUS2B_ACT_RELU) return z > 0.f ? 1.f : 0.f;
 	if (act == NEUS2B_ACT_GELU) {
-		const float s = logistic2(gelu_argument(z)), z2 = fminf(z * z, 1e30f);
-		return fmaf(z * fmaf(-s, s, s), fmaf(6.f * kGeluC * kGeluA, z2, 2.f * kGeluC), s);
+		z = held(z, 1e15f);
+		const float s = logistic2(gelu_argument(z));
+		return fmaf(z * fmaf(-s, s, s), fmaf(6.f * kGeluC * kGeluA, z * z, 2.f * kGeluC), s);
 	}
 	if (act == NEUS2B_ACT_SILU) {
+		z = held(z, 1e15f);
 		const float s = logistic2(-kLog2e * z);
 		return fmaf(z, fmaf(-s, s, s), s);
 	}
