@@ -95,6 +95,38 @@ int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cuda
 	return launch_behind_in_clusters(1, kernel, grid, block, smem, stream, args...);
 }
 
+__device__ __forceinline__ uint64_t now_ns() {
+	uint64_t t;
+	asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+	return t;
+}
+// Waits for a phase of a barrier in shared memory.  False when it has not completed after `limit`, four seconds, or when `hopeless()` says
+// so: nothing that a kernel of these layers waits for takes a millisecond, and every copy that was issued has landed long before a wait
+// is given up.
+template <typename F>
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, F hopeless, uint64_t limit = 4000000000ull) {
+	uint64_t start = 0;
+	for (uint32_t it = 0;; ++it) {
+		uint32_t ok;
+		asm volatile(
+		    "{\n\t.reg .pred p;\n\t"
+		    "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+		    "selp.u32 %0, 1, 0, p;\n\t}"
+		    : "=r"(ok)
+		    : "r"(bar), "r"(parity)
+		    : "memory");
+		if (ok) return true;
+		if ((it & 63u) == 63u) {
+			const uint64_t t = now_ns();
+			if (!start) start = t;
+			else if (t - start > limit || hopeless()) return false;
+		}
+	}
+}
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
+	return wait_phase(bar, parity, [] { return false; });
+}
+
 // Blocks of a cluster and each other's shared memory
 __device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
 	uint32_t p;

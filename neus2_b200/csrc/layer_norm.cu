@@ -171,19 +171,12 @@ __device__ __forceinline__ void init_barrier(uint32_t bar) {
 __device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
 	asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// A row takes microseconds to arrive; the wait gives up after about a second, and the group goes on with what is there.
-__device__ __forceinline__ void wait_row(uint32_t bar, uint32_t parity) {
-	for (uint32_t it = 0; it < (1u << 20); ++it) {
-		uint32_t ok;
-		asm volatile(
-		    "{\n\t.reg .pred p;\n\t"
-		    "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-		    "selp.u32 %0, 1, 0, p;\n\t}"
-		    : "=r"(ok)
-		    : "r"(bar), "r"(parity)
-		    : "memory");
-		if (ok) return;
-	}
+// `given_up`: set in shared memory by the first thread of the block whose wait ran out.  From there on the block waits for no row for long,
+// orders none, and goes on with what is there, through the barriers that its other threads wait at: the call's results are void, and the
+// error flag says so.
+__device__ __forceinline__ void wait_row(uint32_t bar, uint32_t parity, volatile uint32_t& given_up) {
+	if (wait_phase(bar, parity, [&] { return given_up != 0; })) return;
+	given_up = 1;
 	atomicOr(&g_error, 1u);
 }
 template <int TPR>
@@ -213,6 +206,7 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 	constexpr bool kAhead = !F::kStaged && !RING;
 	constexpr int kMaxDepth = 4;
 	__shared__ uint64_t bars[RING ? G * kMaxDepth : 1];
+	__shared__ volatile uint32_t given_up;
 	__shared__ float2 sums[G][2 * (TPR > 32 ? TPR / 32 : 1)];
 	extern __shared__ float4 params4[];  // kStaged: gamma, beta; RING: the rings
 	float* const sg = reinterpret_cast<float*>(params4);
@@ -249,6 +243,7 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 	T* yp = y + (uint64_t)r * y_ld + t * VEC;
 	const uint64_t x_step = (uint64_t)step * x_ld, y_step = (uint64_t)step * y_ld;
 	if (kAhead) fetch(ahead, xp, r < d.n);
+	if (RING && threadIdx.x == 0) given_up = 0;
 	if (RING && t == 0) {
 		for (int i = 0; i < depth; ++i) init_barrier(sptr(&bars[group * kMaxDepth + i]));
 		for (int i = 0; i < depth; ++i) {
@@ -269,7 +264,7 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 		} else if (RING) {
 			const uint32_t bar = sptr(&bars[group * kMaxDepth + slot]);
 			unsigned char* const row = ring + (size_t)slot * row_bytes;
-			if (r < d.n) wait_row(bar, parity);
+			if (r < d.n) wait_row(bar, parity, given_up);
 #pragma unroll
 			for (int k = 0; k < VPT; ++k) {  // (a group that has no row left computes on an old one and stores nothing)
 				const uint32_t c = (k * TPR + t) * VEC;
@@ -277,7 +272,7 @@ __global__ void __launch_bounds__(Forward<T, VEC, TPR, VPT, RING>::kThreads, For
 			}
 			group_barrier<TPR>(group);  // the row is in registers: its place is free
 			const uint64_t next = (uint64_t)r + (uint64_t)depth * step;
-			if (t == 0 && next < d.n) {
+			if (t == 0 && next < d.n && !given_up) {
 				expect_bytes(bar, row_bytes);
 				copy_row(sptr(row), x + next * x_ld, row_bytes, bar);
 			}
@@ -355,6 +350,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 	using B = Backward<TPR, E, RING>;
 	constexpr int kMaxDepth = 4;
 	__shared__ uint64_t bars[RING ? B::kGroups * kMaxDepth : 1];
+	__shared__ volatile uint32_t given_up;
 	constexpr int G = B::kGroups;
 	__shared__ float2 sums[G][2 * (TPR > 32 ? TPR / 32 : 1)];
 	extern __shared__ float4 rings4[];  // the rings; afterwards, where G > 1, the threads' sums [2 E][threads]
@@ -385,6 +381,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 		copy_row(dst + row_bytes, dy + row * dy_ld, row_bytes, bar);
 		if (add) copy_row(dst + 2 * row_bytes, skip + row * skip_ld, row_bytes, bar);
 	};
+	if (RING && threadIdx.x == 0) given_up = 0;
 	if (RING && t == 0) {
 		for (int i = 0; i < depth; ++i) init_barrier(sptr(&bars[group * kMaxDepth + i]));
 		for (int i = 0; i < depth; ++i) {
@@ -400,7 +397,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 		const float m = mu, sc = rs;
 		if ((uint64_t)r + step < d.n) mu = mean[r + step], rs = rstd[r + step];  // of the next row, ahead of its turn
 		const unsigned char* const row = ring + (size_t)slot * slot_bytes;
-		if (RING && r < d.n) wait_row(sptr(&bars[group * kMaxDepth + slot]), parity);
+		if (RING && r < d.n) wait_row(sptr(&bars[group * kMaxDepth + slot]), parity, given_up);
 #pragma unroll
 		for (int k = 0; k < VPT; ++k) {  // zeros outside of the row and behind the last one: they add nothing to any sum
 			const uint32_t c = (k * TPR + t) * VEC;
@@ -415,7 +412,7 @@ __global__ void __launch_bounds__(Backward<TPR, VEC * VPT, RING>::kThreads, Back
 		if (RING) {
 			group_barrier<TPR>(group);  // the rows are in registers: their place is free
 			const uint64_t next = (uint64_t)r + (uint64_t)depth * step;
-			if (t == 0 && next < d.n) order(next, slot);
+			if (t == 0 && next < d.n && !given_up) order(next, slot);
 			if (++slot == depth) slot = 0, parity ^= 1u;
 		}
 		float s1 = 0.f, s2 = 0.f;

@@ -12,32 +12,6 @@ constexpr int kBM = 128, kBK = 64;
 constexpr int kMaxStages = 8, kSmemMost = 227 * 1024;
 
 __device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ uint64_t now_ns() {
-	uint64_t t;
-	asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-	return t;
-}
-// False when the phase has not completed after four seconds: nothing that a tile waits for takes a millisecond, and every copy that
-// was issued has landed long before a role gives up and the CTA ends.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
-	uint64_t start = 0;
-	for (uint32_t it = 0;; ++it) {
-		uint32_t ok;
-		asm volatile(
-		    "{\n\t.reg .pred p;\n\t"
-		    "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-		    "selp.u32 %0, 1, 0, p;\n\t}"
-		    : "=r"(ok)
-		    : "r"(bar), "r"(parity)
-		    : "memory");
-		if (ok) return true;
-		if ((it & 63u) == 63u) {
-			const uint64_t t = now_ns();
-			if (!start) start = t;
-			else if (t - start > 4000000000ull) return false;
-		}
-	}
-}
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
 	asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
