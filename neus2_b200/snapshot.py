@@ -47,6 +47,10 @@ def network_config(cfg):
     """The configuration object the snapshot is embedded in, with the reference's key names (configs/nerf/base.json,
     dtu.json)."""
     g = cfg.grid
+    hyperparams = {"batch_size": int(cfg.batch_size), "ek_loss_weight": float(cfg.ek_loss_weight),
+                   "mask_loss_weight": float(cfg.mask_loss_weight), "anneal_end": int(cfg.anneal_end)}
+    if cfg.max_grad_norm > 0:  # not a key of the reference: written where it is used
+        hyperparams["max_grad_norm"] = float(cfg.max_grad_norm)
     return {
         "encoding": {"otype": "HashGrid", "n_levels": int(g.n_levels), "n_features_per_level": 2,
                      "log2_hashmap_size": int(g.log2_hashmap_size), "base_resolution": int(g.base_resolution),
@@ -62,8 +66,7 @@ def network_config(cfg):
             "decay_base": float(cfg.lr_decay_base), "nested": {
                 "otype": "Adam", "learning_rate": float(cfg.learning_rate), "beta1": float(cfg.beta1), "beta2": float(cfg.beta2),
                 "epsilon": float(cfg.epsilon), "l2_reg": float(cfg.l2_reg)}}},
-        "hyperparams": {"batch_size": int(cfg.batch_size), "ek_loss_weight": float(cfg.ek_loss_weight),
-                        "mask_loss_weight": float(cfg.mask_loss_weight), "anneal_end": int(cfg.anneal_end)},
+        "hyperparams": hyperparams,
     }
 
 
