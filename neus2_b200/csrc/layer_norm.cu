@@ -605,6 +605,9 @@ __global__ void __launch_bounds__(1024) wide_params_kernel(uint32_t n, uint32_t 
 
 
 constexpr uint32_t kWidest = 8192;  // entries that a backward variant holds at most
+constexpr uint32_t kWidestUnaligned = 4096;  // of rows off 16-byte boundaries
+// Blocks a SM that a backward variant for rows of this width runs at most, whether they start on 16-byte boundaries or not.
+constexpr uint32_t most_blocks(uint32_t width) { return width <= 256 ? 8 : width <= 2048 ? 4 : width <= kWidestUnaligned ? 2 : 1; }
 constexpr int kTooWide = -1000;     // no variant holds the row
 
 template <typename T, int VEC, int TPR, int VPT>
@@ -771,8 +774,7 @@ extern "C" int neus2b_layer_norm_forward(const neus2b_layer_norm_desc* desc, con
 extern "C" int neus2b_layer_norm_backward_workspace(const neus2b_layer_norm_desc* desc, uint64_t* bytes) {
 	if (int rc = check_desc(desc)) return rc;
 	if (!bytes) return NEUS2B_E_INVALID;
-	// the most blocks that any variant runs
-	const uint64_t blocks = desc->n < 8u * kSMs ? desc->n : 8u * kSMs;
+	const uint64_t most = (uint64_t)kSMs * most_blocks(desc->width), blocks = desc->n < most ? desc->n : most;
 	*bytes = desc->width <= kWidest && desc->n > kFewRows ? blocks * 2 * desc->width * sizeof(float) : 0;
 	return NEUS2B_OK;
 }
@@ -801,6 +803,9 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 	    (d_skip && bad_rows(d_skip, skip_stride, width, b)) || (d_dL_dx && bad_rows(d_dL_dx, dx_stride, width, b)))
 		return NEUS2B_E_INVALID;
 	if ((d_dL_dx && d_dL_dx == d_x) || clash(d_dL_dx, dx_stride, d_dL_dy, dy_stride, n) || clash(d_dL_dx, dx_stride, d_skip, skip_stride, n)) return NEUS2B_E_INVALID;
+	const bool vec = rows16(d_x, x_stride, b) && rows16(d_dL_dy, dy_stride, b) && rows16(d_skip, skip_stride, b) && rows16(d_dL_dx, dx_stride, b) &&
+	                 width * b % 16 == 0;
+	if (!vec && width > kWidestUnaligned) need = 0;
 	if (need && (!d_workspace || ((uintptr_t)d_workspace & 15) || workspace_bytes < need)) return NEUS2B_E_INVALID;
 	return with_float_type(desc->dtype, [&](auto t) {
 		using T = decltype(t);
@@ -812,7 +817,7 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 		auto go = [&](auto v, auto ring) {
 			using K = decltype(v);
 			using B = Backward<K::kTpr, K::kVpt * K::kVec, decltype(ring)::value>;
-			static_assert(B::kGrid <= 8 * kSMs, "the workspace holds 8 blocks a SM");
+			static_assert(B::kGrid <= kSMs * (int)most_blocks(K::kTpr * K::kVpt * K::kVec), "the workspace holds the sums of every block");
 			const bool few = params && n <= kFewRows;
 			const uint32_t need = (n + B::kGroups - 1) / B::kGroups, most = few ? kCluster : (uint32_t)B::kGrid, blocks = need < most ? need : most;
 			constexpr size_t kSums = B::kGroups > 1 ? 2 * K::kVpt * K::kVec * B::kThreads * sizeof(float) : 0;
@@ -840,7 +845,6 @@ extern "C" int neus2b_layer_norm_backward(const neus2b_layer_norm_desc* desc, co
 			}
 			return NEUS2B_OK;
 		};
-		const bool vec = rows16(d_x, x_stride, b) && rows16(d_dL_dy, dy_stride, b) && rows16(d_skip, skip_stride, b) && rows16(d_dL_dx, dx_stride, b) && width % V == 0;
 		int rc = kTooWide;
 		if (vec && row >= kRingRow) rc = with_backward_ring<T, V>(width, [&](auto v) { return go(v, std::true_type()); });
 		if (rc == kTooWide) {
