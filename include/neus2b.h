@@ -128,7 +128,8 @@ typedef struct neus2b_motion neus2b_motion; /* dynamic sequences: the frame's le
 #define NEUS2B_MMA_TCGEN05 1
 int neus2b_set_mma_path(int path);
 int neus2b_get_mma_path(void);
-/* Sticky device-side error bits (bit 0: a bounded completion wait inside a tcgen05 kernel ran out). Synchronises. */
+/* Sticky device-side error bits of the current device (bit 0: a bounded wait inside a kernel ran out, for a tcgen05 completion or for a
+ * copy into shared memory). Synchronises. */
 int neus2b_device_error_flags(uint32_t* h_flags);
 /* Overwrites the sticky bits (0 clears them).  For hosts that recovered from an error, and for tests of the error path:
  * the training loop reports NEUS2B_E_DEVICE from its statistics call while a bit is set. */
@@ -368,7 +369,9 @@ int neus2b_delta_optimizer_step(const neus2b_adam_cfg* cfg, float* d_sums, float
  * Any width, stride and entry-aligned address is taken; rows that start on 16-byte boundaries are faster.  n == 0 is allowed.
  * Outputs may not overlap inputs unless a comment says so (then with the same stride).  At most 2^30 samples and entries a row
  * (layer norm: 2^31 samples).  Parameter gradients are fp32 and follow grad_mode
- * (NEUS2B_GRAD_*, IGNORE: the pointers are not used).  Every sum has a fixed order: the same call gives the same bits. */
+ * (NEUS2B_GRAD_*, IGNORE: the pointers are not used).  Every sum has a fixed order: the same call gives the same bits.
+ * The kernels' waits are bounded (four seconds).  A call only enqueues, so that it cannot report one that ran out: neus2b_device_error_flags
+ * is not 0 from then on, and what the calls since the last look at it wrote is void.  A host asks where it synchronises anyway. */
 #define NEUS2B_F32 0
 #define NEUS2B_F16 1
 #define NEUS2B_BF16 2

@@ -270,6 +270,8 @@ def adam_step_packed(cfg, grad_mlp, grad_grid, grad_var, state, params, params_e
 
 
 # ------------------------------------------------------------------------------------------------ layers of any width
+# The calls only enqueue.  A bounded wait inside a kernel that ran out shows in _lib.device_error_flags(), which synchronises: where it is not
+# 0, what the calls since the last look at it returned is void.
 _DTYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 
 
