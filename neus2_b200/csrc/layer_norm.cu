@@ -5,9 +5,9 @@
 // (and in the backward pass the sums for their gradients) stay on the SM over all rows of a group.  The variance is the mean square
 // of the centred row, not a difference of sums.
 //
-// Bound by memory where rows are wide (forward, 16384 rows of 4096 bf16: 54 us, 5.0 TB/s), by the instructions around a row where they are
-// short (262144 rows of 64 fp16: 14.1 us, 4.9 TB/s) and by launches and the join where they are few (backward, 8192 rows of 1024 bf16 with
-// a skip connection: 19.6 us of which the join takes 3.5; 33 rows of 1111 fp32: 4.3 us).
+// Bound by memory where rows are wide (forward, 16384 rows of 4096 bf16: 55 us, 4.9 TB/s), by the instructions around a row where they are
+// short (262144 rows of 64 fp16: 14.3 us, 4.8 TB/s) and by launches and the join where they are few (backward, 8192 rows of 1024 bf16 with
+// a skip connection: 19.9 us of which the join takes 3.5; 33 rows of 1111 fp32: 4.3 us).
 #include <type_traits>
 
 #include "dense.cuh"
@@ -508,7 +508,10 @@ __global__ void __launch_bounds__(1024) join_kernel(const float* __restrict__ pa
 	}
 }
 
-// ---- rows that do not fit into the registers of a block: read once for each sum and once for the result (from L2)
+// ---- rows that do not fit into the registers of a block: read once for each sum and once for the result (from L2), entry by entry.  Forward
+// these are rows above 8192 entries off 16-byte boundaries, and above 16384 on them; backward rows above 4096 entries
+// off the boundaries and above 8192 on them, where the parameters' sums take x and dL/dy a second time, 32 columns a block: 4096 x 12288
+// bf16 259 us, 4096 x 6001 fp16 129 us, five to six times the time of their bytes.
 
 // sum over the block, the same value in every thread
 __device__ __forceinline__ float block_sum(float v, float* s) {

@@ -125,9 +125,11 @@ __global__ void __launch_bounds__(256, 3) realign_kernel(const Realign r) {
 }
 
 // What a block of one variant is made of.  Large products are bound by the MMAs and the power they draw: 8192 x 4096 -> 4096 with bias, GELU and
-// residual 203 us, 1350 TFLOP/s of 1403 that a library product sustains; short k by the epilogue (8192 x 1024 -> 4096 with the slopes of a
-// GELU 67 us, 55 without; its chain of loads, MUFU and stores of 16 warps at 96 registers), small products by latency (100 x 256 -> 256 6.6 us, one row through 4096 -> 4096 9.8 us where its weights alone take
-// 5.1).  Tiles of 128 x 64 and 128 x 128 take their operands out of the L2 at about 45 bytes a cycle and SM.  PAIR: two CTAs of a cluster compute a 256 x BN tile together, each with 128 of its rows in its
+// residual takes 210 us in a burst, 1310 TFLOP/s of the 1679 that a library product reaches in one, and 236 to 247 us over seconds, 1110 to
+// 1165 of 1403 (the product alone 193 and 226, a library product of the shape 183 and 217); short k by the epilogue (8192 x 1024 -> 4096
+// with the slopes of a GELU 69 us, 59 without; its chain of loads, MUFU and stores of 16 warps at 96 registers), small products by latency
+// (100 x 256 -> 256 6.6 us, one row through 4096 -> 4096 10.4 us where its weights alone take 5.1).  Tiles of 128 x 64 and 128 x 128 take
+// their operands out of the L2 at about 45 bytes a cycle and SM.  PAIR: two CTAs of a cluster compute a 256 x BN tile together, each with 128 of its rows in its
 // tensor memory and half of B's tile in its shared memory.  The epilogue is a long chain of dependent steps, so that it takes 16 warps to
 // keep up with the MMAs: on wide tiles they share the columns, narrow ones (BN 64) go to four groups in turn, each with an accumulator.
 template <int BN, bool AMN, bool BMN, bool SWAP, bool WGRAD, bool PAIR>
