@@ -93,7 +93,10 @@ public:
 	                   GPUMatrixDynamic<T>* dL_dinput = nullptr, bool use_inference_params = false, EGradientMode param_gradients_mode = EGradientMode::Overwrite) override {
 		(void)output;
 		const uint32_t n = input.n();
-		if (!n) return;
+		if (!n) { /* the gradient of nothing is 0 */
+			if (param_gradients_mode == EGradientMode::Overwrite) CUDA_CHECK_THROW(cudaMemsetAsync(m_gradients, 0, n_params() * sizeof(T), stream));
+			return;
+		}
 #if defined(__CUDACC__)
 		const auto& f = dynamic_cast<const ForwardContext&>(ctx);
 		const T* p = use_inference_params ? m_inference_params : m_params;
